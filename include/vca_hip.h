@@ -515,6 +515,41 @@ int vca_adam_scaled_f32(long long n, float* p, const float* g, float* m, float* 
                         const float* scale, const int* flag, void* stream);
 int vca_loss_scale_update(float* scale, int* state, float growth, float backoff, int interval, void* stream);
 
+/* Element types of the entry points that take tensors of several. */
+#define VCA_T_F32 0
+#define VCA_T_BF16 1
+#define VCA_T_F16 2
+
+/* Global norm of ntensor gradient tensors and clipping by it (torch.nn.utils.clip_grad_norm_ with the 2-norm; the
+ * reference trains without clipping).  h_ptrs / h_numel / h_types are host arrays, read before the call returns:
+ * device pointer (aligned to its element), element count (0 allowed) and VCA_T_* of each tensor, taken as dense memory.
+ * scale: {s, 1/s} of a loss scaler whose factor the gradients carry, or NULL.  ws: at least
+ * vca_grad_norm_ws_doubles(ntensor) doubles, contents irrelevant, not shared by calls that may overlap in time.
+ *   vca_grad_norm   out[0] = sqrt(sum g^2) / s
+ *   vca_grad_clip   the same, then every g *= min(1, max_norm / (out[0] + 1e-6)) in place; the tensors must not overlap
+ * The sum is held in fp64 and in a fixed order: equal inputs give equal bits. */
+long long vca_grad_norm_ws_doubles(int ntensor);
+int vca_grad_norm(int ntensor, const void* const* h_ptrs, const long long* h_numel, const int* h_types,
+                  const float* scale, double* ws, long long ws_doubles, float* out, void* stream);
+int vca_grad_clip(int ntensor, const void* const* h_ptrs, const long long* h_numel, const int* h_types, float max_norm,
+                  const float* scale, double* ws, long long ws_doubles, float* out, void* stream);
+
+/* The Adam update of an optimizer's flat buffers (vca_adam_f32's arithmetic) on gradients clipped by their joint norm:
+ * g enters as g * min(1, max_norm / (norm + 1e-6)) / s and is not written.  Every buffer 16-byte aligned, n % 4 == 0.
+ * ++*step_dev happens inside; scale / flag (both or neither) are the loss scaler's: a gradient that is not finite sets
+ * *flag, and with *flag up nothing is updated and the count stays.  ws as above for ntensor = ngroup;
+ * out[4] = {norm, factor, learning rate / bias correction, root of the second bias correction}. */
+#define VCA_MAX_ADAM_GROUPS 32
+typedef struct {
+  float* p;
+  const float* g;
+  float *m, *v, *vmax;  /* vmax: NULL without amsgrad */
+  long long n;
+} vca_adam_group;
+int vca_adam_clip_f32(int ngroup, const vca_adam_group* h_groups, float max_norm, double beta1, double beta2,
+                      double eps, double weight_decay, int* step_dev, const float* lr_dev, const float* scale, int* flag,
+                      double* ws, long long ws_doubles, float* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(_HERE, 'libvca_hip.so')
 LIB_PATH_F16 = os.path.join(_HERE, 'libvca_hip_f16.so')
 ELEM = ['bf16']          # element type of the matrix products: 'bf16' or 'fp16' (set by ops.set_precision)
 SOURCES = ('conv_f32.hip', 'conv_bf16.hip', 'pointwise.hip', 'misc.hip', 'rnn.hip', 'attention.hip', 'stem.hip',
-           'sync_loss.hip', 'layout.hip', 'audio.hip', 'video.hip', 'ctc.hip', 'wgrad_cin1.hip', 'linear.hip')
+           'sync_loss.hip', 'layout.hip', 'audio.hip', 'video.hip', 'ctc.hip', 'wgrad_cin1.hip', 'linear.hip', 'gradnorm.hip')
 
 
 # Packed fp32 instructions stay off: on this part some of their forms, which the compiler makes out of ordinary float
@@ -88,9 +88,17 @@ class LossHeads(ctypes.Structure):
     _fields_ = [('nhead', ctypes.c_int), ('total_blocks', ctypes.c_int), ('h', LossHead * MAX_LOSS_HEADS)]
 
 
+class AdamGroup(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ('p', 'g', 'm', 'v', 'vmax')] + [('n', ctypes.c_longlong)]
+
+
+MAX_ADAM_GROUPS = 32
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # VCA_T_*
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_D = ctypes.c_double
 _LL = ctypes.c_longlong
 _SIGS = {
     'vca_abi_version': ([], _I),
@@ -177,6 +185,10 @@ _SIGS = {
     'vca_loss_scale_count': ([_P, _P, _P], _I),
     'vca_adam_scaled_f32': ([_LL, _P, _P, _P, _P, _P, _F, _F, _F, _F, _P, _P, _P, _P, _P], _I),
     'vca_loss_scale_update': ([_P, _P, _F, _F, _I, _P], _I),
+    'vca_grad_norm_ws_doubles': ([_I], _LL),
+    'vca_grad_norm': ([_I, _P, _P, _P, _P, _P, _LL, _P, _P], _I),
+    'vca_grad_clip': ([_I, _P, _P, _P, _F, _P, _P, _LL, _P, _P], _I),
+    'vca_adam_clip_f32': ([_I, _P, _F, _D, _D, _D, _D, _P, _P, _P, _P, _P, _LL, _P, _P], _I),
 }
 
 _libs = {}

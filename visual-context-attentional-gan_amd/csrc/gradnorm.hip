@@ -1,0 +1,507 @@
+// Global norm of many gradient tensors, clipping by it, and the Adam update that takes the clipping factor along.
+//
+//   norm = sqrt(sum over all tensors and elements of g^2) / loss scale
+//   c    = min(1, max_norm / (norm + 1e-6))           (a NaN norm gives a NaN factor, an infinite one the factor 0)
+//   clip:  g <- c g          Adam:  g' = c g / loss scale + wd p, then the usual moments and update
+//
+// All of it streams memory: the norm reads every byte once, clipping reads again and writes, the update reads p, g, m,
+// v (, vmax) and writes all but g.  Squares and sums are held in fp64: one conversion and one fp64 FMA per value are far
+// below what the vector units can do while the value arrives from HBM, no square over- or underflows for any fp32
+// gradient (so the sum is finite exactly when every gradient is, which the loss scaler's overflow test uses), and the
+// result is the exact sum to fp64 rounding.  No atomics: a list is cut into chunks, every chunk's sum goes to its own
+// workspace slot and the slots are added in a fixed order, so equal inputs give equal bits.
+//
+// The tensor table travels in the kernel arguments (TABLE tensors a launch), so nothing has to be uploaded, kept alive
+// or invalidated, and a captured launch carries its own copy.
+#include "common.h"
+
+namespace {
+
+constexpr int TABLE = 160;            // tensors a launch: 160 x 21 bytes of kernel arguments, under the 4 KB limit
+constexpr int THR = 256;
+constexpr int MAX_CHUNKS = 2048;      // chunks a list is cut into, not counting each tensor's last one: 8 workgroups a CU
+constexpr long long MIN_CHUNK = 16384;   // bytes: four 16-byte loads a thread
+constexpr int SMALL_WAVES = 16;
+constexpr long long SMALL_CHUNK = 4096;  // bytes a wave takes at a time in the single-workgroup form
+constexpr int SMALL_ITEMS = 64;          // chunks up to which one workgroup does everything
+
+struct Table {
+  const void* p[TABLE];
+  long long n[TABLE];                 // elements
+  int first[TABLE];                   // first chunk of tensor i
+  unsigned char type[TABLE];
+  int count, chunks, part0;           // tensors, chunks of this launch, workspace slot of its first chunk
+  long long chunk;                    // bytes a chunk
+};
+
+// The tensor that holds chunk b: the last one with first <= b (empty tensors are not in the table, so no two share a
+// `first`).  One load a lane instead of a search.
+__device__ __forceinline__ int tensor_of(const Table& t, int b) {
+  const int lane = threadIdx.x & 63;
+  int k = 0;
+#pragma unroll
+  for (int j = 0; j < (TABLE + 63) / 64; ++j) {
+    const int i = j * 64 + lane;
+    const bool le = i < t.count && t.first[i < TABLE ? i : 0] <= b;
+    k += __popcll(__ballot(le));
+  }
+  return __builtin_amdgcn_readfirstlane(k - 1);
+}
+
+template <typename T> struct Vec;     // a 16-byte piece
+template <> struct Vec<float> { static constexpr int N = 4; };
+template <> struct Vec<__bf16> { static constexpr int N = 8; };
+template <> struct Vec<_Float16> { static constexpr int N = 8; };
+
+template <typename T> union Piece {
+  uint4 u;
+  T e[16 / sizeof(T)];
+};
+
+// The part of one chunk that lies in 16-byte pieces, and the elements before the tensor's first and behind its last
+// whole piece.  Offsets are bytes from the tensor's start rounded down to 16, so every piece is aligned whatever the
+// tensor's own alignment, and no byte outside the tensor is touched.
+struct Span {
+  long long v0, v1;                   // pieces [v0, v1)
+  long long h0, h1, t0, t1;           // single elements [h0, h1) and [t0, t1), as byte offsets
+};
+
+__device__ __forceinline__ Span span_of(const void* p, long long n, int esz, long long c, long long chunk) {
+  const long long beg = (long long)(reinterpret_cast<uintptr_t>(p) & 15), end = beg + n * esz;
+  const long long lo = c * chunk, hi = min(lo + chunk, end);
+  long long vf = (beg + 15) >> 4, vl = end >> 4;    // the tensor's whole pieces
+  Span s;
+  s.h0 = s.h1 = s.t0 = s.t1 = 0;
+  if (vf > vl) {                      // the tensor lies inside one piece
+    s.v0 = s.v1 = 0;
+    s.h0 = beg;
+    s.h1 = end;
+    return s;
+  }
+  s.v0 = max(vf, lo >> 4);
+  s.v1 = min(vl, (lo + chunk) >> 4);
+  if (c == 0 && beg) {
+    s.h0 = beg;
+    s.h1 = vf << 4;
+  }
+  if (hi == end && (end & 15)) {
+    s.t0 = vl << 4;
+    s.t1 = end;
+  }
+  return s;
+}
+
+template <typename T, int NT>
+__device__ __forceinline__ double sumsq(const void* p, long long n, long long c, long long chunk, int tid) {
+  const char* base = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
+  const Span s = span_of(p, n, sizeof(T), c, chunk);
+  constexpr int N = Vec<T>::N;
+  double a0 = 0., a1 = 0.;
+  auto add = [&](const uint4& u) {
+    Piece<T> q;
+    q.u = u;
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const double x = (double)(float)q.e[e], y = (double)(float)q.e[e + 1];
+      a0 = fma(x, x, a0);
+      a1 = fma(y, y, a1);
+    }
+  };
+  const uint4* v = reinterpret_cast<const uint4*>(base);
+  long long i = s.v0 + tid;
+  for (; i + 3 * NT < s.v1; i += 4 * NT) {          // four pieces in flight a thread
+    const uint4 u0 = v[i], u1 = v[i + NT], u2 = v[i + 2 * NT], u3 = v[i + 3 * NT];
+    add(u0);
+    add(u1);
+    add(u2);
+    add(u3);
+  }
+  for (; i < s.v1; i += NT) add(v[i]);
+  auto single = [&](long long b, long long e) {
+    const long long o = b + (long long)tid * sizeof(T);
+    if (o < e) {
+      const double x = (double)(float)*reinterpret_cast<const T*>(base + o);
+      a0 = fma(x, x, a0);
+    }
+  };
+  single(s.h0, s.h1);                 // at most 15 elements: fewer than the threads
+  single(s.t0, s.t1);
+  return a0 + a1;
+}
+
+template <typename T, int NT>
+__device__ __forceinline__ void scale_by(void* p, long long n, long long c, long long chunk, int tid, float f) {
+  char* base = reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
+  const Span s = span_of(p, n, sizeof(T), c, chunk);
+  constexpr int N = Vec<T>::N;
+  auto mul = [&](const uint4& u) {
+    Piece<T> q;
+    q.u = u;
+#pragma unroll
+    for (int e = 0; e < N; ++e) q.e[e] = (T)((float)q.e[e] * f);
+    return q.u;
+  };
+  uint4* v = reinterpret_cast<uint4*>(base);
+  long long i = s.v0 + tid;
+  for (; i + 3 * NT < s.v1; i += 4 * NT) {
+    const uint4 u0 = v[i], u1 = v[i + NT], u2 = v[i + 2 * NT], u3 = v[i + 3 * NT];
+    v[i] = mul(u0);
+    v[i + NT] = mul(u1);
+    v[i + 2 * NT] = mul(u2);
+    v[i + 3 * NT] = mul(u3);
+  }
+  for (; i < s.v1; i += NT) v[i] = mul(v[i]);
+  auto single = [&](long long b, long long e) {
+    const long long o = b + (long long)tid * sizeof(T);
+    if (o < e) {
+      T* q = reinterpret_cast<T*>(base + o);
+      *q = (T)((float)*q * f);
+    }
+  };
+  single(s.h0, s.h1);
+  single(s.t0, s.t1);
+}
+
+template <int NT>
+__device__ __forceinline__ double chunk_sumsq(const Table& t, int b, int tid) {
+  const int k = tensor_of(t, b);
+  const int c = b - t.first[k];
+  if (t.type[k] == VCA_T_F32) return sumsq<float, NT>(t.p[k], t.n[k], c, t.chunk, tid);
+  if (t.type[k] == VCA_T_BF16) return sumsq<__bf16, NT>(t.p[k], t.n[k], c, t.chunk, tid);
+  return sumsq<_Float16, NT>(t.p[k], t.n[k], c, t.chunk, tid);
+}
+
+template <int NT>
+__device__ __forceinline__ void chunk_scale(const Table& t, int b, int tid, float f) {
+  const int k = tensor_of(t, b);
+  const int c = b - t.first[k];
+  void* p = const_cast<void*>(t.p[k]);
+  if (t.type[k] == VCA_T_F32) scale_by<float, NT>(p, t.n[k], c, t.chunk, tid, f);
+  else if (t.type[k] == VCA_T_BF16) scale_by<__bf16, NT>(p, t.n[k], c, t.chunk, tid, f);
+  else scale_by<_Float16, NT>(p, t.n[k], c, t.chunk, tid, f);
+}
+
+__device__ __forceinline__ double wave_sum_d(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// Sum over a workgroup of NW waves, in every thread; the same order of additions in every workgroup.
+template <int NW>
+__device__ __forceinline__ double block_sum_d(double v, double* part) {
+  v = wave_sum_d(v);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double t = 0.;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) t += part[i];
+  return t;
+}
+
+// norm and clipping factor from the sum of squares of the gradients as stored (scale: {s, 1/s} or null)
+__device__ __forceinline__ double true_norm(double total, const float* scale) {
+  return sqrt(total) * (scale ? (double)scale[1] : 1.);
+}
+
+__device__ __forceinline__ float clip_factor(double norm, float max_norm) {
+  const double c = (double)max_norm / (norm + 1e-6);
+  return c >= 1. ? 1.f : (float)c;    // a NaN stays one
+}
+
+__global__ __launch_bounds__(THR) void norm_chunks_kernel(const Table t, double* __restrict__ ws) {
+  __shared__ double part[THR / 64];
+  const double v = block_sum_d<THR / 64>(chunk_sumsq<THR>(t, blockIdx.x, threadIdx.x), part);
+  if (threadIdx.x == 0) ws[t.part0 + blockIdx.x] = v;
+}
+
+__device__ __forceinline__ double fold(const double* __restrict__ ws, int n, double* part) {
+  double a = 0.;
+  for (int i = threadIdx.x; i < n; i += THR) a += ws[i];
+  return block_sum_d<THR / 64>(a, part);
+}
+
+__global__ __launch_bounds__(THR) void norm_fold_kernel(const double* __restrict__ ws, int n,
+                                                        const float* __restrict__ scale, float* __restrict__ out) {
+  __shared__ double part[THR / 64];
+  const double total = fold(ws, n, part);
+  if (threadIdx.x == 0) out[0] = (float)true_norm(total, scale);
+}
+
+// Every workgroup adds up the slots itself (at most some 2200 values out of L2, under the time of one more launch)
+// and scales its chunk; with a factor of one there is nothing to do.  Chunks are taken from the last to the first: the
+// norm's pass left the end of the list in the caches.
+__global__ __launch_bounds__(THR) void clip_chunks_kernel(const Table t, const double* __restrict__ ws, int n,
+                                                          float max_norm, const float* __restrict__ scale,
+                                                          float* __restrict__ out) {
+  __shared__ double part[THR / 64];
+  const double norm = true_norm(fold(ws, n, part), scale);
+  if (out && blockIdx.x == 0 && threadIdx.x == 0) out[0] = (float)norm;
+  const float f = clip_factor(norm, max_norm);
+  if (f == 1.f) return;
+  chunk_scale<THR>(t, t.chunks - 1 - (int)blockIdx.x, threadIdx.x, f);
+}
+
+// Short lists: one workgroup whose waves take chunks in turn, so that norm and clipping are a single launch.
+template <bool CLIP>
+__global__ __launch_bounds__(SMALL_WAVES * 64) void norm_small_kernel(const Table t, float max_norm,
+                                                                      const float* __restrict__ scale,
+                                                                      float* __restrict__ out) {
+  __shared__ double part[SMALL_WAVES];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  double a = 0.;
+  for (int b = wave; b < t.chunks; b += SMALL_WAVES) a += chunk_sumsq<64>(t, b, lane);
+  const double norm = true_norm(block_sum_d<SMALL_WAVES>(a, part), scale);
+  if (threadIdx.x == 0) out[0] = (float)norm;
+  if (!CLIP) return;
+  const float f = clip_factor(norm, max_norm);
+  if (f == 1.f) return;
+  for (int b = wave; b < t.chunks; b += SMALL_WAVES) chunk_scale<64>(t, b, lane, f);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Adam with the clipping factor
+// ---------------------------------------------------------------------------------------------------------------
+struct Groups {
+  vca_adam_group g[VCA_MAX_ADAM_GROUPS];
+  int first[VCA_MAX_ADAM_GROUPS];     // first workgroup of group i
+  int count;
+  long long chunk4;                   // float4s a workgroup
+};
+
+struct AdamCfg {
+  float b1, b2, omb1, omb2, eps, wd;  // omb = 1 - beta, rounded once (1.f - 0.999f is off by 1e-5 of itself)
+  double b1d, b2d;
+};
+
+// out: {norm, c / loss scale, learning rate / (1 - b1^t), sqrt(1 - b2^t)}.  With a scaler a gradient that is not finite
+// raises the flag and the step count stays.
+__global__ __launch_bounds__(THR) void adam_words_kernel(const double* __restrict__ ws, int n, float max_norm,
+                                                         const float* __restrict__ scale, int* __restrict__ flag,
+                                                         int* __restrict__ step_dev, const float* __restrict__ lr_dev,
+                                                         AdamCfg cfg, float* __restrict__ out) {
+  __shared__ double part[THR / 64];
+  const double total = fold(ws, n, part);
+  if (threadIdx.x) return;
+  const double norm = true_norm(total, scale);
+  out[0] = (float)norm;
+  out[1] = clip_factor(norm, max_norm) * (scale ? scale[1] : 1.f);
+  if (flag && (flag[0] || !isfinite(total))) {
+    flag[0] = 1;
+    return;
+  }
+  const int step = step_dev[0] + 1;
+  step_dev[0] = step;
+  const double t = (double)step;
+  out[2] = (float)((double)lr_dev[0] / (1. - pow(cfg.b1d, t)));
+  out[3] = (float)sqrt(1. - pow(cfg.b2d, t));
+}
+
+__device__ __forceinline__ void adam4(float4& P, const float4& G, float4& M, float4& V, float4& X, bool ams,
+                                      const AdamCfg& c, float f, float step, float root) {
+  float* pp = &P.x;
+  const float* gg = &G.x;
+  float *mm = &M.x, *vv = &V.x, *xx = &X.x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float gr = gg[j] * f + c.wd * pp[j];
+    mm[j] = c.b1 * mm[j] + c.omb1 * gr;
+    vv[j] = c.b2 * vv[j] + c.omb2 * gr * gr;
+    float q = vv[j];
+    if (ams) q = xx[j] = fmaxf(xx[j], vv[j]);
+    pp[j] -= step * mm[j] / (sqrtf(q) / root + c.eps);
+  }
+}
+
+__global__ __launch_bounds__(THR) void adam_clip_kernel(const Groups t, const AdamCfg cfg, const int* __restrict__ flag,
+                                                        const float* __restrict__ words) {
+  if (flag && flag[0]) return;
+  int k = 0;
+  for (int i = 1; i < t.count; ++i)
+    if (t.first[i] <= (int)blockIdx.x) k = i;
+  const vca_adam_group g = t.g[k];
+  const float f = words[1], step = words[2], root = words[3];
+  const bool ams = g.vmax != nullptr;
+  const long long n4 = g.n >> 2, lo = (long long)(blockIdx.x - t.first[k]) * t.chunk4, hi = min(lo + t.chunk4, n4);
+  float4 *p = reinterpret_cast<float4*>(g.p), *m = reinterpret_cast<float4*>(g.m), *v = reinterpret_cast<float4*>(g.v),
+         *x = reinterpret_cast<float4*>(g.vmax);
+  const float4* gr = reinterpret_cast<const float4*>(g.g);
+  for (long long i = lo + threadIdx.x; i < hi; i += THR) {
+    float4 P = p[i], M = m[i], V = v[i], X = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 G = gr[i];
+    if (ams) X = x[i];
+    adam4(P, G, M, V, X, ams, cfg, f, step, root);
+    p[i] = P;
+    m[i] = M;
+    v[i] = V;
+    if (ams) x[i] = X;
+  }
+}
+
+int type_size(int t) { return t == VCA_T_F32 ? 4 : (t == VCA_T_BF16 || t == VCA_T_F16) ? 2 : 0; }
+
+// Checks a list and finds its bytes; false for one that no kernel may see.
+bool list_ok(int n, const void* const* p, const long long* numel, const int* type, long long& bytes) {
+  if (n < 0 || (n && (!p || !numel || !type))) return false;
+  bytes = 0;
+  for (int i = 0; i < n; ++i) {
+    const int e = type_size(type[i]);
+    if (!e || numel[i] < 0 || numel[i] > (1ll << 46)) return false;
+    if (numel[i] && (!p[i] || (reinterpret_cast<uintptr_t>(p[i]) & (e - 1)))) return false;
+    bytes += numel[i] * e;
+  }
+  return true;
+}
+
+long long chunks_of(const void* p, long long numel, int e, long long chunk) {
+  if (!numel) return 0;
+  return ((long long)(reinterpret_cast<uintptr_t>(p) & 15) + numel * e + chunk - 1) / chunk;
+}
+
+long long chunk_bytes(long long bytes) {
+  const long long c = (bytes / MAX_CHUNKS + MIN_CHUNK - 1) / MIN_CHUNK * MIN_CHUNK;
+  return c < MIN_CHUNK ? MIN_CHUNK : c;
+}
+
+// Fills a launch's table with the list's tensors from i on (empty ones are left out); returns the next tensor.
+int fill(Table& t, int i, int n, const void* const* p, const long long* numel, const int* type, long long chunk,
+         int part0) {
+  t.count = t.chunks = 0;
+  t.part0 = part0;
+  t.chunk = chunk;
+  for (; i < n && t.count < TABLE; ++i) {
+    const long long c = chunks_of(p[i], numel[i], type_size(type[i]), chunk);
+    if (!c) continue;
+    t.p[t.count] = p[i];
+    t.n[t.count] = numel[i];
+    t.type[t.count] = (unsigned char)type[i];
+    t.first[t.count] = t.chunks;
+    t.chunks += (int)c;
+    ++t.count;
+  }
+  return i;
+}
+
+long long total_chunks(int n, const void* const* p, const long long* numel, const int* type, long long chunk) {
+  long long c = 0;
+  for (int i = 0; i < n; ++i) c += chunks_of(p[i], numel[i], type_size(type[i]), chunk);
+  return c;
+}
+
+// Launches the partial sums of a list; parts = slots written.
+int norm_partials(int n, const void* const* p, const long long* numel, const int* type, long long bytes, double* ws,
+                  long long ws_doubles, hipStream_t s, int& parts) {
+  const long long chunk = chunk_bytes(bytes);
+  const long long need = total_chunks(n, p, numel, type, chunk);
+  VCA_CHECK_ARG(need <= ws_doubles && (need == 0 || (ws && (reinterpret_cast<uintptr_t>(ws) & 7) == 0)));
+  parts = 0;
+  Table t;
+  for (int i = 0; i < n;) {
+    i = fill(t, i, n, p, numel, type, chunk, parts);
+    if (t.chunks) hipLaunchKernelGGL(norm_chunks_kernel, dim3(t.chunks), dim3(THR), 0, s, t, ws);
+    parts += t.chunks;
+  }
+  return vca_launch_status();
+}
+
+// One workgroup is enough: the whole list in one table and few chunks.
+bool small_list(int n, const void* const* p, const long long* numel, const int* type, Table& t) {
+  if (total_chunks(n, p, numel, type, SMALL_CHUNK) > SMALL_ITEMS) return false;
+  return fill(t, 0, n, p, numel, type, SMALL_CHUNK, 0) == n;
+}
+
+}  // namespace
+
+extern "C" long long vca_grad_norm_ws_doubles(int ntensor) { return ntensor < 0 ? 0 : (long long)MAX_CHUNKS + 2ll * ntensor; }
+
+extern "C" int vca_grad_norm(int ntensor, const void* const* h_ptrs, const long long* h_numel, const int* h_types,
+                             const float* scale, double* ws, long long ws_doubles, float* out, void* stream) {
+  long long bytes = 0;
+  VCA_CHECK_ARG(out && list_ok(ntensor, h_ptrs, h_numel, h_types, bytes));
+  hipStream_t s = (hipStream_t)stream;
+  Table t;
+  if (small_list(ntensor, h_ptrs, h_numel, h_types, t)) {
+    hipLaunchKernelGGL(norm_small_kernel<false>, dim3(1), dim3(SMALL_WAVES * 64), 0, s, t, 0.f, scale, out);
+    return vca_launch_status();
+  }
+  int parts = 0;
+  const int rc = norm_partials(ntensor, h_ptrs, h_numel, h_types, bytes, ws, ws_doubles, s, parts);
+  if (rc) return rc;
+  hipLaunchKernelGGL(norm_fold_kernel, dim3(1), dim3(THR), 0, s, ws, parts, scale, out);
+  return vca_launch_status();
+}
+
+extern "C" int vca_grad_clip(int ntensor, const void* const* h_ptrs, const long long* h_numel, const int* h_types,
+                             float max_norm, const float* scale, double* ws, long long ws_doubles, float* out,
+                             void* stream) {
+  long long bytes = 0;
+  VCA_CHECK_ARG(out && max_norm >= 0.f && list_ok(ntensor, h_ptrs, h_numel, h_types, bytes));
+  hipStream_t s = (hipStream_t)stream;
+  Table t;
+  if (small_list(ntensor, h_ptrs, h_numel, h_types, t)) {
+    hipLaunchKernelGGL(norm_small_kernel<true>, dim3(1), dim3(SMALL_WAVES * 64), 0, s, t, max_norm, scale, out);
+    return vca_launch_status();
+  }
+  int parts = 0;
+  const int rc = norm_partials(ntensor, h_ptrs, h_numel, h_types, bytes, ws, ws_doubles, s, parts);
+  if (rc) return rc;
+  const long long chunk = chunk_bytes(bytes);
+  bool first = true;
+  for (int i = 0; i < ntensor;) {
+    i = fill(t, i, ntensor, h_ptrs, h_numel, h_types, chunk, 0);
+    if (!t.chunks) continue;
+    hipLaunchKernelGGL(clip_chunks_kernel, dim3(t.chunks), dim3(THR), 0, s, t, ws, parts, max_norm, scale,
+                       first ? out : nullptr);
+    first = false;
+  }
+  return vca_launch_status();
+}
+
+extern "C" int vca_adam_clip_f32(int ngroup, const vca_adam_group* h_groups, float max_norm, double beta1, double beta2,
+                                 double eps, double weight_decay, int* step_dev, const float* lr_dev,
+                                 const float* scale, int* flag, double* ws, long long ws_doubles, float* out,
+                                 void* stream) {
+  VCA_CHECK_ARG(ngroup >= 1 && ngroup <= VCA_MAX_ADAM_GROUPS && h_groups && max_norm >= 0.f && step_dev && lr_dev && out);
+  VCA_CHECK_ARG(!scale == !flag);
+  const void* p[VCA_MAX_ADAM_GROUPS];
+  long long numel[VCA_MAX_ADAM_GROUPS], total = 0;
+  int type[VCA_MAX_ADAM_GROUPS];
+  Groups t;
+  t.count = ngroup;
+  for (int i = 0; i < ngroup; ++i) {
+    const vca_adam_group& g = h_groups[i];
+    VCA_CHECK_ARG(g.n > 0 && (g.n % 4) == 0 && g.n <= (1ll << 44) && g.p && g.g && g.m && g.v);
+    VCA_CHECK_ARG(((reinterpret_cast<uintptr_t>(g.p) | reinterpret_cast<uintptr_t>(g.g) | reinterpret_cast<uintptr_t>(g.m) |
+                    reinterpret_cast<uintptr_t>(g.v) | reinterpret_cast<uintptr_t>(g.vmax)) & 15) == 0);
+    p[i] = g.g;
+    numel[i] = g.n;
+    type[i] = VCA_T_F32;
+    t.g[i] = g;
+    total += g.n;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  int parts = 0;
+  const int rc = norm_partials(ngroup, p, numel, type, total * 4, ws, ws_doubles, s, parts);
+  if (rc) return rc;
+  AdamCfg cfg;
+  cfg.b1 = (float)beta1;
+  cfg.b2 = (float)beta2;
+  cfg.omb1 = (float)(1. - beta1);
+  cfg.omb2 = (float)(1. - beta2);
+  cfg.eps = (float)eps;
+  cfg.wd = (float)weight_decay;
+  cfg.b1d = beta1;
+  cfg.b2d = beta2;
+  hipLaunchKernelGGL(adam_words_kernel, dim3(1), dim3(THR), 0, s, ws, parts, max_norm, scale, flag, step_dev, lr_dev, cfg,
+                     out);
+  // 4 float4s a thread, more where the list is so long that this would be over 16384 workgroups
+  t.chunk4 = 4 * THR;
+  while ((total / 4) / t.chunk4 > 16384) t.chunk4 *= 2;
+  int blocks = 0;
+  for (int i = 0; i < ngroup; ++i) {
+    t.first[i] = blocks;
+    blocks += (int)((numel[i] / 4 + t.chunk4 - 1) / t.chunk4);
+  }
+  hipLaunchKernelGGL(adam_clip_kernel, dim3(blocks), dim3(THR), 0, s, t, cfg, flag, out);
+  return vca_launch_status();
+}

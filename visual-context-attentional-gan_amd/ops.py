@@ -2111,6 +2111,120 @@ class LossScaler:
         return int(self.state[3])
 
 
+class GradNorm:
+    """Global 2-norm of a fixed list of gradient tensors, and clipping by it (torch.nn.utils.clip_grad_norm_'s
+    semantics, on gradient tensors instead of parameters).  Build it once for gradients that stay where they are
+    (flatten_module's views, buckets) and call norm() or clip_() every step; grad_norm() and clip_grad_norm_() below are
+    the same for a list that is used once.
+
+    tensors: fp32 / bf16 / fp16 in any mixture, any sizes (empty ones too), any alignment, dense (contiguous up to a
+    permutation of the dimensions), all on one device.  The object holds references to them, so their memory stays
+    valid; it does not notice when a parameter is given another .grad.
+
+    norm and clip_ return the norm before clipping as a 0-dim fp32 device tensor, without a host synchronisation; both
+    can be captured into a HIP graph, and two calls may run on two streams at once (each has its own workspace) as far
+    as the tensors themselves allow it.  scaler: a LossScaler whose factor the gradients carry; the norm returned and
+    compared with max_norm is then that of the unscaled gradients, while clip_ leaves them scaled.  A gradient that is
+    not finite makes the norm so: with an infinite norm clip_ multiplies by 0, with a NaN by NaN, as torch does."""
+
+    def __init__(self, tensors):
+        self.tensors = ts = list(tensors)
+        if not ts:
+            raise ValueError('GradNorm: no tensors')
+        dev = ts[0].device
+        for t in ts:
+            if isinstance(t, torch.nn.Parameter):
+                raise TypeError('GradNorm takes gradients, not parameters: pass [p.grad for p in ...]')
+            if not t.is_cuda or t.device != dev:
+                raise ValueError('GradNorm: all tensors must be on one GPU, got %s and %s' % (dev, t.device))
+            if t.dtype not in _lib.TYPES:
+                raise TypeError('GradNorm: fp32, bf16 or fp16 tensors, got %s' % t.dtype)
+            if not _dense(t):
+                raise ValueError('GradNorm: a tensor of shape %s and strides %s is not dense memory'
+                                 % (tuple(t.shape), t.stride()))
+        n = len(ts)
+        self.device = dev
+        self._n = n
+        self._ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in ts])
+        self._numel = (ctypes.c_longlong * n)(*[t.numel() for t in ts])
+        self._types = (ctypes.c_int * n)(*[_lib.TYPES[t.dtype] for t in ts])
+        self._ws = int(_lib.lib().vca_grad_norm_ws_doubles(n))
+        self._disjoint = None
+
+    def norm(self, scaler=None):
+        """sqrt(sum of squares of all elements) (divided by the loss scale)."""
+        with _on_device(self.device):
+            out, ws = self._buffers()
+            check(_lib.lib().vca_grad_norm(self._n, self._ptrs, self._numel, self._types,
+                                           None if scaler is None else ptr(scaler.scale), ws.data_ptr(), self._ws,
+                                           out.data_ptr(), stream()), 'grad_norm')
+        return out
+
+    def clip_(self, max_norm, scaler=None):
+        """Scale every tensor in place by min(1, max_norm / (norm + 1e-6)) and return the norm."""
+        max_norm = _max_norm(max_norm)
+        if self._disjoint is None:
+            at = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in self.tensors if t.numel())
+            self._disjoint = all(a + n <= b for (a, n), (b, _) in zip(at, at[1:]))
+        if not self._disjoint:
+            raise ValueError('GradNorm.clip_: two of the tensors share memory (the same gradient twice?)')
+        with _on_device(self.device):
+            out, ws = self._buffers()
+            check(_lib.lib().vca_grad_clip(self._n, self._ptrs, self._numel, self._types, max_norm,
+                                           None if scaler is None else ptr(scaler.scale), ws.data_ptr(), self._ws,
+                                           out.data_ptr(), stream()), 'grad_clip')
+        torch.autograd.graph.increment_version(self.tensors)
+        return out
+
+    def _buffers(self):
+        return (torch.empty((), device=self.device, dtype=torch.float32),
+                torch.empty(self._ws, device=self.device, dtype=torch.float64))
+
+
+def grad_norm(tensors, scaler=None):
+    """Global 2-norm of a list of gradient tensors; see GradNorm."""
+    return GradNorm(tensors).norm(scaler)
+
+
+def clip_grad_norm_(tensors, max_norm, scaler=None):
+    """Clip a list of gradient tensors in place by their global 2-norm and return it; see GradNorm."""
+    return GradNorm(tensors).clip_(max_norm, scaler)
+
+
+def _max_norm(v):
+    v = float(v)
+    if not v >= 0.0:
+        raise ValueError('max_norm must not be negative or NaN, got %r' % v)
+    return v
+
+
+def _dense(t):
+    """Whether t's elements fill one contiguous range of memory, in whatever order of dimensions."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if st != want:
+            return False
+        want *= n
+    return True
+
+
+class _on_device:
+    """Make `device` current for the enclosed launches (which go to its current stream); free where it is already."""
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
 class FusedAdam:
     """torch.optim.Adam semantics (coupled L2 weight decay, optional amsgrad; train.py:82-83) as one kernel launch
     per flat buffer.  `groups` is a list of (flat_params, flat_grads) from flatten_module.
@@ -2146,12 +2260,26 @@ class FusedAdam:
             self.lr_dev.copy_(torch.full((1,), lr, dtype=torch.float32), non_blocking=False)
             self._lr_written = lr
 
-    def step(self, scaler=None, side=0):
+    def step(self, scaler=None, side=0, max_norm=None):
         """scaler: a LossScaler whose scale the gradients carry; side: 0 / 1, which of its overflow flags this
         optimizer raises (discriminator / generator side).  With a scaler the step is skipped on the device when any
-        gradient is Inf / NaN (parameters, moments and the step count stay)."""
+        gradient is Inf / NaN (parameters, moments and the step count stay).
+
+        max_norm: clip by the global norm of all groups' (unscaled) gradients.  The factor min(1, max_norm /
+        (norm + 1e-6)) enters the update where the gradients are read, so clipping costs one read of them and no write
+        (they stay as they are); with a scaler that read is also the overflow test.  Returns the norm as a 0-dim
+        device tensor (None without max_norm)."""
+        if max_norm is not None:
+            max_norm = _max_norm(max_norm)
+            if len(self.groups) > _lib.MAX_ADAM_GROUPS:
+                raise ValueError('FusedAdam.step: max_norm takes at most %d groups' % _lib.MAX_ADAM_GROUPS)
         if not torch.cuda.is_current_stream_capturing():
             self.sync_lr()
+        if max_norm is not None:
+            with _on_device(self.t_dev.device):
+                norm = self._clipped(scaler, side, max_norm)
+            self._stepped()
+            return norm
         L = _lib.lib()
         if scaler is not None:
             flag = scaler.state.data_ptr() + 4 * (1 + side)
@@ -2173,6 +2301,27 @@ class FusedAdam:
                 check(L.vca_adam_f32(f.numel(), ptr(f), ptr(g), ptr(st['m']), ptr(st['v']), ptr(st['vmax']), lr,
                                      self.betas[0], self.betas[1], self.eps, self.weight_decay, self.t,
                                      self.t_dev.data_ptr(), self.lr_dev.data_ptr(), stream()), 'adam')
+        self._stepped()
+
+    def _clipped(self, scaler, side, max_norm):
+        L = _lib.lib()
+        n = len(self.groups)
+        tab = (_lib.AdamGroup * n)(*[(ptr(f), ptr(g), ptr(st['m']), ptr(st['v']), ptr(st['vmax']), f.numel())
+                                     for (f, g), st in zip(self.groups, self.state)])
+        nws = int(L.vca_grad_norm_ws_doubles(n))
+        dev = self.t_dev.device
+        ws = torch.empty(nws, device=dev, dtype=torch.float64)
+        out = torch.empty(4, device=dev, dtype=torch.float32)
+        check(L.vca_adam_clip_f32(n, tab, max_norm, self.betas[0], self.betas[1], self.eps, self.weight_decay,
+                                  self.t_dev.data_ptr(), self.lr_dev.data_ptr(),
+                                  None if scaler is None else ptr(scaler.scale),
+                                  None if scaler is None else scaler.state.data_ptr() + 4 * (1 + side),
+                                  ws.data_ptr(), nws, out.data_ptr(), stream()), 'adam_clip')
+        self.t += 1
+        return out[0]
+
+    def _stepped(self):
+        for f, _ in self.groups:
             ep = _flat_epoch.get(f.data_ptr())
             if ep is not None:
                 ep[0] += 1

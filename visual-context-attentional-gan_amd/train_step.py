@@ -112,8 +112,12 @@ class GanStep:
     """Callable running one full G+D step; variant 'grid' = train.py, 'lrs' = train_LRS.py."""
 
     def __init__(self, models, optimizers, variant='grid', group=None, force_exchange=False, ctc=None, overlap=None,
-                 scaler=None):
-        """scaler: an ops.LossScaler; required (and created by default) when the precision mode computes gradients in
+                 scaler=None, max_norm=None):
+        """max_norm: clip each side's gradients by their global norm in front of its optimizer step: a number for both
+        sides or a pair (generator side, discriminator side), None in the pair for a side that is not clipped.  The
+        norms before clipping are returned as g_norm / d_norm (under data parallelism those of the reduced gradients,
+        equal on every rank).
+        scaler: an ops.LossScaler; required (and created by default) when the precision mode computes gradients in
         IEEE half ('fp16', 'fp16-mixed', 'fp16x3'; BASELINE configs[4] "fp16 with loss-scaling"): both backward passes
         are seeded with the scale, the optimizers divide it out and skip their step on overflow, the scale adapts at
         the end of every step.  The reported losses are unscaled.
@@ -143,6 +147,7 @@ class GanStep:
         if scaler is None and ops.half_gradients():
             scaler = ops.LossScaler(next(models['gen'].parameters()).device)
         self.scaler = scaler
+        self.g_max_norm, self.d_max_norm = max_norm if isinstance(max_norm, (tuple, list)) else (max_norm, max_norm)
         if dist.is_available() and dist.is_initialized():
             ops.set_seed(torch.initial_seed(), dist.get_rank(group))   # each replica draws its own dropout masks
 
@@ -335,7 +340,7 @@ class GanStep:
         """d_optimizer.step(), the generator losses and their backward pass; with overlap the pass ends at the phoneme
         features and g_trunk() takes it through the visual front-end."""
         m, st = self.m, self._st
-        self.d_opt.step(self.scaler, 0)
+        d_norm = self.d_opt.step(self.scaler, 0, self.d_max_norm)
         g1, g2, g3 = st['g']
         phon, sd, T = st['phon'], st['sd'], st['T']
         dis = (m['dis1'], m['dis2'], m['dis3'])
@@ -392,6 +397,8 @@ class GanStep:
                         grad_p=st['grad_p'], g1=g1.detach(), g2=g2.detach(), g3=g3.detach(), gs=gs.detach())
         if self.ctc is not None:
             self._st['ctc_loss'] = out[4]
+        if d_norm is not None:
+            self._st['d_norm'] = d_norm
         self._cut = cut
 
     def g_trunk(self):
@@ -407,7 +414,9 @@ class GanStep:
 
     def finish(self):
         """g_optimizer.step() (train.py:236); returns the step's losses and outputs."""
-        self.g_opt.step(self.scaler, 1)
+        g_norm = self.g_opt.step(self.scaler, 1, self.g_max_norm)
+        if g_norm is not None:
+            self._st['g_norm'] = g_norm
         if self.scaler is not None:
             self.scaler.update()
         ops.step_end(self._st['g3'].device)
