@@ -520,6 +520,33 @@ int vca_loss_scale_update(float* scale, int* state, float growth, float backoff,
 #define VCA_T_BF16 1
 #define VCA_T_F16 2
 
+/* Linear layer with bias, activation and residual in the product's epilogue (nn.Linear and what follows it; visual_front.py:21,
+ * generator.py:145-148,167,335 are plain ones), forward and gradients, on tensors of one type:
+ *   C[m][n] = act(sum_k A(m, k) B(n, k) + bias[n]) + res[m][n]
+ * A(m, k) = a[m lda + k] or, with a_col, a[k lda + m]; B(n, k) = b[n ldb + k] or, with b_col, b[k ldb + n]; res and c have
+ * row strides ldr and ldc (all in elements; ldr may be 0).  y = x W^T: neither; dx = dz W: b_col; dW = dz^T x: both.
+ * Any sizes and strides, pointers aligned to their element.  bias, res, z may be NULL; z [M][N] receives the value
+ * under the activation (for the backward pass).  res may be c: the product is added to it.
+ * type: VCA_T_F32, or the 16-bit type of this build (vca_elem_type).  nsplit: products per element pair, 1 for 16-bit
+ * tensors; fp32 tensors 0 (exact fp32 MFMA), 3 or 1 (split into / rounded to 16 bits in registers).
+ * act: 0 none, 1 leaky (slope), 3 relu, 4 tanh, 5 gelu (erf), 6 gelu (tanh form), 7 silu.
+ * ws: vca_matmul_act_ws_floats(d, a, b) floats for the partial products of a reduction split over workgroups (0: none). */
+typedef struct {
+  int M, N, K, type, nsplit, a_col, b_col, act;
+  float slope;
+  long long lda, ldb, ldc, ldr;
+} vca_matmul_desc;
+long long vca_matmul_act_ws_floats(const vca_matmul_desc* d, const void* a, const void* b);
+int vca_matmul_act(const vca_matmul_desc* d, const void* a, const void* b, const void* bias, const void* res, void* c,
+                   void* z, float* ws, long long ws_floats, void* stream);
+
+/* dz = gy act'(z) and db[n] (+)= sum_m dz[m][n] (of the unrounded dz) in one pass over dense [M][N] matrices.  Without an
+ * activation (act 0, z and dz NULL) only db is formed, from gy.  db may be NULL; db_add: add to it.
+ * ws: vca_act_bwd_ws_floats floats, needed with db. */
+long long vca_act_bwd_ws_floats(int type, int M, int N);
+int vca_act_bwd(int type, int M, int N, int act, float slope, const void* gy, const void* z, void* dz, void* db,
+                int db_add, float* ws, long long ws_floats, void* stream);
+
 /* Global norm of ntensor gradient tensors and clipping by it (torch.nn.utils.clip_grad_norm_ with the 2-norm; the
  * reference trains without clipping).  h_ptrs / h_numel / h_types are host arrays, read before the call returns:
  * device pointer (aligned to its element), element count (0 allowed) and VCA_T_* of each tensor, taken as dense memory.

@@ -1,0 +1,428 @@
+"""ops.linear_act (vca_matmul_act / vca_act_bwd: a linear layer with bias, activation and residual in the product's
+epilogue, forward and gradients) against 64-bit arithmetic, element by element.
+
+Tolerances (u = 2^-24, e = half an ulp of the tensors' type, finfo.eps / 2; |.| of matrices element by element):
+  z      the product: q |x| |w|^T for the operands' own rounding (q = 0 for exact fp32 and 16-bit tensors; split into
+         16-bit parts of half-ulp h: the dropped lo lo and the rounding of the two lo parts, 3 h^2, single product:
+         2 h + h^2) and (K + 8) u (|x| |w|^T + |b|) for fp32 accumulation in any order
+  y      |act'| <= 1.13 times that, 8 u (|z| + 1) for the activation's own evaluation, 2 u (|act| + |r|), and e |y|
+  dz     |gy| |act''| (dz + e |z|) with |act''| <= 1.13 for the smooth activations, 16 u |gy|; where a kinked
+         activation's |z| is within dz + e |z| of its kink the slope may be the other one; and e |dz|
+  dx     dz's error times |w|, the product's own error as above, and e |dx|; dw likewise with |x|; db = sum |gy| ... of
+         dz before its rounding, M u sum |dz|, and e |db|
+Half precision adds its smallest subnormal's half, 2^-25, per rounding."""
+import ctypes
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = {'fp32': torch.float32, 'bf16': torch.bfloat16, 'fp16': torch.float16}
+ACTS = {None: lambda z: z * 1.0, 'relu': F.relu, 'leaky0.2': lambda z: F.leaky_relu(z, 0.2), 'tanh': torch.tanh,
+        'gelu': F.gelu, 'gelu_tanh': lambda z: F.gelu(z, approximate='tanh'), 'silu': F.silu}
+
+
+@pytest.fixture(autouse=True)
+def _reset_precision():
+    yield
+    from vcagan_amd import ops
+    ops.set_precision('fp32')
+
+
+def _half(mode):
+    return 2.0 ** -11 if mode.startswith('fp16') else 2.0 ** -8
+
+
+def _split_error(mode, dtype, grad):
+    """q of the operands' rounding."""
+    if dtype != torch.float32 or mode == 'fp32':
+        return 0.0
+    h = _half(mode)
+    single = mode in ('bf16', 'fp16') or (grad and mode in ('mixed', 'fp16-mixed'))
+    return 2 * h + h * h if single else 3 * h * h
+
+
+def _inputs(M, K, N, dtype, seed, bias=True, res=True):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)
+    x, w = r(M, K).to(dtype).cuda(), (r(N, K) / K ** 0.5).to(dtype).cuda()
+    return (x, w, (r(N) * 0.5).to(dtype).cuda() if bias else None, r(M, N).to(dtype).cuda() if res else None,
+            r(M, N).to(dtype).cuda())
+
+
+def _mm(a, b):
+    return torch.mm(a.contiguous(), b.contiguous())
+
+
+def _reference(x, w, b, r, gy, act, mode):
+    """{name: (value, bound)} of y, dx, dw, db, dr."""
+    t = x.dtype
+    e = torch.finfo(t).eps / 2 if t != torch.float32 else U
+    tiny = 2.0 ** -25 if t == torch.float16 else 0.0
+    sub = 2.0 ** -24 if mode.startswith('fp16') and t == torch.float32 else 0.0     # a split part below half's range
+    M, K, N = x.shape[0], x.shape[1], w.shape[0]
+    X, W, G = x.double(), w.double(), gy.double()
+    q = _split_error(mode, t, False)
+    P = _mm(X.abs(), W.abs().t())
+    z = _mm(X, W.t())
+    if b is not None:
+        z, P = z + b.double(), P + b.double().abs()
+    ez = (q + (K + 8) * U) * P + sub * (X.abs().sum(1, True) + W.abs().sum(1)[None])
+    zz = z.clone().requires_grad_(True)
+    h = ACTS[act](zz)
+    slope, = torch.autograd.grad(h.sum(), zz)
+    h = h.detach()
+    y = h if r is None else h + r.double()
+    out = {'y': (y, 1.13 * ez + 8 * U * (z.abs() + 1) + 2 * U * (h.abs() + y.abs()) + e * y.abs() + tiny)}
+    dz = G * slope
+    if act is None:
+        eu = torch.zeros_like(dz)
+    else:
+        off = ez + e * z.abs() + tiny
+        eu = (G.abs() * torch.where(z.abs() <= off, 1.0, 0.0) if act in ('relu', 'leaky0.2')
+              else 1.13 * G.abs() * off) + 16 * U * G.abs()
+    ed = eu + (0.0 if act is None else e * (dz.abs() + eu) + tiny)
+    q = _split_error(mode, t, True)
+    D = dz.abs() + ed
+    dx, dw = _mm(dz, W), _mm(dz.t(), X)
+    out['dx'] = (dx, _mm(ed, W.abs()) + (q + (N + 8) * U) * _mm(D, W.abs()) + e * dx.abs() + tiny +
+                 sub * (D.sum(1, True) + W.abs().sum(0)[None]))
+    out['dw'] = (dw, _mm(ed.t(), X.abs()) + (q + (M + 8) * U) * _mm(D.t(), X.abs()) + e * dw.abs() + tiny +
+                 sub * (D.sum(0)[:, None] + X.abs().sum(0)[None]))
+    db = dz.sum(0)
+    out['db'] = (db, eu.sum(0) + (M + 8) * U * D.sum(0) + e * db.abs() + tiny)
+    out['dr'] = (G, torch.zeros_like(G))
+    return out
+
+
+def _check(got, want, what):
+    val, tol = want
+    off = (got.double().reshape(val.shape) - val).abs() - 1.01 * tol - 1e-30
+    assert bool((off <= 0).all()), (what, float(off.max()), float(tol.max()))
+
+
+def _run(M, K, N, dtype, act, seed, mode='fp32', bias=True, res=True):
+    from vcagan_amd import ops
+    ops.set_precision(mode)
+    x, w, b, r, gy = _inputs(M, K, N, dtype, seed, bias, res)
+    want = _reference(x, w, b, r, gy, act, mode)
+    with torch.no_grad():
+        y0 = ops.linear_act(x, w, b, act=act, residual=r)
+    leaves = [t for t in (x, w, b, r) if t is not None]
+    for t in leaves:
+        t.requires_grad_(True)
+    y = ops.linear_act(x, w, b, act=act, residual=r)
+    assert y.dtype == dtype and y.shape == (M, N) and torch.equal(y.detach(), y0)
+    grads = dict(zip([n for n, t in zip('xwbr', (x, w, b, r)) if t is not None], torch.autograd.grad(y, leaves, gy)))
+    _check(y.detach(), want['y'], ('y', M, K, N))
+    for n, g in grads.items():
+        assert g.dtype == dtype
+        _check(g, want['d' + n], ('d' + n, M, K, N))
+
+
+# rows, reduction, columns: single ones, below and just over every tile and chunk, odd and even, few rows with long
+# reductions (split over workgroups), the serving kernel's 16-row edge, the 256-wide tiles with and without a tail
+SHAPES = [(1, 1, 1), (1, 8, 16), (2, 3, 5), (1, 512, 512), (7, 129, 33), (15, 1000, 18), (16, 2048, 40), (17, 2048, 40),
+          (64, 64, 64), (127, 32, 129), (128, 64, 128), (129, 65, 127), (200, 1111, 77), (333, 96, 513), (40, 5000, 12),
+          (600, 256, 1280)]
+
+
+@gpu
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('i', range(len(SHAPES)))
+def test_forward_and_gradients(i, dtype):
+    M, K, N = SHAPES[i]
+    _run(M, K, N, TYPES[dtype], list(ACTS)[i % len(ACTS)], 100 + i, bias=i % 5 != 1, res=i % 3 != 1)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+@pytest.mark.parametrize('M,K,N', [(4096, 128, 4096), (3500, 136, 4001), (4104, 200, 4000)])
+def test_large_tiles(M, K, N, dtype):
+    _run(M, K, N, TYPES[dtype], 'gelu', 7)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('act', list(ACTS))
+def test_activations(act, dtype):
+    _run(70, 48, 90, TYPES[dtype], act, 5)
+    _run(3, 200, 50, TYPES[dtype], act, 6)
+
+
+@gpu
+@pytest.mark.parametrize('mode', ['bf16x3', 'bf16', 'mixed', 'fp16x3', 'fp16', 'fp16-mixed'])
+@pytest.mark.parametrize('M,K,N', [(1, 40, 24), (65, 129, 130), (300, 512, 257), (130, 96, 64)])
+def test_fp32_tensors_follow_the_precision_mode(M, K, N, mode):
+    _run(M, K, N, torch.float32, 'silu', 11, mode)
+
+
+@gpu
+def test_gradient_against_differences():
+    from vcagan_amd import ops
+    x, w, b, r, gy = _inputs(9, 21, 14, torch.float32, 3)
+    for act in (None, 'tanh', 'gelu', 'gelu_tanh', 'silu'):
+        ts = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
+        f = lambda *a: float((ops.linear_act(*a[:3], act=act, residual=a[3]).double() * gy.double()).sum())
+        grads = torch.autograd.grad(ops.linear_act(*ts[:3], act=act, residual=ts[3]), ts, gy)
+        h = 2.0 ** -7
+        for i, g in enumerate(grads):
+            v = torch.randn(ts[i].shape, generator=torch.Generator().manual_seed(i)).cuda()
+            with torch.no_grad():
+                plus, minus = ([t if j != i else t + s * h * v for j, t in enumerate(ts)] for s in (1, -1))
+                diff = (f(*plus) - f(*minus)) / (2 * h)
+            # third derivatives are below 2: h^2 / 6 * 2 * sum |gy| |dz|^3, and fp32 noise of the values over h
+            step = (v.abs() @ w.abs().t()) if i == 0 else (x.abs() @ v.abs().t()) if i == 1 else v.abs().expand(9, 14)
+            tol = float((gy.abs() * (h * h / 3 * step ** 3 + 40 * U * (x.abs() @ w.abs().t() + 4) / h)).sum())
+            assert abs(float((g.double() * v.double()).sum()) - diff) <= tol, (act, i)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+def test_strides_alignment_and_leading_dimensions(dtype):
+    """Rows inside a wider matrix, starts off any vector's alignment, a transposed weight, a broadcast residual, 3-D
+    inputs, an expanded incoming gradient: the results are those of dense copies, bit for bit."""
+    from vcagan_amd import ops
+    t = TYPES[dtype]
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g).to(t).cuda()
+    for lead, K, N in (((3, 11), 72, 40), ((2, 2, 5), 33, 19), ((160,), 130, 136)):
+        big = r(*lead, K + 9)
+        x = big[..., 3:3 + K]
+        w = r(K, N).t()
+        b = r(2 * N)[1:2 * N:2]
+        for res in (r(N).expand(*lead, N), r(*lead, 2 * N)[..., N:], r(*lead[::-1], N).permute(
+                *range(len(lead))[::-1], len(lead))):
+            dense = [v.detach().clone().contiguous().requires_grad_(True) for v in (x, w, b, res)]
+            views = [v.detach().requires_grad_(True) for v in (x, w, b, res)]
+            y = ops.linear_act(dense[0], dense[1], dense[2], act='gelu', residual=dense[3])
+            v = ops.linear_act(views[0], views[1], views[2], act='gelu', residual=views[3])
+            assert y.shape == lead + (N,) and torch.equal(y, v)
+            gy = r(N).expand(*lead, N)
+            for a, c in zip(torch.autograd.grad(y, dense, gy.contiguous()), torch.autograd.grad(v, views, gy)):
+                assert torch.equal(a, c)
+    # a residual that broadcasts takes the sum of the rows' gradients
+    row = r(N).requires_grad_(True)
+    y = ops.linear_act(r(9, K), r(N, K), residual=row.expand(9, N))
+    y.sum().backward()
+    assert torch.equal(row.grad, torch.full_like(row, 9.0))
+
+
+@gpu
+def test_empty_and_single():
+    from vcagan_amd import ops
+    x = torch.zeros(0, 12, device='cuda', requires_grad=True)
+    w = torch.randn(7, 12).cuda().requires_grad_(True)
+    b = torch.randn(7).cuda().requires_grad_(True)
+    y = ops.linear_act(x, w, b, act='relu', residual=torch.zeros(0, 7, device='cuda'))
+    assert y.shape == (0, 7)
+    y.sum().backward()
+    assert x.grad.shape == (0, 12) and float(w.grad.abs().max()) == 0.0 and float(b.grad.abs().max()) == 0.0
+    assert ops.linear_act(torch.zeros(3, 0, 12, device='cuda'), w).shape == (3, 0, 7)
+    v = torch.randn(12).cuda()
+    assert torch.equal(ops.linear_act(v, w, b).detach(), ops.linear_act(v[None], w, b)[0].detach())
+
+
+@gpu
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+def test_values_that_are_not_finite_stay_in_their_rows(dtype):
+    """A NaN or an infinity in a row of x reaches that row of y and nothing else, whatever its neighbours in the tile."""
+    from vcagan_amd import ops
+    x, w, b, r, _ = _inputs(150, 72, 130, TYPES[dtype], 2)
+    clean = ops.linear_act(x, w, b, act='relu', residual=r)
+    x[149, 71], x[3, 0] = math.nan, math.inf
+    y = ops.linear_act(x, w, b, act='relu', residual=r)
+    keep = torch.ones(150, dtype=torch.bool, device='cuda')
+    keep[149] = keep[3] = False
+    assert torch.equal(y[keep], clean[keep])
+    assert bool(y[149].isnan().all()) and bool((y[3].isinf() | (y[3] == r[3])).all())
+
+
+@gpu
+def test_slopes_far_out():
+    """The smooth activations' slopes reach 0 and 1 far from the origin instead of 0 x infinity."""
+    from vcagan_amd import ops
+    z = torch.tensor([-3e38, -1e20, -200.0, -61.0, 61.0, 200.0, 1e20, 3e38]).cuda()[:, None].requires_grad_(True)
+    one = torch.ones(1, 1).cuda()
+    for act, low in (('gelu', 0.0), ('gelu_tanh', 0.0), ('silu', 0.0), ('tanh', 0.0)):
+        y = ops.linear_act(z, one, act=act)
+        gz, = torch.autograd.grad(y.sum(), z)
+        hi = 0.0 if act == 'tanh' else 1.0
+        assert bool((gz[:4].abs() < 1e-24).all()) and torch.equal(gz[4:], torch.full_like(gz[4:], hi)), (act, gz)
+        assert bool(y.isfinite().all())
+
+
+@gpu
+def test_rows_of_the_output_beyond_it_stay():
+    """Through the C ABI: C with a row stride wider than its rows, and memory behind the last row, are left alone."""
+    from vcagan_amd import _lib
+    L = _lib.lib()
+    for M, K, N in ((5, 64, 24), (150, 64, 70), (130, 2048, 9)):
+        x, w, _, _, _ = _inputs(M, K, N, torch.float32, 4)
+        c = torch.full((M + 2, N + 5), 7.5, device='cuda')
+        d = _lib.MatmulDesc(M, N, K, 0, 0, 0, 0, 0, 0.0, K, K, N + 5, 0)
+        n = L.vca_matmul_act_ws_floats(d, x.data_ptr(), w.data_ptr())
+        ws = torch.empty(n + 4, device='cuda')
+        ws[n:] = 3.25
+        assert L.vca_matmul_act(d, x.data_ptr(), w.data_ptr(), None, None, c.data_ptr(), None, ws.data_ptr(), n,
+                                torch.cuda.current_stream().cuda_stream) == 0
+        assert bool((c[:, N:] == 7.5).all()) and bool((c[M:] == 7.5).all()) and bool((ws[n:] == 3.25).all())
+        want = _mm(x.double(), w.double().t())
+        assert bool(((c[:M, :N].double() - want).abs() <= (K + 8) * U * _mm(x.double().abs(), w.double().abs().t())).all())
+
+
+@gpu
+def test_direct_gradients_and_input_grads_only():
+    from vcagan_amd import ops
+    x, w, b, _, gy = _inputs(90, 64, 48, torch.float32, 8)
+    p, q = torch.nn.Parameter(w.clone()), torch.nn.Parameter(b.clone())
+    x1 = x.clone().requires_grad_(True)
+    gx, gw, gb = torch.autograd.grad(ops.linear_act(x1, p, q, act='silu'), (x1, p, q), gy)
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    with ops.direct_param_grad():
+        for _ in range(2):
+            ops.linear_act(x1, p, q, act='silu').backward(gy)
+    assert torch.equal(x1.grad, gx + gx)
+    assert float((p.grad - 1 - 2 * gw).abs().max()) <= 4 * U * float(1 + 2 * gw.abs().max())
+    assert float((q.grad - 1 - 2 * gb).abs().max()) <= 4 * U * float(1 + 2 * gb.abs().max())
+    x2 = x.clone().requires_grad_(True)
+    p.grad = q.grad = None
+    with ops.input_grads_only():
+        ops.linear_act(x2, p, q, act='silu').backward(gy)
+    assert torch.equal(x2.grad, gx) and p.grad is None and q.grad is None
+
+
+@gpu
+def test_streams_and_graph_replay():
+    """Forward and backward captured together and replayed on new inputs beside eager work of the same shapes."""
+    from vcagan_amd import ops
+    x, w, b, r, gy = _inputs(40, 1500, 70, torch.bfloat16, 9)
+    ts = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
+
+    def one():
+        y = ops.linear_act(ts[0], ts[1], ts[2], act='gelu', residual=ts[3])
+        return [y.detach()] + list(torch.autograd.grad(y, ts, gy))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        eager = one()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(eager, one()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = one()
+    for rep in range(4):
+        with torch.no_grad():
+            for i, t in enumerate(ts + [gy]):
+                t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(9 * rep + i)))
+        want = one()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, want)), rep
+
+
+@gpu
+def test_a_training_step_of_the_operators_together():
+    """Two fused layers with a residual, the global norm of their gradients, clipping inside the Adam update: parameters
+    after three steps against 64-bit arithmetic.  Tolerance: with exact fp32 products a gradient is off by at most 1e-5
+    of its tensor's largest value (reductions of 96 terms: 104 u, twice through the two layers); Adam's update is at
+    most 4 lr a step whatever the gradient, and moves by less than lr x 1e-3 where the gradient is over a hundredth of
+    the largest one, so the mean deviation is below 1e-3 lr and no element's exceeds 2 lr a step."""
+    from vcagan_amd import ops
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            g = torch.Generator().manual_seed(0)
+            self.w1 = torch.nn.Parameter(torch.randn(96, 64, generator=g) / 8)
+            self.b1 = torch.nn.Parameter(torch.randn(96, generator=g) / 8)
+            self.w2 = torch.nn.Parameter(torch.randn(64, 96, generator=g) / 10)
+            self.b2 = torch.nn.Parameter(torch.randn(64, generator=g) / 8)
+    net = Net().cuda()
+    ref = [p.detach().double() for p in net.parameters()]
+    opt = ops.FusedAdam([ops.flatten_module(net)], lr=1e-3)
+    flat = [torch.zeros_like(p) for p in ref], [torch.zeros_like(p) for p in ref]
+    for t in (1, 2, 3):
+        g = torch.Generator().manual_seed(t)
+        x, gy = (torch.randn(80, 64, generator=g).cuda() for _ in range(2))
+        opt.zero_grad()
+        with ops.direct_param_grad():
+            y = ops.linear_act(ops.linear_act(x, net.w1, net.b1, act='gelu'), net.w2, net.b2, residual=x)
+            y.backward(gy)
+        norm = opt.step(max_norm=1.0)
+        rp = [p.clone().requires_grad_(True) for p in ref]
+        F.linear(F.gelu(F.linear(x.double(), rp[0], rp[1])), rp[2], rp[3]).backward(gy.double())
+        total = math.sqrt(sum(float(p.grad.pow(2).sum()) for p in rp))
+        assert abs(float(norm) - total) <= 1e-5 * total
+        for i, p in enumerate(rp):
+            gr = p.grad * min(1.0, 1.0 / (total + 1e-6))
+            flat[0][i] = 0.9 * flat[0][i] + 0.1 * gr
+            flat[1][i] = 0.999 * flat[1][i] + 0.001 * gr * gr
+            ref[i] = ref[i] - 1e-3 / (1 - 0.9 ** t) * flat[0][i] / ((flat[1][i] / (1 - 0.999 ** t)).sqrt() + 1e-8)
+    for p, q in zip(net.parameters(), ref):
+        off = (p.detach().double() - q).abs()
+        assert float(off.mean()) <= 1e-6 and float(off.max()) <= 6e-3
+
+
+@gpu
+def test_refusals_on_device_tensors():
+    from vcagan_amd import ops
+    x, w, b, r, _ = _inputs(6, 12, 8, torch.float32, 0)
+    with pytest.raises(ValueError):
+        ops.linear_act(x, w, b, act='swish')
+    with pytest.raises(ValueError):
+        ops.linear_act(x, w.t())
+    with pytest.raises(ValueError):
+        ops.linear_act(x, w, b[:7])
+    with pytest.raises(ValueError):
+        ops.linear_act(x, w, b, residual=r[:1])
+    with pytest.raises(ValueError):
+        ops.linear_act(x, w.cpu())
+    with pytest.raises(ValueError):
+        ops.linear_act(torch.zeros(4, 0).cuda(), torch.zeros(3, 0).cuda())
+    with pytest.raises(TypeError):
+        ops.linear_act(x, w.half())
+    with pytest.raises(TypeError):
+        ops.linear_act(x.double(), w.double())
+    xr = x.requires_grad_(True)
+    y = ops.linear_act(xr, w, b, act='tanh')
+    g, = torch.autograd.grad(y.sum(), xr, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_refusals_without_a_gpu():
+    from vcagan_amd import ops
+    with pytest.raises(ValueError):
+        ops.linear_act(torch.zeros(2, 4), torch.zeros(3, 4))
+    with pytest.raises(TypeError):
+        ops.linear_act(torch.zeros(2, 4).double(), torch.zeros(3, 4).double())
+
+
+def test_entry_points_refuse_before_any_launch():
+    from vcagan_amd import _lib
+    for elem, own, other in (('bf16', 1, 2), ('fp16', 2, 1)):
+        L = _lib.lib(elem)
+        ok = dict(M=64, N=64, K=64, type=0, nsplit=0, a_col=0, b_col=0, act=0, slope=0.0, lda=64, ldb=64, ldc=64, ldr=64)
+        call = lambda a=64, b=64, c=64, ws=64, n=1 << 30, bias=None, **kw: L.vca_matmul_act(
+            _lib.MatmulDesc(**dict(ok, **kw)), a, b, bias, None, c, None, ws, n, None)
+        for kw in (dict(M=0), dict(N=0), dict(K=0), dict(K=-5), dict(type=3), dict(type=other, nsplit=1),
+                   dict(type=own, nsplit=0), dict(type=own, nsplit=3), dict(nsplit=2), dict(act=2), dict(act=8),
+                   dict(lda=63), dict(ldb=63), dict(ldc=63), dict(ldr=-1), dict(a_col=1, b_col=0),
+                   dict(b_col=1, ldb=63), dict(a_col=1, b_col=1, lda=63), dict(a=None), dict(b=None), dict(c=None),
+                   dict(a=66), dict(bias=65)):
+            assert call(**kw) == -22, kw
+        long = dict(K=1 << 16, lda=1 << 16, ldb=1 << 16)
+        n = L.vca_matmul_act_ws_floats(_lib.MatmulDesc(**dict(ok, **long)), 64, 64)
+        assert n > 0 and n % (64 * 64) == 0
+        assert call(ws=None, **long) == -22 and call(n=n - 1, **long) == -22 and call(ws=68, **long) == -22
+        f = lambda type=0, M=4, N=4, act=6, gy=64, z=64, dz=64, db=64, ws=64, n=1 << 20: L.vca_act_bwd(
+            type, M, N, act, 0.0, gy, z, dz, db, 0, ws, n, None)
+        for kw in (dict(type=other), dict(M=0), dict(N=0), dict(act=2), dict(act=9), dict(gy=None), dict(z=None),
+                   dict(dz=None, db=None), dict(ws=None), dict(n=3), dict(act=0), dict(act=0, z=None), dict(z=66)):
+            assert f(**kw) == -22, kw
+        assert L.vca_act_bwd_ws_floats(0, 0, 4) == 0

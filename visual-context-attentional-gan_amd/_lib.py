@@ -20,7 +20,8 @@ LIB_PATH = os.path.join(_HERE, 'libvca_hip.so')
 LIB_PATH_F16 = os.path.join(_HERE, 'libvca_hip_f16.so')
 ELEM = ['bf16']          # element type of the matrix products: 'bf16' or 'fp16' (set by ops.set_precision)
 SOURCES = ('conv_f32.hip', 'conv_bf16.hip', 'pointwise.hip', 'misc.hip', 'rnn.hip', 'attention.hip', 'stem.hip',
-           'sync_loss.hip', 'layout.hip', 'audio.hip', 'video.hip', 'ctc.hip', 'wgrad_cin1.hip', 'linear.hip', 'gradnorm.hip')
+           'sync_loss.hip', 'layout.hip', 'audio.hip', 'video.hip', 'ctc.hip', 'wgrad_cin1.hip', 'linear.hip',
+           'gradnorm.hip', 'linear_act.hip')
 
 
 # Packed fp32 instructions stay off: on this part some of their forms, which the compiler makes out of ordinary float
@@ -86,6 +87,11 @@ MAX_LOSS_HEADS, MAX_LOSS_SLOTS = 24, 16
 
 class LossHeads(ctypes.Structure):
     _fields_ = [('nhead', ctypes.c_int), ('total_blocks', ctypes.c_int), ('h', LossHead * MAX_LOSS_HEADS)]
+
+
+class MatmulDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ('M', 'N', 'K', 'type', 'nsplit', 'a_col', 'b_col', 'act')] + \
+        [('slope', ctypes.c_float)] + [(n, ctypes.c_longlong) for n in ('lda', 'ldb', 'ldc', 'ldr')]
 
 
 class AdamGroup(ctypes.Structure):
@@ -185,6 +191,10 @@ _SIGS = {
     'vca_loss_scale_count': ([_P, _P, _P], _I),
     'vca_adam_scaled_f32': ([_LL, _P, _P, _P, _P, _P, _F, _F, _F, _F, _P, _P, _P, _P, _P], _I),
     'vca_loss_scale_update': ([_P, _P, _F, _F, _I, _P], _I),
+    'vca_matmul_act_ws_floats': ([ctypes.POINTER(MatmulDesc), _P, _P], _LL),
+    'vca_matmul_act': ([ctypes.POINTER(MatmulDesc)] + [_P] * 7 + [_LL, _P], _I),
+    'vca_act_bwd_ws_floats': ([_I, _I, _I], _LL),
+    'vca_act_bwd': ([_I, _I, _I, _I, _F, _P, _P, _P, _P, _I, _P, _LL, _P], _I),
     'vca_grad_norm_ws_doubles': ([_I], _LL),
     'vca_grad_norm': ([_I, _P, _P, _P, _P, _P, _LL, _P, _P], _I),
     'vca_grad_clip': ([_I, _P, _P, _P, _F, _P, _P, _LL, _P, _P], _I),
@@ -194,11 +204,12 @@ _SIGS = {
 _libs = {}
 
 
-def lib():
-    """The library whose matrix products use the element type in ELEM."""
-    L = _libs.get(ELEM[0])
+def lib(elem=None):
+    """The library whose matrix products use the element type elem ('bf16' or 'fp16'; by default the one in ELEM)."""
+    elem = ELEM[0] if elem is None else elem
+    L = _libs.get(elem)
     if L is None:
-        path = {'bf16': LIB_PATH, 'fp16': LIB_PATH_F16}[ELEM[0]]
+        path = {'bf16': LIB_PATH, 'fp16': LIB_PATH_F16}[elem]
         if not os.path.exists(path):
             raise RuntimeError('%s is not built (%s); run `python __graft_entry__.py`' % (os.path.basename(path), path))
         L = ctypes.CDLL(path)
@@ -206,8 +217,8 @@ def lib():
             fn = getattr(L, name)
             fn.argtypes = args
             fn.restype = res
-        assert L.vca_elem_type() == {'bf16': 0, 'fp16': 1}[ELEM[0]], path
-        _libs[ELEM[0]] = L
+        assert L.vca_elem_type() == {'bf16': 0, 'fp16': 1}[elem], path
+        _libs[elem] = L
     return L
 
 

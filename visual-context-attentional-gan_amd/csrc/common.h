@@ -83,6 +83,8 @@ static inline void vca_zero_async(float* p, size_t n, hipStream_t s) {
 
 // Activation codes shared by the conv prologue and the pointwise kernels.
 enum { VCA_ACT_NONE = 0, VCA_ACT_LEAKY = 1, VCA_ACT_PRELU = 2, VCA_ACT_RELU = 3, VCA_ACT_TANH = 4 };
+// Further ones of the linear layer's epilogue.
+enum { VCA_ACT_GELU = 5, VCA_ACT_GELU_TANH = 6, VCA_ACT_SILU = 7 };
 
 __device__ __forceinline__ float vca_act(float z, int act, float slope) {
   // slope: the leaky slope, or this channel's PReLU weight

@@ -1,0 +1,812 @@
+// Linear layers with bias, activation and residual in the product's epilogue, forward and gradients, on fp32 and 16-bit
+// tensors of any size, row stride and alignment:
+//
+//   z = x W^T + b     y = act(z) + r          (one pass over the product: z is rounded and kept for the backward pass)
+//   dz = gy act'(z)   db = sum_m dz           (one pass over gy and z)
+//   dx = dz W         dW = dz^T x             (products with one or both operands read along their columns)
+//
+// All three products are C[m][n] = sum_k A(m, k) B(n, k); an operand is stored either with k contiguous (x, W in the
+// forward pass, dz in dx) or with its own index contiguous (W in dx, dz and x in dW).  Neither is ever transposed in
+// memory: a column-major operand is staged as it lies and transposed on the way from LDS to the registers.
+//
+// Arithmetic: 16-bit tensors of the library's element type take one product with fp32 accumulation.  fp32 tensors take
+// the exact fp32 MFMA (nsplit 0) or are split in registers into 16-bit parts (nsplit 3: hi hi + hi lo + lo hi; 1: hi).
+// Bias, activation and residual are applied to the fp32 accumulator, so a result is rounded once.
+#include "common.h"
+
+namespace {
+
+enum { MODE_16 = 0, MODE_F32 = 1, MODE_S3 = 2, MODE_S1 = 3 };   // 16-bit tensors; fp32: exact, three products, one
+
+template <int MODE> struct ElemOf { typedef float T; };
+template <> struct ElemOf<MODE_16> { typedef vca_e16 T; };
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+struct MatArgs {
+  const void *a, *b, *bias, *res;
+  void *c, *z;
+  float* part;                        // [ksplit][M][npad] partial products (ksplit > 1)
+  long long lda, ldb, ldc, ldr;       // elements
+  int M, N, K;
+  int ntm, ntn, ksplit, cpz, npad;    // tiles, reduction ranges, chunks a range, padded columns of a partial product
+  int act;
+  float slope;
+};
+
+// 16 bytes from any address that is aligned to its element: gfx950 takes unaligned wide accesses, the packed type makes
+// the compiler use them.
+struct __attribute__((packed, aligned(2))) Any16 { uint4 u; };
+
+template <typename T> union Vec16 {
+  uint4 u;
+  T e[16 / sizeof(T)];
+};
+
+// ------------------------------------------------------------------------------------------------
+// activations, in fp32
+// ------------------------------------------------------------------------------------------------
+constexpr float GELU_C = 0.7978845608028654f, GELU_A = 0.044715f;   // sqrt(2 / pi)
+
+__device__ __forceinline__ float act_f(float z, int act, float slope) {
+  switch (act) {
+    case VCA_ACT_LEAKY: return z > 0.f ? z : z * slope;
+    case VCA_ACT_RELU: return z <= 0.f ? 0.f : z;            // a NaN stays one
+    case VCA_ACT_TANH: return tanhf(z);
+    case VCA_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case VCA_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(GELU_C * (z + GELU_A * z * z * z)));
+    case VCA_ACT_SILU: return z / (1.f + expf(-z));
+    default: return z;
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void act_all(float (&v)[V], int act, float slope) {
+  switch (act) {                       // one test for the V values
+#define VCA_EACH(code)                                       \
+  case code: {                                               \
+    _Pragma("unroll") for (int r = 0; r < V; ++r) v[r] = act_f(v[r], code, slope); \
+    break;                                                   \
+  }
+    VCA_EACH(VCA_ACT_LEAKY)
+    VCA_EACH(VCA_ACT_RELU)
+    VCA_EACH(VCA_ACT_TANH)
+    VCA_EACH(VCA_ACT_GELU)
+    VCA_EACH(VCA_ACT_GELU_TANH)
+    VCA_EACH(VCA_ACT_SILU)
+#undef VCA_EACH
+    default: break;
+  }
+}
+
+__device__ __forceinline__ float act_slope(float z, int act, float slope) {
+  // beyond +-60 the smooth activations' slopes are 0 or 1 to fp32; the clamp keeps 0 x infinity out of them (a NaN
+  // comes through the unclamped term)
+  const float c = fminf(fmaxf(z, -60.f), 60.f);
+  switch (act) {
+    case VCA_ACT_LEAKY: return z > 0.f ? 1.f : slope;
+    case VCA_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+    case VCA_ACT_TANH: {
+      const float h = tanhf(z);
+      return 1.f - h * h;
+    }
+    case VCA_ACT_GELU:
+      return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + c * expf(-0.5f * c * c) * 0.3989422804014327f;
+    case VCA_ACT_GELU_TANH: {
+      const float h = tanhf(GELU_C * (z + GELU_A * z * z * z));
+      return 0.5f * (1.f + h) + 0.5f * c * (1.f - h * h) * GELU_C * (1.f + 3.f * GELU_A * c * c);
+    }
+    case VCA_ACT_SILU: {
+      const float e = 1.f / (1.f + expf(-z));
+      return e * (1.f + c * (1.f - e));
+    }
+    default: return 1.f;
+  }
+}
+
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) AnyVec { T e[V]; };
+
+// Bias, activation and residual of V neighbouring columns n .. n + V - 1 of row m; stores y and, if kept, z.
+template <typename T, int V>
+__device__ __forceinline__ void finish(const MatArgs& g, int m, int n, float (&v)[V]) {
+  typedef AnyVec<T, V> Any;
+  const T* bias = reinterpret_cast<const T*>(g.bias);
+  const T* res = reinterpret_cast<const T*>(g.res);
+  T* c = reinterpret_cast<T*>(g.c) + (size_t)m * g.ldc + n;
+  T* z = g.z ? reinterpret_cast<T*>(g.z) + (size_t)m * g.N + n : nullptr;
+  const bool whole = n + V <= g.N;
+  auto add = [&](const T* p) {
+    if (whole) {
+      const Any q = *reinterpret_cast<const Any*>(p);
+#pragma unroll
+      for (int r = 0; r < V; ++r) v[r] += (float)q.e[r];
+    } else {
+#pragma unroll
+      for (int r = 0; r < V; ++r)
+        if (n + r < g.N) v[r] += (float)p[r];
+    }
+  };
+  auto store = [&](T* p) {
+    if (whole) {
+      Any q;
+#pragma unroll
+      for (int r = 0; r < V; ++r) q.e[r] = (T)v[r];
+      *reinterpret_cast<Any*>(p) = q;
+    } else {
+#pragma unroll
+      for (int r = 0; r < V; ++r)
+        if (n + r < g.N) p[r] = (T)v[r];
+    }
+  };
+  if (bias) add(bias + n);
+  if (z) store(z);
+  act_all(v, g.act, g.slope);
+  if (res) add(res + (size_t)m * g.ldr + n);
+  store(c);
+}
+
+// ------------------------------------------------------------------------------------------------
+// The tiled product.  A workgroup owns a BM x BN tile of C and walks the reduction in chunks of 128 bytes of a row
+// (64 16-bit or 32 fp32 elements) through two LDS stages: chunk c + 1 travels while chunk c feeds the matrix cores, one
+// barrier a chunk.  DMA: whole chunks go straight from memory to LDS (16-byte pieces, operands 16-byte aligned); the
+// reduction's last, partial chunk, and every chunk of operands of another alignment, go through registers with masks.
+//
+// LDS images of an operand with R rows in the tile:
+//   k contiguous      [R][128 B], 16-byte pieces of a row XOR-ed with row & 7: the 16 rows a fragment load touches
+//                     spread over all banks
+//   index contiguous  [chunk][R elements]; 16-bit: 32-byte blocks XOR-ed with (k & 3) | (k >> 1 & 4), fp32: 64-byte
+//                     blocks with 2 bits of k, so that the rows of k one fragment load touches fall on different banks
+// 16-bit fragments of a column-major image come from ds_read_b64_tr_b16, which hands lane i of 16 the i-th column of a
+// 4 x 16 block; fp32 fragments are single words.  The order of k inside a chunk only has to be the same for A and B.
+// B is the MFMA's row operand, so a lane ends with four neighbouring columns of one row of C.
+// ------------------------------------------------------------------------------------------------
+template <int MODE, int R>
+__device__ __forceinline__ int col_swizzle(int k) {       // in 16-byte pieces
+  if (MODE == MODE_16) return ((k & 3) | ((k >> 1) & 4)) << 1;
+  return ((MODE == MODE_F32 ? k >> 2 : k >> 3) & 3) << 2;
+}
+
+template <int MODE, bool KC, int R, int NT>
+struct Operand {
+  typedef typename ElemOf<MODE>::T T;
+  static constexpr int ESZ = sizeof(T), EPP = 16 / ESZ, BK = 128 / ESZ;
+  static constexpr int PIECES = R * 8 / NT;               // 16-byte pieces a thread stages
+  static constexpr int PPR = R * ESZ / 16;                // pieces of a row of k (index contiguous)
+  const char* src[PIECES];                                // this thread's pieces of the next chunk to fetch (DMA)
+  const char* base;
+  long long ldb;                                          // bytes
+  int o0, outer, K, tid;
+
+  __device__ __forceinline__ void piece(int it, int& row, int& pc) const {   // tile row (of C or of k), source piece
+    const int q = it * NT + tid;
+    if (KC) {
+      row = q >> 3;
+      pc = (q & 7) ^ (row & 7);
+    } else {
+      row = q / PPR;
+      pc = (q % PPR) ^ col_swizzle<MODE, R>(row);
+    }
+  }
+
+  __device__ __forceinline__ void init(const void* p, long long ld, int o0_, int outer_, int K_, int tid_) {
+    base = reinterpret_cast<const char*>(p);
+    ldb = ld * ESZ;
+    o0 = o0_;
+    outer = outer_;
+    K = K_;
+    tid = tid_;
+  }
+
+  // addresses of the first chunk's pieces, clamped into the operand (rows and columns of C beyond its edge are computed
+  // from repeated values and never stored)
+  __device__ __forceinline__ void start(int c) {
+#pragma unroll
+    for (int it = 0; it < PIECES; ++it) {
+      int row, pc;
+      piece(it, row, pc);
+      if (KC) src[it] = base + (long long)min(o0 + row, outer - 1) * ldb + (long long)c * 128 + pc * 16;
+      else src[it] = base + (long long)(c * BK + row) * ldb + (long long)min(o0 + pc * EPP, outer - EPP) * ESZ;
+    }
+  }
+
+  __device__ __forceinline__ void dma(char* stage) {
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+    for (int it = 0; it < PIECES; ++it) {
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[it],
+                                       (__attribute__((address_space(3))) void*)(stage + (it * NT + wave * 64) * 16), 16,
+                                       0, 0);
+      src[it] += KC ? 128ll : BK * ldb;
+    }
+  }
+
+  __device__ __forceinline__ void fetch(int c, uint4 (&r)[PIECES]) const {
+#pragma unroll
+    for (int it = 0; it < PIECES; ++it) {
+      int row, pc;
+      piece(it, row, pc);
+      r[it] = make_uint4(0, 0, 0, 0);
+      const int o = o0 + (KC ? row : pc * EPP), k = c * BK + (KC ? pc * EPP : row);
+      if (o >= outer || k >= K) continue;
+      const int left = KC ? K - k : outer - o;            // elements of the piece that exist
+      const char* p = base + (KC ? (long long)o * ldb + (long long)k * ESZ : (long long)k * ldb + (long long)o * ESZ);
+      if (left >= EPP) {
+        r[it] = reinterpret_cast<const Any16*>(p)->u;
+      } else {
+        Vec16<T> v;
+#pragma unroll
+        for (int e = 0; e < EPP; ++e) v.e[e] = e < left ? reinterpret_cast<const T*>(p)[e] : (T)0.f;
+        r[it] = v.u;
+      }
+    }
+  }
+
+  __device__ __forceinline__ void put(char* stage, const uint4 (&r)[PIECES]) const {
+#pragma unroll
+    for (int it = 0; it < PIECES; ++it) *reinterpret_cast<uint4*>(stage + (it * NT + tid) * 16) = r[it];
+  }
+};
+
+// Fragment loads.  sub: first of the 16 rows or columns of C; lane = 16 g + lc.
+template <bool KC, int R>
+__device__ __forceinline__ bf16x8 frag16(const char* s, int sub, int kk, int lc, int g) {
+  if (KC) return *reinterpret_cast<const bf16x8*>(s + (sub + lc) * 128 + (((kk * 4 + g) ^ (lc & 7)) << 4));
+  const int k = kk * 32 + 8 * g + (lc >> 2);
+  const char* p = s + k * (R * 2) + (((sub >> 4) ^ ((k & 3) | ((k >> 1) & 4))) << 5) + (lc & 3) * 8;
+  union { s16x4 h[2]; bf16x8 v; } f;
+  f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+  f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * R * 2));
+  return f.v;
+}
+
+template <bool KC, int R>
+__device__ __forceinline__ f32x4 frag32(const char* s, int sub, int kk, int lc, int g) {   // k = 16 kk + 4 g + 0 .. 3
+  if (KC) return *reinterpret_cast<const f32x4*>(s + (sub + lc) * 128 + (((kk * 4 + g) ^ (lc & 7)) << 4));
+  f32x4 f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int k = kk * 16 + 4 * g + e;
+    f[e] = *reinterpret_cast<const float*>(s + k * (R * 4) + (((sub >> 4) ^ ((k >> 2) & 3)) << 6) + lc * 4);
+  }
+  return f;
+}
+
+template <bool KC, int R>
+__device__ __forceinline__ void frag_split(const char* s, int sub, int lc, int g, bf16x8& hi, bf16x8& lo) {  // k = 8 g ...
+  float v[8];
+  if (KC) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 t = *reinterpret_cast<const f32x4*>(s + (sub + lc) * 128 + (((2 * g + h) ^ (lc & 7)) << 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * h + e] = t[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int k = 8 * g + e;
+      v[e] = *reinterpret_cast<const float*>(s + k * (R * 4) + (((sub >> 4) ^ ((k >> 3) & 3)) << 6) + lc * 4);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const vca_e16 h = (vca_e16)v[e];
+    hi[e] = h;
+    lo[e] = (vca_e16)(v[e] - (float)h);
+  }
+}
+
+// Workgroup -> tile.  Consecutive workgroups go to the 8 XCDs in turn; each XCD gets a contiguous range of the tiles,
+// and those run through groups of 8 tile rows column by column, so the tiles an XCD's L2 holds share operands.
+__device__ __forceinline__ void tile_of(const MatArgs& g, int& tm, int& tn, int& kz) {
+  const int total = gridDim.x, id = blockIdx.x;
+  const int x = id & 7, per = total >> 3, rem = total & 7;
+  int t = x * per + min(x, rem) + (id >> 3);
+  const int tiles = g.ntm * g.ntn;
+  kz = t / tiles;
+  t -= kz * tiles;
+  const int band = 8 * g.ntn, grp = t / band, m0 = grp * 8, rows = min(8, g.ntm - m0);
+  t -= grp * band;
+  tm = m0 + t % rows;
+  tn = t / rows;
+}
+
+template <int MODE, bool AKC, bool BKC, int BM, int BN, int NWM, int NWN, bool DMA>
+__global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  typedef typename ElemOf<MODE>::T T;
+  constexpr int NT = NWM * NWN * 64, BK = 128 / (int)sizeof(T);
+  constexpr int TM = BM / NWM / 16, TN = BN / NWN / 16;
+  constexpr int STAGE = (BM + BN) * 128;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lc = lane & 15, lg = lane >> 4;
+  const int wm = wave / NWN, wn = wave % NWN;
+  int tm, tn, kz;
+  tile_of(g, tm, tn, kz);
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int c0 = kz * g.cpz, c1 = min((g.K + BK - 1) / BK, c0 + g.cpz);
+  const int whole = DMA ? max(c0, min(c1, g.K / BK)) : c0;   // chunks [c0, whole) travel by DMA, the rest through registers
+
+  Operand<MODE, AKC, BM, NT> A;
+  Operand<MODE, BKC, BN, NT> B;
+  A.init(g.a, g.lda, m0, g.M, g.K, tid);
+  B.init(g.b, g.ldb, n0, g.N, g.K, tid);
+
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  auto compute = [&](const char* sa) {
+    const char* sb = sa + BM * 128;
+    if (MODE == MODE_16) {
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        bf16x8 fb[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) fb[j] = frag16<BKC, BN>(sb, (wn * TN + j) * 16, kk, lc, lg);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const bf16x8 fa = frag16<AKC, BM>(sa, (wm * TM + i) * 16, kk, lc, lg);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = VCA_MFMA_16x16x32(fb[j], fa, acc[i][j]);
+        }
+      }
+    } else if (MODE == MODE_F32) {
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        f32x4 fb[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) fb[j] = frag32<BKC, BN>(sb, (wn * TN + j) * 16, kk, lc, lg);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const f32x4 fa = frag32<AKC, BM>(sa, (wm * TM + i) * 16, kk, lc, lg);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[j][e], fa[e], acc[i][j], 0, 0, 0);
+        }
+      }
+    } else {
+      bf16x8 bh[TN], bl[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) frag_split<BKC, BN>(sb, (wn * TN + j) * 16, lc, lg, bh[j], bl[j]);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        bf16x8 ah, al;
+        frag_split<AKC, BM>(sa, (wm * TM + i) * 16, lc, lg, ah, al);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          if (MODE == MODE_S3) {
+            acc[i][j] = VCA_MFMA_16x16x32(bl[j], ah, acc[i][j]);
+            acc[i][j] = VCA_MFMA_16x16x32(bh[j], al, acc[i][j]);
+          }
+          acc[i][j] = VCA_MFMA_16x16x32(bh[j], ah, acc[i][j]);
+        }
+      }
+    }
+  };
+
+  if (c0 < whole) {
+    A.start(c0);
+    B.start(c0);
+    A.dma(smem);
+    B.dma(smem + BM * 128);
+    for (int c = c0; c < whole; ++c) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // chunk c has landed, in every wave behind the barrier
+      __syncthreads();
+      char* next = smem + ((c - c0 + 1) & 1) * STAGE;     // every wave has left this stage: it is behind chunk c - 1
+      if (c + 1 < whole) {
+        A.dma(next);
+        B.dma(next + BM * 128);
+      }
+      compute(smem + ((c - c0) & 1) * STAGE);
+    }
+  }
+  if (whole < c1) {                                       // not by DMA: chunk c + 1 waits in registers under chunk c
+    uint4 ra[A.PIECES], rb[B.PIECES];
+    A.fetch(whole, ra);
+    B.fetch(whole, rb);
+    __syncthreads();
+    for (int c = whole; c < c1; ++c) {
+      char* st = smem + ((c - whole) & 1) * STAGE;
+      A.put(st, ra);
+      B.put(st + BM * 128, rb);
+      __syncthreads();                                    // (two stages: the writers of c + 1 need not wait for c)
+      if (c + 1 < c1) {
+        A.fetch(c + 1, ra);
+        B.fetch(c + 1, rb);
+      }
+      compute(st);
+    }
+  }
+
+  if (g.ksplit > 1) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int m = m0 + (wm * TM + i) * 16 + lc;
+      if (m >= g.M) continue;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int n = n0 + (wn * TN + j) * 16 + 4 * lg;
+        if (n < g.npad)
+          *reinterpret_cast<f32x4*>(g.part + ((size_t)kz * g.M + m) * g.npad + n) = acc[i][j];
+      }
+    }
+    return;
+  }
+  // The accumulators pass through LDS (fp32, 16-byte pieces of a row XOR-ed with the row) so that a thread finishes 16
+  // bytes of a row of C and a wave writes whole lines, in one or two halves of each wave's rows.
+  constexpr int V = 16 / (int)sizeof(T), HALVES = BM * BN * 4 > 2 * STAGE ? 2 : 1, HM = TM / HALVES, TPR = BN / V;
+#pragma unroll
+  for (int h = 0; h < HALVES; ++h) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < HM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int row = (wm * HM + i) * 16 + lc, pc = (wn * TN + j) * 4 + lg;
+        *reinterpret_cast<f32x4*>(smem + row * (BN * 4) + ((pc ^ lc) << 4)) = acc[h * HM + i][j];
+      }
+    __syncthreads();
+#pragma unroll 1
+    for (int q = tid; q < NWM * HM * 16 * TPR; q += NT) {
+      const int row = q / TPR, col = (q % TPR) * V;
+      const int m = m0 + (row / (HM * 16) * TM + h * HM) * 16 + row % (HM * 16), n = n0 + col;
+      if (m >= g.M || n >= g.N) continue;
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; e += 4) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(smem + row * (BN * 4) + ((((col + e) >> 2) ^ (row & 15)) << 4));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[e + r] = t[r];
+      }
+      finish<T, V>(g, m, n, v);
+    }
+  }
+}
+
+// C from the ksplit partial products, added in order of the reduction, through the same epilogue
+template <typename T>
+__global__ __launch_bounds__(256) void matmul_fold_kernel(const MatArgs g) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int nv = (g.N + V - 1) / V;
+  const size_t total = (size_t)g.M * nv, slab = (size_t)g.M * g.npad;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+    const int m = (int)(i / nv), n = (int)(i - (size_t)m * nv) * V;
+    const float* p = g.part + (size_t)m * g.npad + n;      // npad is a multiple of 8
+    float v[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = 0.f;
+    for (int s = 0; s < g.ksplit; ++s)
+#pragma unroll
+      for (int e = 0; e < V; e += 4) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(p + s * slab + e);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[e + r] += t[r];
+      }
+    finish<T, V>(g, m, n, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Few rows (M <= 16, both operands with k contiguous): the product reads W once and does next to nothing with it, so
+// there is no tile to share through LDS.  A workgroup owns 16 columns of C; its waves take the reduction's chunks in
+// turn, each lane streaming its own 16 bytes of a W row (and of an x row, out of the caches) straight into an MFMA
+// operand, UNROLL chunks in flight; the waves' partial tiles meet in LDS.  Rows of x beyond M repeat the last one.
+// ------------------------------------------------------------------------------------------------
+constexpr int FEW_WAVES = 8;
+
+template <int MODE>
+__global__ __launch_bounds__(FEW_WAVES * 64) void few_rows_kernel(const MatArgs g) {
+  typedef typename ElemOf<MODE>::T T;
+  constexpr int EPP = 16 / (int)sizeof(T), CK = 4 * EPP;   // elements a lane and a chunk take
+  constexpr int UNROLL = 8;
+  __shared__ f32x4 red[FEW_WAVES][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lc = lane & 15, lg = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const T* wp = reinterpret_cast<const T*>(g.b) + (long long)min(n0 + lc, g.N - 1) * g.ldb;
+  const T* xp = reinterpret_cast<const T*>(g.a) + (long long)min(lc, g.M - 1) * g.lda;
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto load = [&](const T* p, int c) {
+    const int k = c * CK + lg * EPP;
+    if (k + EPP <= g.K) return reinterpret_cast<const Any16*>(p + k)->u;
+    Vec16<T> v;
+#pragma unroll
+    for (int e = 0; e < EPP; ++e) v.e[e] = k + e < g.K ? p[k + e] : (T)0.f;
+    return v.u;
+  };
+  auto mul = [&](const uint4& uw, const uint4& ux) {
+    if (MODE == MODE_16) {
+      union { uint4 u; bf16x8 v; } w, x;
+      w.u = uw;
+      x.u = ux;
+      acc = VCA_MFMA_16x16x32(w.v, x.v, acc);
+    } else {
+      union { uint4 u; float f[4]; } w, x;
+      w.u = uw;
+      x.u = ux;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(w.f[e], x.f[e], acc, 0, 0, 0);
+    }
+  };
+  const int nc = (g.K + CK - 1) / CK;
+  int c = wave;
+  for (; c + (UNROLL - 1) * FEW_WAVES < nc - 1; c += UNROLL * FEW_WAVES) {     // whole chunks only
+    uint4 w[UNROLL], x[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int k = (c + u * FEW_WAVES) * CK + lg * EPP;
+      w[u] = reinterpret_cast<const Any16*>(wp + k)->u;
+      x[u] = reinterpret_cast<const Any16*>(xp + k)->u;
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) mul(w[u], x[u]);
+  }
+  for (; c < nc; c += FEW_WAVES) mul(load(wp, c), load(xp, c));
+  red[wave][lane] = acc;
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int w = 1; w < FEW_WAVES; ++w) acc += red[w][lane];
+  const int n = n0 + 4 * lg;
+  if (lc < g.M && n < g.N) {
+    float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+    finish<T, 4>(g, lc, n, v);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// dz = gy act'(z) and the columns' sums of it.  A workgroup takes a strip of 32 x 16 bytes of columns and a range of
+// rows (8 at a time); its column sums (of the unrounded dz, fp32) go to a slab, slabs are added in order.
+// ------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void act_bwd_kernel(int M, int N, int act, float slope, const T* __restrict__ gy,
+                                                      const T* __restrict__ z, T* __restrict__ dz,
+                                                      float* __restrict__ part, int rows) {
+  constexpr int V = 16 / (int)sizeof(T);
+  __shared__ float red[8][32 * V];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int n = (blockIdx.x * 32 + tx) * V;
+  const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
+  float s[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) s[e] = 0.f;
+  if (n + V <= N) {
+    for (int r = r0 + ty; r < r1; r += 8) {
+      const size_t o = (size_t)r * N + n;
+      Vec16<T> a, b, d;
+      a.u = reinterpret_cast<const Any16*>(gy + o)->u;
+      if (z) b.u = reinterpret_cast<const Any16*>(z + o)->u;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float v = (float)a.e[e];
+        if (z) v *= act_slope((float)b.e[e], act, slope);
+        s[e] += v;
+        d.e[e] = (T)v;
+      }
+      if (dz) reinterpret_cast<Any16*>(dz + o)->u = d.u;
+    }
+  } else if (n < N) {
+    for (int r = r0 + ty; r < r1; r += 8) {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (n + e < N) {
+          const size_t o = (size_t)r * N + n + e;
+          float v = (float)gy[o];
+          if (z) v *= act_slope((float)z[o], act, slope);
+          s[e] += v;
+          if (dz) dz[o] = (T)v;
+        }
+    }
+  }
+  if (!part) return;
+#pragma unroll
+  for (int e = 0; e < V; ++e) red[ty][tx * V + e] = s[e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * V; i += 256) {
+    float t = 0.f;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) t += red[y][i];
+    const int col = blockIdx.x * 32 * V + i;
+    if (col < N) part[(size_t)blockIdx.y * N + col] = t;
+  }
+}
+
+// db[n] (+)= sum of the slabs: 16 columns a workgroup, each column's slabs in 16 interleaved runs
+template <typename T>
+__global__ __launch_bounds__(256) void bias_fold_kernel(int N, int slabs, const float* __restrict__ part,
+                                                        T* __restrict__ db, int add) {
+  __shared__ float red[16][17];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, n = blockIdx.x * 16 + tx;
+  float t = 0.f;
+  if (n < N) {
+#pragma unroll 8
+    for (int s = ty; s < slabs; s += 16) t += part[(size_t)s * N + n];
+  }
+  red[ty][tx] = t;
+  __syncthreads();
+  if (ty || n >= N) return;
+#pragma unroll
+  for (int y = 1; y < 16; ++y) t += red[y][tx];
+  db[n] = (T)(add ? t + (float)db[n] : t);
+}
+
+// ------------------------------------------------------------------------------------------------
+// host
+// ------------------------------------------------------------------------------------------------
+bool act_ok(int act) { return (act >= VCA_ACT_NONE && act <= VCA_ACT_SILU) && act != VCA_ACT_PRELU; }
+
+int mode_of(const vca_matmul_desc& d) {
+  if (d.type == VCA_T_F32) return d.nsplit == 0 ? MODE_F32 : d.nsplit == 3 ? MODE_S3 : d.nsplit == 1 ? MODE_S1 : -1;
+  return d.type == (VCA_ELEM_TYPE ? VCA_T_F16 : VCA_T_BF16) && d.nsplit == 1 ? MODE_16 : -1;
+}
+
+struct Plan {
+  MatArgs g;
+  int mode, tile;                     // 128 or 256; 0: few rows
+  bool dma;
+};
+
+int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p) {
+  VCA_CHECK_ARG(dp);
+  const vca_matmul_desc& d = *dp;
+  p.mode = mode_of(d);
+  VCA_CHECK_ARG(p.mode >= 0 && d.M > 0 && d.N > 0 && d.K > 0 && act_ok(d.act));
+  VCA_CHECK_ARG(!(d.a_col && !d.b_col));                   // no product here reads only its rows by columns
+  const int esz = d.type == VCA_T_F32 ? 4 : 2, bk = 128 / esz;
+  VCA_CHECK_ARG(d.lda >= (d.a_col ? d.M : (d.M > 1 ? d.K : 0)) && d.ldb >= (d.b_col ? d.N : (d.N > 1 ? d.K : 0)) &&
+                d.ldc >= (d.M > 1 ? d.N : 0) && d.ldr >= 0);
+  MatArgs& g = p.g;
+  g.M = d.M;
+  g.N = d.N;
+  g.K = d.K;
+  g.lda = d.lda;
+  g.ldb = d.ldb;
+  g.ldc = d.ldc;
+  g.ldr = d.ldr;
+  g.act = d.act;
+  g.slope = d.slope;
+  g.npad = (d.N + 7) / 8 * 8;
+  g.part = nullptr;
+  g.ksplit = 1;
+  g.cpz = (d.K + bk - 1) / bk;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) |
+                         (uintptr_t)(d.lda * esz) | (uintptr_t)(d.ldb * esz);
+  const int per16 = 16 / esz;
+  p.dma = (bits & 15) == 0 && (!d.a_col || d.M % per16 == 0) && (!d.b_col || d.N % per16 == 0);
+  if (d.M <= 16 && !d.a_col && !d.b_col && (p.mode == MODE_16 || p.mode == MODE_F32)) {
+    p.tile = 0;
+    return 0;
+  }
+  auto tiles = [&](int t) { return (long long)((d.M + t - 1) / t) * ((d.N + t - 1) / t); };
+  p.tile = p.mode == MODE_16 && p.dma && tiles(256) >= 192 ? 256 : 128;
+  g.ntm = (d.M + p.tile - 1) / p.tile;
+  g.ntn = (d.N + p.tile - 1) / p.tile;
+  VCA_CHECK_ARG(tiles(p.tile) < (1 << 24));
+  const int nt = g.ntm * g.ntn, nc = g.cpz;
+  // few tiles: split the reduction over workgroups until the chip is covered, four chunks a range at least
+  int ks = 1;
+  while (nt * ks < 384 && nc / (ks + 1) >= 4 && ks < 32) ++ks;
+  g.cpz = (nc + ks - 1) / ks;
+  g.ksplit = (nc + g.cpz - 1) / g.cpz;
+  return 0;
+}
+
+template <int MODE, bool AKC, bool BKC, int BM, int NWM, int NWN, bool DMA>
+int launch_tile(const MatArgs& g, hipStream_t s) {
+  const size_t lds = 2 * (size_t)(BM + BM) * 128;
+  if (lds > 64 * 1024) VCA_MAX_LDS((matmul_kernel<MODE, AKC, BKC, BM, BM, NWM, NWN, DMA>));
+  hipLaunchKernelGGL((matmul_kernel<MODE, AKC, BKC, BM, BM, NWM, NWN, DMA>), dim3(g.ntm * g.ntn * g.ksplit),
+                     dim3(NWM * NWN * 64), lds, s, g);
+  return vca_launch_status();
+}
+
+template <int MODE, bool AKC, bool BKC>
+int launch_layout(const Plan& p, hipStream_t s) {
+  if (MODE == MODE_16 && p.tile == 256) return launch_tile<MODE_16, AKC, BKC, 256, 2, 4, true>(p.g, s);
+  return p.dma ? launch_tile<MODE, AKC, BKC, 128, 2, 2, true>(p.g, s)
+               : launch_tile<MODE, AKC, BKC, 128, 2, 2, false>(p.g, s);
+}
+
+template <int MODE>
+int launch_mode(const Plan& p, bool a_col, bool b_col, hipStream_t s) {
+  if (a_col) return launch_layout<MODE, false, false>(p, s);
+  if (b_col) return launch_layout<MODE, true, false>(p, s);
+  return launch_layout<MODE, true, true>(p, s);
+}
+
+int act_rows(int M, int N, int esz) {                     // rows a workgroup of act_bwd_kernel takes
+  const long long strips = ((long long)N * esz + 511) / 512;
+  int rows = 8;
+  auto slabs = [&]() { return ((long long)M + rows - 1) / rows; };
+  while ((rows < 256 && strips * slabs() > 1024) || slabs() > 65535) rows *= 2;   // (65535: the grid's second dimension)
+  return rows;
+}
+
+}  // namespace
+
+extern "C" long long vca_matmul_act_ws_floats(const vca_matmul_desc* d, const void* a, const void* b) {
+  Plan p;
+  if (plan_of(d, a, b, p) != 0) return 0;
+  return p.tile && p.g.ksplit > 1 ? (long long)p.g.ksplit * p.g.M * p.g.npad : 0;
+}
+
+extern "C" int vca_matmul_act(const vca_matmul_desc* d, const void* a, const void* b, const void* bias, const void* res,
+                              void* c, void* z, float* ws, long long ws_floats, void* stream) {
+  Plan p;
+  VCA_CHECK_ARG(a && b && c);
+  const int rc = plan_of(d, a, b, p);
+  if (rc) return rc;
+  const int esz = d->type == VCA_T_F32 ? 4 : 2;
+  VCA_CHECK_ARG(((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(bias) |
+                  reinterpret_cast<uintptr_t>(res) | reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(z)) &
+                 (esz - 1)) == 0);
+  MatArgs& g = p.g;
+  g.a = a;
+  g.b = b;
+  g.bias = bias;
+  g.res = res;
+  g.c = c;
+  g.z = z;
+  hipStream_t s = (hipStream_t)stream;
+  if (p.tile == 0) {
+    const dim3 grid((g.N + 15) / 16);
+    if (p.mode == MODE_16) hipLaunchKernelGGL(few_rows_kernel<MODE_16>, grid, dim3(FEW_WAVES * 64), 0, s, g);
+    else hipLaunchKernelGGL(few_rows_kernel<MODE_F32>, grid, dim3(FEW_WAVES * 64), 0, s, g);
+    return vca_launch_status();
+  }
+  if (g.ksplit > 1) {
+    VCA_CHECK_ARG(ws && ws_floats >= (long long)g.ksplit * g.M * g.npad && (reinterpret_cast<uintptr_t>(ws) & 15) == 0);
+    g.part = ws;
+  }
+  int e = 0;
+  const bool ac = d->a_col != 0, bc = d->b_col != 0;
+  switch (p.mode) {
+    case MODE_16: e = launch_mode<MODE_16>(p, ac, bc, s); break;
+    case MODE_F32: e = launch_mode<MODE_F32>(p, ac, bc, s); break;
+    case MODE_S3: e = launch_mode<MODE_S3>(p, ac, bc, s); break;
+    default: e = launch_mode<MODE_S1>(p, ac, bc, s); break;
+  }
+  if (e || g.ksplit == 1) return e;
+  const size_t nv = (size_t)g.M * (g.npad / (16 / esz));
+  const dim3 grid((unsigned)(nv / 256 + 1 > 4096 ? 4096 : nv / 256 + 1));
+  if (esz == 4) hipLaunchKernelGGL(matmul_fold_kernel<float>, grid, dim3(256), 0, s, g);
+  else hipLaunchKernelGGL(matmul_fold_kernel<vca_e16>, grid, dim3(256), 0, s, g);
+  return vca_launch_status();
+}
+
+extern "C" long long vca_act_bwd_ws_floats(int type, int M, int N) {
+  if (M <= 0 || N <= 0 || type < VCA_T_F32 || type > VCA_T_F16) return 0;
+  const int rows = act_rows(M, N, type == VCA_T_F32 ? 4 : 2);
+  return ((long long)M + rows - 1) / rows * N;
+}
+
+extern "C" int vca_act_bwd(int type, int M, int N, int act, float slope, const void* gy, const void* z, void* dz, void* db,
+                           int db_add, float* ws, long long ws_floats, void* stream) {
+  const int own16 = VCA_ELEM_TYPE ? VCA_T_F16 : VCA_T_BF16;
+  VCA_CHECK_ARG((type == VCA_T_F32 || type == own16) && M > 0 && N > 0 && act_ok(act) && gy && (dz || db));
+  VCA_CHECK_ARG((act == VCA_ACT_NONE) == !z && (!dz || z));
+  const int esz = type == VCA_T_F32 ? 4 : 2, rows = act_rows(M, N, esz), slabs = (int)(((long long)M + rows - 1) / rows);
+  VCA_CHECK_ARG(((reinterpret_cast<uintptr_t>(gy) | reinterpret_cast<uintptr_t>(z) | reinterpret_cast<uintptr_t>(dz) |
+                  reinterpret_cast<uintptr_t>(db)) & (esz - 1)) == 0);
+  VCA_CHECK_ARG(!db || (ws && ws_floats >= (long long)slabs * N && (reinterpret_cast<uintptr_t>(ws) & 3) == 0));
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 grid((unsigned)(((long long)N * esz + 511) / 512), (unsigned)slabs);
+  float* part = db ? ws : nullptr;
+  if (esz == 4)
+    hipLaunchKernelGGL(act_bwd_kernel<float>, grid, dim3(256), 0, s, M, N, act, slope, (const float*)gy, (const float*)z,
+                       (float*)dz, part, rows);
+  else
+    hipLaunchKernelGGL(act_bwd_kernel<vca_e16>, grid, dim3(256), 0, s, M, N, act, slope, (const vca_e16*)gy,
+                       (const vca_e16*)z, (vca_e16*)dz, part, rows);
+  if (db) {
+    const dim3 fg((N + 15) / 16);
+    if (esz == 4) hipLaunchKernelGGL(bias_fold_kernel<float>, fg, dim3(256), 0, s, N, slabs, ws, (float*)db, db_add);
+    else hipLaunchKernelGGL(bias_fold_kernel<vca_e16>, fg, dim3(256), 0, s, N, slabs, ws, (vca_e16*)db, db_add);
+  }
+  return vca_launch_status();
+}
