@@ -530,13 +530,13 @@ int vca_loss_scale_update(float* scale, int* state, float growth, float backoff,
  * type: VCA_T_F32, or the 16-bit type of this build (vca_elem_type).  nsplit: products per element pair, 1 for 16-bit
  * tensors; fp32 tensors 0 (exact fp32 MFMA), 3 or 1 (split into / rounded to 16 bits in registers).
  * act: 0 none, 1 leaky (slope), 3 relu, 4 tanh, 5 gelu (erf), 6 gelu (tanh form), 7 silu.
- * ws: vca_matmul_act_ws_floats(d, a, b) floats for the partial products of a reduction split over workgroups (0: none). */
+ * ws: vca_matmul_act_ws_floats(d) floats for the partial products of a reduction split over workgroups (0: none). */
 typedef struct {
   int M, N, K, type, nsplit, a_col, b_col, act;
   float slope;
   long long lda, ldb, ldc, ldr;
 } vca_matmul_desc;
-long long vca_matmul_act_ws_floats(const vca_matmul_desc* d, const void* a, const void* b);
+long long vca_matmul_act_ws_floats(const vca_matmul_desc* d);
 int vca_matmul_act(const vca_matmul_desc* d, const void* a, const void* b, const void* bias, const void* res, void* c,
                    void* z, float* ws, long long ws_floats, void* stream);
 
@@ -546,6 +546,20 @@ int vca_matmul_act(const vca_matmul_desc* d, const void* a, const void* b, const
 long long vca_act_bwd_ws_floats(int type, int M, int N);
 int vca_act_bwd(int type, int M, int N, int act, float slope, const void* gy, const void* z, void* dz, void* db,
                 int db_add, float* ws, long long ws_floats, void* stream);
+
+/* The backward pass of y = act(x W^T + bias) + res in one call: dz and db as vca_act_bwd (with act 0, z and dz are NULL
+ * and dz is gy), then dx = dz W and dw = dz^T x as vca_matmul_act.  gy, z, dz [M][N], dx [M][K], dw [N][K] dense, x and w
+ * with row strides ldx and ldw.  dx, dw, db may be NULL; dw_add / db_add: add to what is there.  ws: at least
+ * vca_linear_act_bwd_ws_floats(b) floats (its pointers are not looked at by the query), used by the launches in turn. */
+typedef struct {
+  int M, N, K, type, nsplit, act, dw_add, db_add;
+  float slope;
+  long long ldx, ldw;
+  const void *gy, *x, *w, *z;
+  void *dz, *dx, *dw, *db;
+} vca_linear_bwd;
+long long vca_linear_act_bwd_ws_floats(const vca_linear_bwd* b);
+int vca_linear_act_bwd(const vca_linear_bwd* b, float* ws, long long ws_floats, void* stream);
 
 /* Global norm of ntensor gradient tensors and clipping by it (torch.nn.utils.clip_grad_norm_ with the 2-norm; the
  * reference trains without clipping).  h_ptrs / h_numel / h_types are host arrays, read before the call returns:

@@ -264,7 +264,7 @@ def test_rows_of_the_output_beyond_it_stay():
         x, w, _, _, _ = _inputs(M, K, N, torch.float32, 4)
         c = torch.full((M + 2, N + 5), 7.5, device='cuda')
         d = _lib.MatmulDesc(M, N, K, 0, 0, 0, 0, 0, 0.0, K, K, N + 5, 0)
-        n = L.vca_matmul_act_ws_floats(d, x.data_ptr(), w.data_ptr())
+        n = L.vca_matmul_act_ws_floats(d)
         ws = torch.empty(n + 4, device='cuda')
         ws[n:] = 3.25
         assert L.vca_matmul_act(d, x.data_ptr(), w.data_ptr(), None, None, c.data_ptr(), None, ws.data_ptr(), n,
@@ -417,7 +417,7 @@ def test_entry_points_refuse_before_any_launch():
                    dict(a=66), dict(bias=65)):
             assert call(**kw) == -22, kw
         long = dict(K=1 << 16, lda=1 << 16, ldb=1 << 16)
-        n = L.vca_matmul_act_ws_floats(_lib.MatmulDesc(**dict(ok, **long)), 64, 64)
+        n = L.vca_matmul_act_ws_floats(_lib.MatmulDesc(**dict(ok, **long)))
         assert n > 0 and n % (64 * 64) == 0
         assert call(ws=None, **long) == -22 and call(n=n - 1, **long) == -22 and call(ws=68, **long) == -22
         f = lambda type=0, M=4, N=4, act=6, gy=64, z=64, dz=64, db=64, ws=64, n=1 << 20: L.vca_act_bwd(
@@ -426,3 +426,12 @@ def test_entry_points_refuse_before_any_launch():
                    dict(dz=None, db=None), dict(ws=None), dict(n=3), dict(act=0), dict(act=0, z=None), dict(z=66)):
             assert f(**kw) == -22, kw
         assert L.vca_act_bwd_ws_floats(0, 0, 4) == 0
+        bwd = dict(M=64, N=64, K=64, type=0, nsplit=0, act=6, dw_add=0, db_add=0, slope=0.0, ldx=64, ldw=64, gy=64, x=64,
+                   w=64, z=64, dz=64, dx=64, dw=64, db=64)
+        n = L.vca_linear_act_bwd_ws_floats(_lib.LinearBwd(**bwd))
+        assert n > 0
+        g = lambda ws=64, n=n, **kw: L.vca_linear_act_bwd(_lib.LinearBwd(**dict(bwd, **kw)), ws, n, None)
+        for kw in (dict(gy=None), dict(M=0), dict(K=0), dict(act=0), dict(act=2), dict(z=None), dict(dz=None),
+                   dict(type=other, nsplit=1), dict(nsplit=2), dict(w=None), dict(x=None), dict(ldx=63), dict(ldw=63),
+                   dict(n=n - 1), dict(ws=None), dict(ws=72)):
+            assert g(**kw) == -22, kw

@@ -94,6 +94,12 @@ class MatmulDesc(ctypes.Structure):
         [('slope', ctypes.c_float)] + [(n, ctypes.c_longlong) for n in ('lda', 'ldb', 'ldc', 'ldr')]
 
 
+class LinearBwd(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ('M', 'N', 'K', 'type', 'nsplit', 'act', 'dw_add', 'db_add')] + \
+        [('slope', ctypes.c_float)] + [(n, ctypes.c_longlong) for n in ('ldx', 'ldw')] + \
+        [(n, ctypes.c_void_p) for n in ('gy', 'x', 'w', 'z', 'dz', 'dx', 'dw', 'db')]
+
+
 class AdamGroup(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ('p', 'g', 'm', 'v', 'vmax')] + [('n', ctypes.c_longlong)]
 
@@ -191,10 +197,12 @@ _SIGS = {
     'vca_loss_scale_count': ([_P, _P, _P], _I),
     'vca_adam_scaled_f32': ([_LL, _P, _P, _P, _P, _P, _F, _F, _F, _F, _P, _P, _P, _P, _P], _I),
     'vca_loss_scale_update': ([_P, _P, _F, _F, _I, _P], _I),
-    'vca_matmul_act_ws_floats': ([ctypes.POINTER(MatmulDesc), _P, _P], _LL),
+    'vca_matmul_act_ws_floats': ([ctypes.POINTER(MatmulDesc)], _LL),
     'vca_matmul_act': ([ctypes.POINTER(MatmulDesc)] + [_P] * 7 + [_LL, _P], _I),
     'vca_act_bwd_ws_floats': ([_I, _I, _I], _LL),
     'vca_act_bwd': ([_I, _I, _I, _I, _F, _P, _P, _P, _P, _I, _P, _LL, _P], _I),
+    'vca_linear_act_bwd_ws_floats': ([ctypes.POINTER(LinearBwd)], _LL),
+    'vca_linear_act_bwd': ([ctypes.POINTER(LinearBwd), _P, _LL, _P], _I),
     'vca_grad_norm_ws_doubles': ([_I], _LL),
     'vca_grad_norm': ([_I, _P, _P, _P, _P, _P, _LL, _P, _P], _I),
     'vca_grad_clip': ([_I, _P, _P, _P, _F, _P, _P, _LL, _P, _P], _I),
@@ -234,7 +242,7 @@ def ptr(t):
 
 
 def stream():
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def check(rc, what):

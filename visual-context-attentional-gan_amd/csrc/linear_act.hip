@@ -12,6 +12,8 @@
 // Arithmetic: 16-bit tensors of the library's element type take one product with fp32 accumulation.  fp32 tensors take
 // the exact fp32 MFMA (nsplit 0) or are split in registers into 16-bit parts (nsplit 3: hi hi + hi lo + lo hi; 1: hi).
 // Bias, activation and residual are applied to the fp32 accumulator, so a result is rounded once.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -247,6 +249,11 @@ struct Operand {
   }
 };
 
+// (The restrict gives the read alias information; without any the compiler waits for every LDS-DMA in flight before it.)
+__device__ __forceinline__ s16x4 read_transposed(const char* __restrict__ p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
+
 // Fragment loads.  sub: first of the 16 rows or columns of C; lane = 16 g + lc.
 template <bool KC, int R>
 __device__ __forceinline__ bf16x8 frag16(const char* s, int sub, int kk, int lc, int g) {
@@ -254,8 +261,8 @@ __device__ __forceinline__ bf16x8 frag16(const char* s, int sub, int kk, int lc,
   const int k = kk * 32 + 8 * g + (lc >> 2);
   const char* p = s + k * (R * 2) + (((sub >> 4) ^ ((k & 3) | ((k >> 1) & 4))) << 5) + (lc & 3) * 8;
   union { s16x4 h[2]; bf16x8 v; } f;
-  f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
-  f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * R * 2));
+  f.h[0] = read_transposed(p);
+  f.h[1] = read_transposed(p + 4 * R * 2);
   return f.v;
 }
 
@@ -309,6 +316,57 @@ __device__ __forceinline__ void tile_of(const MatArgs& g, int& tm, int& tn, int&
   t -= grp * band;
   tm = m0 + t % rows;
   tn = t / rows;
+}
+
+// The end of a tile.  A split reduction stores its partial tile as it is.  Otherwise the accumulators pass through LDS
+// (fp32, 16-byte pieces of a row XOR-ed with the row) so that a thread finishes 16 bytes of a row of C and a wave writes
+// whole lines, in as many parts as the tile is larger than the LDS of the two stages.
+template <typename T, int BM, int BN, int NWM, int NWN>
+__device__ __forceinline__ void store_tile(const MatArgs& g, const f32x4 (&acc)[BM / NWM / 16][BN / NWN / 16], char* smem,
+                                           int m0, int n0, int kz, int wm, int wn, int lc, int lg, int tid) {
+  constexpr int NT = NWM * NWN * 64, TM = BM / NWM / 16, TN = BN / NWN / 16;
+  if (g.ksplit > 1) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int m = m0 + (wm * TM + i) * 16 + lc;
+      if (m >= g.M) continue;
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int n = n0 + (wn * TN + j) * 16 + 4 * lg;
+        if (n < g.npad)
+          *reinterpret_cast<f32x4*>(g.part + ((size_t)kz * g.M + m) * g.npad + n) = acc[i][j];
+      }
+    }
+    return;
+  }
+  constexpr int V = 16 / (int)sizeof(T), PARTS = BM * BN * 4 / (2 * (BM + BN) * 128) < 1 ? 1 : BM * BN * 4 / (2 * (BM + BN) * 128);
+  constexpr int HM = TM / PARTS, TPR = BN / V;
+#pragma unroll
+  for (int h = 0; h < PARTS; ++h) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < HM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int row = (wm * HM + i) * 16 + lc, pc = (wn * TN + j) * 4 + lg;
+        *reinterpret_cast<f32x4*>(smem + row * (BN * 4) + ((pc ^ lc) << 4)) = acc[h * HM + i][j];
+      }
+    __syncthreads();
+#pragma unroll 1
+    for (int q = tid; q < NWM * HM * 16 * TPR; q += NT) {
+      const int row = q / TPR, col = (q % TPR) * V;
+      const int m = m0 + (row / (HM * 16) * TM + h * HM) * 16 + row % (HM * 16), n = n0 + col;
+      if (m >= g.M || n >= g.N) continue;
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; e += 4) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(smem + row * (BN * 4) + ((((col + e) >> 2) ^ (row & 15)) << 4));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[e + r] = t[r];
+      }
+      finish<T, V>(g, m, n, v);
+    }
+  }
 }
 
 template <int MODE, bool AKC, bool BKC, int BM, int BN, int NWM, int NWN, bool DMA>
@@ -423,49 +481,167 @@ __global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g)
     }
   }
 
-  if (g.ksplit > 1) {
+  store_tile<T, BM, BN, NWM, NWN>(g, acc, smem, m0, n0, kz, wm, wn, lc, lg, tid);
+}
+
+// ------------------------------------------------------------------------------------------------
+// The tiled product for large 16-bit ones: 256 x 256 tiles, four waves of 128 x 128 each.  LDS carries 2 x 64 KB stages
+// and feeds each wave 2 x 16 KB of fragments a chunk: half of what eight waves of 128 x 64 would read, and three
+// quarters of the time the matrix cores need for the chunk.  One wave a SIMD has nobody to hide behind, so the wave
+// overlaps by itself: while the 64 MFMAs of one half chunk run, the 16 fragments of the next half are read (the second
+// half of chunk c, then the first of chunk c + 1), an LDS read between every few MFMAs.  The chunk's only barrier sits
+// in its middle: there every wave has its last fragments of chunk c in registers, chunk c + 1 has landed (it was sent a
+// whole chunk earlier), and chunk c's stage is free to be refilled with chunk c + 2.
+// ------------------------------------------------------------------------------------------------
+template <bool KC>
+struct WideOperand {
+  static constexpr int NT = 512, PIECES = 4;
+  const char* at;                     // the tile's first element of the next chunk to fetch: uniform
+  long long step;                     // bytes a chunk
+  unsigned off[PIECES];               // this thread's pieces, relative to it
+
+  __device__ __forceinline__ void init(const void* p, long long ld, int o0, int outer, int c0, int tid) {
+    const long long ldb = ld * 2;
+    at = reinterpret_cast<const char*>(p) + (KC ? o0 * ldb + c0 * 128ll : c0 * 64 * ldb + o0 * 2ll);
+    step = KC ? 128 : 64 * ldb;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int m = m0 + (wm * TM + i) * 16 + lc;
-      if (m >= g.M) continue;
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int n = n0 + (wn * TN + j) * 16 + 4 * lg;
-        if (n < g.npad)
-          *reinterpret_cast<f32x4*>(g.part + ((size_t)kz * g.M + m) * g.npad + n) = acc[i][j];
+    for (int it = 0; it < PIECES; ++it) {
+      const int q = it * NT + tid;
+      if (KC) {
+        const int row = q >> 3;
+        off[it] = (unsigned)(min(row, outer - 1 - o0) * (int)ldb + ((q & 7) ^ (row & 7)) * 16);
+      } else {
+        const int k = q >> 5, pc = (q & 31) ^ col_swizzle<MODE_16, 256>(k);
+        off[it] = (unsigned)(k * (int)ldb + min(pc * 8, outer - 8 - o0) * 2);
       }
     }
-    return;
   }
-  // The accumulators pass through LDS (fp32, 16-byte pieces of a row XOR-ed with the row) so that a thread finishes 16
-  // bytes of a row of C and a wave writes whole lines, in one or two halves of each wave's rows.
-  constexpr int V = 16 / (int)sizeof(T), HALVES = BM * BN * 4 > 2 * STAGE ? 2 : 1, HM = TM / HALVES, TPR = BN / V;
+
+  __device__ __forceinline__ void dma(char* stage, int wave, int it) const {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(at + off[it]),
+                                     (__attribute__((address_space(3))) void*)(stage + (it * NT + wave * 64) * 16), 16,
+                                     0, 0);
+  }
+};
+
+template <bool AKC, bool BKC>
+__global__ __launch_bounds__(512) void matmul_wide_kernel(const MatArgs g) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr int BM = 256, STAGE = 2 * BM * 128, TM = 8, TN = 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lc = lane & 15, lg = lane >> 4, wm = wave >> 2, wn = wave & 3;
+  int tm, tn, kz;
+  tile_of(g, tm, tn, kz);
+  const int m0 = tm * BM, n0 = tn * BM;
+  const int c0 = kz * g.cpz, c1 = min((g.K + 63) / 64, c0 + g.cpz), whole = max(c0, min(c1, g.K / 64));
+
+  f32x4 acc[TM][TN];
 #pragma unroll
-  for (int h = 0; h < HALVES; ++h) {
-    __syncthreads();
+  for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int i = 0; i < HM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int row = (wm * HM + i) * 16 + lc, pc = (wn * TN + j) * 4 + lg;
-        *reinterpret_cast<f32x4*>(smem + row * (BN * 4) + ((pc ^ lc) << 4)) = acc[h * HM + i][j];
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // Fragment addresses as frag16's, but from one lane offset an operand: a fragment's place (sub = 16 i) is a constant
+  // added where k is contiguous, a constant XOR-ed where it is not (a row of k has 16 blocks, i sits in the swizzled
+  // bits), and so is kk the other way round.
+  auto lane_off = [&](bool kc, int sub) {
+    if (kc) return (unsigned)((sub + lc) * 128 + ((lg ^ (lc & 7)) << 4));
+    const int k = 8 * lg + (lc >> 2);
+    return (unsigned)(k * 512 + (((sub >> 4) ^ ((k & 3) | ((k >> 1) & 4))) << 5) + (lc & 3) * 8);
+  };
+  const unsigned oa = lane_off(AKC, wm * TM * 16), ob = lane_off(BKC, wn * TN * 16);
+  auto read_frag = [&](bool kc, unsigned o, const char* image, int kk, int i) {
+    if (kc) return *reinterpret_cast<const bf16x8*>(image + (o ^ (kk << 6)) + i * 2048);
+    const char* p = image + (o ^ (i << 5)) + kk * 16384;
+    union { s16x4 h[2]; bf16x8 v; } f;
+    f.h[0] = read_transposed(p);
+    f.h[1] = read_transposed(p + 2048);
+    return f.v;
+  };
+  auto read_a = [&](const char* st, int kk, int i) { return read_frag(AKC, oa, st, kk, i); };
+  auto read_b = [&](const char* st, int kk, int j) { return read_frag(BKC, ob, st + BM * 128, kk, j); };
+
+  if (c0 < whole) {
+    WideOperand<AKC> A;
+    WideOperand<BKC> B;
+    A.init(g.a, g.lda, m0, g.M, c0, tid);
+    B.init(g.b, g.ldb, n0, g.N, c0, tid);
+    auto send = [&](char* st, int it) {                   // one of the eight pieces a thread sends of a chunk
+      if (it < 4) A.dma(st, wave, it);
+      else B.dma(st + BM * 128, wave, it - 4);
+      if (it == 7) {
+        A.at += A.step;
+        B.at += B.step;
       }
+    };
+    bf16x8 fa[TM], fb0[TN], fb1[TN];
+#pragma unroll
+    for (int it = 0; it < 8; ++it) send(smem, it);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-#pragma unroll 1
-    for (int q = tid; q < NWM * HM * 16 * TPR; q += NT) {
-      const int row = q / TPR, col = (q % TPR) * V;
-      const int m = m0 + (row / (HM * 16) * TM + h * HM) * 16 + row % (HM * 16), n = n0 + col;
-      if (m >= g.M || n >= g.N) continue;
-      float v[V];
+    if (c0 + 1 < whole) {
 #pragma unroll
-      for (int e = 0; e < V; e += 4) {
-        const f32x4 t = *reinterpret_cast<const f32x4*>(smem + row * (BN * 4) + ((((col + e) >> 2) ^ (row & 15)) << 4));
+      for (int it = 0; it < 8; ++it) send(smem + STAGE, it);
+    }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[e + r] = t[r];
+    for (int j = 0; j < TN; ++j) fb0[j] = read_b(smem, 0, j);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fa[i] = read_a(smem, 0, i);
+    // One half chunk: its MFMAs row by row, and behind each row that row's fragment of the next half (half kk of stage
+    // st) and, in the second half, one piece of the chunk after the next.
+    auto half = [&](const bf16x8 (&fb)[TN], const char* st, int kk, bf16x8 (&nb)[TN], char* to, auto sends) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        if constexpr (decltype(sends)::value) send(to, i);
+        if (i < TN) nb[i] = read_b(st, kk, i);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = VCA_MFMA_16x16x32(fb[j], fa[i], acc[i][j]);
+        fa[i] = read_a(st, kk, i);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      finish<T, V>(g, m, n, v);
+    };
+    // chunk c + 1 has landed, and chunk c's last fragments are in registers
+    auto meet = [&]() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    int c = c0;
+    for (; c + 2 < whole; ++c) {
+      char* st = smem + ((c - c0) & 1) * STAGE;
+      half(fb0, st, 1, fb1, nullptr, std::false_type());
+      meet();
+      half(fb1, smem + ((c - c0 + 1) & 1) * STAGE, 0, fb0, st, std::true_type());
+    }
+    for (; c < whole; ++c) {                              // the last two: nothing left to send
+      half(fb0, smem + ((c - c0) & 1) * STAGE, 1, fb1, nullptr, std::false_type());
+      meet();
+      // (behind the last chunk this reads the other stage's old contents, which nothing uses)
+      half(fb1, smem + ((c - c0 + 1) & 1) * STAGE, 0, fb0, nullptr, std::false_type());
     }
   }
+  if (whole < c1) {                                       // the reduction's partial chunk, through registers
+    Operand<MODE_16, AKC, BM, 512> A;
+    Operand<MODE_16, BKC, BM, 512> B;
+    A.init(g.a, g.lda, m0, g.M, g.K, tid);
+    B.init(g.b, g.ldb, n0, g.N, g.K, tid);
+    uint4 ra[A.PIECES], rb[B.PIECES];
+    A.fetch(whole, ra);
+    B.fetch(whole, rb);
+    __syncthreads();
+    A.put(smem, ra);
+    B.put(smem + BM * 128, rb);
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      bf16x8 fb[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fb[j] = read_b(smem, kk, j);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const bf16x8 fa = read_a(smem, kk, i);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = VCA_MFMA_16x16x32(fb[j], fa, acc[i][j]);
+      }
+    }
+  }
+  store_tile<vca_e16, BM, BM, 2, 4>(g, acc, smem, m0, n0, kz, wm, wn, lc, lg, tid);
 }
 
 // C from the ksplit partial products, added in order of the reduction, through the same epilogue
@@ -690,7 +866,7 @@ int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p) {
   const int nt = g.ntm * g.ntn, nc = g.cpz;
   // few tiles: split the reduction over workgroups until the chip is covered, four chunks a range at least
   int ks = 1;
-  while (nt * ks < 384 && nc / (ks + 1) >= 4 && ks < 32) ++ks;
+  while (nt * ks < 256 && nc / (ks + 1) >= 4 && ks < 32) ++ks;
   g.cpz = (nc + ks - 1) / ks;
   g.ksplit = (nc + g.cpz - 1) / g.cpz;
   return 0;
@@ -707,7 +883,11 @@ int launch_tile(const MatArgs& g, hipStream_t s) {
 
 template <int MODE, bool AKC, bool BKC>
 int launch_layout(const Plan& p, hipStream_t s) {
-  if (MODE == MODE_16 && p.tile == 256) return launch_tile<MODE_16, AKC, BKC, 256, 2, 4, true>(p.g, s);
+  if (MODE == MODE_16 && p.tile == 256) {
+    VCA_MAX_LDS((matmul_wide_kernel<AKC, BKC>));
+    hipLaunchKernelGGL((matmul_wide_kernel<AKC, BKC>), dim3(p.g.ntm * p.g.ntn * p.g.ksplit), dim3(512), 128 * 1024, s, p.g);
+    return vca_launch_status();
+  }
   return p.dma ? launch_tile<MODE, AKC, BKC, 128, 2, 2, true>(p.g, s)
                : launch_tile<MODE, AKC, BKC, 128, 2, 2, false>(p.g, s);
 }
@@ -717,6 +897,18 @@ int launch_mode(const Plan& p, bool a_col, bool b_col, hipStream_t s) {
   if (a_col) return launch_layout<MODE, false, false>(p, s);
   if (b_col) return launch_layout<MODE, true, false>(p, s);
   return launch_layout<MODE, true, true>(p, s);
+}
+
+// Workspace floats of a product, whatever its operands' alignment.
+long long ws_floats_of(const vca_matmul_desc* d) {
+  long long n = 0;
+  for (uintptr_t at : {(uintptr_t)16, (uintptr_t)4}) {
+    Plan p;
+    if (plan_of(d, reinterpret_cast<const void*>(at), reinterpret_cast<const void*>(at), p) != 0) return 0;
+    const long long f = p.tile && p.g.ksplit > 1 ? (long long)p.g.ksplit * p.g.M * p.g.npad : 0;
+    n = f > n ? f : n;
+  }
+  return n;
 }
 
 int act_rows(int M, int N, int esz) {                     // rows a workgroup of act_bwd_kernel takes
@@ -729,10 +921,8 @@ int act_rows(int M, int N, int esz) {                     // rows a workgroup of
 
 }  // namespace
 
-extern "C" long long vca_matmul_act_ws_floats(const vca_matmul_desc* d, const void* a, const void* b) {
-  Plan p;
-  if (plan_of(d, a, b, p) != 0) return 0;
-  return p.tile && p.g.ksplit > 1 ? (long long)p.g.ksplit * p.g.M * p.g.npad : 0;
+extern "C" long long vca_matmul_act_ws_floats(const vca_matmul_desc* d) {
+  return ws_floats_of(d);
 }
 
 extern "C" int vca_matmul_act(const vca_matmul_desc* d, const void* a, const void* b, const void* bias, const void* res,
@@ -809,4 +999,53 @@ extern "C" int vca_act_bwd(int type, int M, int N, int act, float slope, const v
     else hipLaunchKernelGGL(bias_fold_kernel<vca_e16>, fg, dim3(256), 0, s, N, slabs, ws, (vca_e16*)db, db_add);
   }
   return vca_launch_status();
+}
+
+// The three products' descriptors of a backward pass.
+static vca_matmul_desc bwd_dx(const vca_linear_bwd& b) {
+  vca_matmul_desc d = {b.M, b.K, b.N, b.type, b.nsplit, 0, 1, VCA_ACT_NONE, 0.f, b.N, b.ldw, b.K, 0};
+  return d;
+}
+
+static vca_matmul_desc bwd_dw(const vca_linear_bwd& b) {
+  vca_matmul_desc d = {b.N, b.K, b.M, b.type, b.nsplit, 1, 1, VCA_ACT_NONE, 0.f, b.N, b.ldx, b.K, b.K};
+  return d;
+}
+
+extern "C" long long vca_linear_act_bwd_ws_floats(const vca_linear_bwd* b) {
+  if (!b || b->M <= 0 || b->N <= 0 || b->K <= 0) return 0;
+  const vca_matmul_desc x = bwd_dx(*b), w = bwd_dw(*b);
+  long long n = vca_act_bwd_ws_floats(b->type, b->M, b->N);
+  const long long nx = ws_floats_of(&x), nw = ws_floats_of(&w);
+  n = nx > n ? nx : n;
+  return nw > n ? nw : n;
+}
+
+extern "C" int vca_linear_act_bwd(const vca_linear_bwd* b, float* ws, long long ws_floats, void* stream) {
+  VCA_CHECK_ARG(b && b->gy && b->M > 0 && b->N > 0 && b->K > 0 && (b->act == VCA_ACT_NONE) == !b->z);
+  VCA_CHECK_ARG((!b->dx || b->w) && (!b->dw || b->x) && ((b->act == VCA_ACT_NONE) == !b->dz || !(b->dx || b->dw)));
+  // (checked before the first launch: a refused call has written nothing)
+  const vca_matmul_desc x = bwd_dx(*b), w = bwd_dw(*b);
+  Plan p;
+  if (b->dx) {
+    const int rc = plan_of(&x, b->gy, b->w, p);
+    if (rc) return rc;
+  }
+  if (b->dw) {
+    const int rc = plan_of(&w, b->gy, b->x, p);
+    if (rc) return rc;
+  }
+  VCA_CHECK_ARG(ws_floats >= vca_linear_act_bwd_ws_floats(b) && (!ws_floats || (ws && (reinterpret_cast<uintptr_t>(ws) & 15) == 0)));
+  if (b->dz || b->db) {
+    const int rc = vca_act_bwd(b->type, b->M, b->N, b->act, b->slope, b->gy, b->z, b->dz, b->db, b->db_add, ws, ws_floats,
+                               stream);
+    if (rc) return rc;
+  }
+  const void* dz = b->dz ? b->dz : b->gy;
+  if (b->dx) {
+    const int rc = vca_matmul_act(&x, dz, b->w, nullptr, nullptr, b->dx, nullptr, ws, ws_floats, stream);
+    if (rc) return rc;
+  }
+  if (b->dw) return vca_matmul_act(&w, dz, b->x, nullptr, b->dw_add ? b->dw : nullptr, b->dw, nullptr, ws, ws_floats, stream);
+  return 0;
 }

@@ -793,14 +793,14 @@ def linear(x, w, bias=None):
 # linear layers with bias, activation and residual in the product's epilogue
 # --------------------------------------------------------------------------- #
 ACT_GELU, ACT_GELU_TANH, ACT_SILU = 5, 6, 7
-_LINEAR_ACTS = {'relu': (ACT_RELU, 0.0), 'leaky0.2': (ACT_LEAKY, 0.2), 'tanh': (ACT_TANH, 0.0), 'gelu': (ACT_GELU, 0.0),
-                'gelu_tanh': (ACT_GELU_TANH, 0.0), 'silu': (ACT_SILU, 0.0)}
+_LINEAR_ACTS = {None: (ACT_NONE, 0.0), 'relu': (ACT_RELU, 0.0), 'leaky0.2': (ACT_LEAKY, 0.2), 'tanh': (ACT_TANH, 0.0),
+                'gelu': (ACT_GELU, 0.0), 'gelu_tanh': (ACT_GELU_TANH, 0.0), 'silu': (ACT_SILU, 0.0)}
 
 
 def _linear_act_code(act):
-    if act is None or isinstance(act, torch.nn.Identity):
-        return ACT_NONE, 0.0
-    if isinstance(act, torch.nn.GELU):
+    if isinstance(act, torch.nn.Identity):
+        act = None
+    elif isinstance(act, torch.nn.GELU):
         act = 'gelu_tanh' if act.approximate == 'tanh' else 'gelu'
     elif isinstance(act, torch.nn.SiLU):
         act = 'silu'
@@ -810,103 +810,103 @@ def _linear_act_code(act):
         act = 'tanh'
     elif isinstance(act, torch.nn.LeakyReLU):
         return ACT_LEAKY, float(act.negative_slope)
-    if act not in _LINEAR_ACTS:
-        raise ValueError('linear_act: activation %r (one of None, %s, or the nn module of one)'
-                         % (act, ', '.join(sorted(_LINEAR_ACTS))))
-    return _LINEAR_ACTS[act]
+    try:
+        return _LINEAR_ACTS[act]
+    except (KeyError, TypeError):
+        raise ValueError('linear_act: activation %r (one of %s, or the torch.nn module of one)'
+                         % (act, ', '.join(str(k) for k in _LINEAR_ACTS))) from None
 
 
 def _rows_2d(t, broadcast=False):
     """t (..., C) as a matrix of rows, without a copy where the rows are dense and equally spaced.  broadcast: rows that
     are all the same one (stride 0) may stay so."""
-    c = t.shape[-1]
-    if t.dim() == 2:
-        m = t
-    else:
+    m = t
+    if t.dim() != 2:
+        c = t.shape[-1]
         try:
-            m = t.view(-1, c) if t.numel() else t.reshape(-1, c)
+            m = t.view(-1, c)
         except RuntimeError:
             m = t.reshape(-1, c)
-    if c > 1 and m.stride(1) != 1 or m.shape[0] > 1 and m.stride(0) < c and not (broadcast and m.stride(0) == 0):
+    if m.is_contiguous():
+        return m
+    (rows, c), (step, unit) = m.shape, m.stride()
+    if c > 1 and unit != 1 or rows > 1 and step < c and not (broadcast and step == 0):
         m = m.contiguous()
     return m
 
 
-def _typed(dtype):
-    """The library that takes tensors of this type (16-bit products are compiled per type)."""
-    if dtype == torch.float32:
-        return _lib.lib()
-    return _lib.lib('bf16' if dtype == torch.bfloat16 else 'fp16')
+_ELEM_OF = {torch.float32: None, torch.bfloat16: 'bf16', torch.float16: 'fp16'}   # 16-bit products are compiled per type
+_act_ws = {}     # sizes and types of a forward or backward pass -> workspace floats
 
 
-def _matmul(a, a_col, b, b_col, M, N, K, nsplit, bias=None, act=(ACT_NONE, 0.0), res=None, out=None, z=None):
-    """C[m][n] = act(sum_k A(m, k) B(n, k) + bias[n]) + res[m][n] (vca_matmul_act); a, b, res, out: 2-D, rows dense."""
-    L = _typed(a.dtype)
-    if out is None:
-        out = torch.empty((M, N), device=a.device, dtype=a.dtype)
-    lead = lambda t: t.stride(0) if t.shape[0] > 1 else t.shape[1]     # the stride of a single row is anything
-    d = _lib.MatmulDesc(M, N, K, _lib.TYPES[a.dtype], nsplit, a_col, b_col, act[0], act[1], lead(a), lead(b), lead(out),
-                        0 if res is None else lead(res))
-    n = int(L.vca_matmul_act_ws_floats(d, a.data_ptr(), b.data_ptr()))
-    ws = torch.empty(n, device=a.device, dtype=torch.float32) if n else None
-    at = lambda t: None if t is None else t.data_ptr()
-    check(L.vca_matmul_act(d, a.data_ptr(), b.data_ptr(), at(bias), at(res), out.data_ptr(), at(z), at(ws), n, stream()),
-          'matmul_act')
-    return out
+def _row_step(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]               # a single row's stride may be anything
+
+
+def _linear_act_fwd(x, w, bias, res, code, z=None):
+    (M, K), N, dt = x.shape, w.shape[0], x.dtype
+    y = torch.empty((M, N), device=x.device, dtype=dt)
+    L = _lib.lib(_ELEM_OF[dt])
+    ns = _nsplit() if dt == torch.float32 else 1
+    d = _lib.MatmulDesc(M, N, K, _lib.TYPES[dt], ns, 0, 0, code[0], code[1], _row_step(x), _row_step(w), N,
+                        0 if res is None else _row_step(res))
+    key = (M, N, K, dt, ns)
+    n = _act_ws.get(key)
+    if n is None:
+        n = _act_ws[key] = int(L.vca_matmul_act_ws_floats(d))
+    ws = torch.empty(n, device=x.device, dtype=torch.float32) if n else None
+    check(L.vca_matmul_act(d, x.data_ptr(), w.data_ptr(), None if bias is None else bias.data_ptr(),
+                           None if res is None else res.data_ptr(), y.data_ptr(), None if z is None else z.data_ptr(),
+                           None if ws is None else ws.data_ptr(), n, stream()), 'matmul_act')
+    return y
 
 
 class LinearActFn(torch.autograd.Function):
-    """See linear_act.  x, res: matrices of rows (any row stride)."""
+    """See linear_act.  x, w, res: matrices of rows (any row stride)."""
 
     @staticmethod
-    def forward(ctx, x, w, bias, res, act, keep):
-        M, K = x.shape
-        N = w.shape[0]
-        z = torch.empty((M, N), device=x.device, dtype=x.dtype) if keep and act[0] != ACT_NONE else None
-        ns = _nsplit() if x.dtype == torch.float32 else 1
-        y = _matmul(x, 0, w, 0, M, N, K, ns, bias, act, res, None, z)
+    def forward(ctx, x, w, bias, res, code):
+        z = None
+        if code[0] != ACT_NONE and any(ctx.needs_input_grad[:3]):
+            z = torch.empty((x.shape[0], w.shape[0]), device=x.device, dtype=x.dtype)
         ctx.save_for_backward(x, w, z)
-        ctx.act = act
-        ctx.bias_param = bias
-        return y
+        ctx.code, ctx.bias_param = code, bias
+        return _linear_act_fwd(x, w, bias, res, code, z)
 
     @staticmethod
     @once
     def backward(ctx, gy):
         x, w, z = ctx.saved_tensors
-        M, K = x.shape
-        N = w.shape[0]
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         if _inputs_only[0]:
             need_w = need_b = False
         gx = gw = gb = None
         if need_x or need_w or need_b:
-            with _on_device(x.device):
-                g = gy.contiguous()
-                L = _typed(x.dtype)
-                ns = _nsplit(True) if x.dtype == torch.float32 else 1
-                bsink = _grad_sink(ctx.bias_param) if need_b else None
-                dz = torch.empty((M, N), device=x.device, dtype=x.dtype) if z is not None else None
-                if dz is not None or need_b:
-                    if need_b:
-                        gb = bsink if bsink is not None else torch.empty((N,), device=x.device, dtype=x.dtype)
-                    n = int(L.vca_act_bwd_ws_floats(_lib.TYPES[x.dtype], M, N)) if need_b else 0
-                    ws = torch.empty(n, device=x.device, dtype=torch.float32) if n else None
-                    at = lambda t: None if t is None else t.data_ptr()
-                    check(L.vca_act_bwd(_lib.TYPES[x.dtype], M, N, ctx.act[0], ctx.act[1], g.data_ptr(), at(z), at(dz),
-                                        at(gb), 0 if bsink is None else 1, at(ws), n, stream()), 'act_bwd')
-                    if bsink is not None:
-                        gb = None
-                if dz is None:
-                    dz = g
-                if need_x:
-                    gx = _matmul(dz, 0, w, 1, M, K, N, ns)
-                if need_w:
-                    sink = _grad_sink(w)
-                    gw = _matmul(dz, 1, x, 1, N, K, M, ns, res=sink, out=sink)
-                    if sink is not None:
-                        gw = None
-        return gx, gw, gb, gy if need_r else None, None, None
+            (M, K), N, dt, dev = x.shape, w.shape[0], x.dtype, x.device
+            g = gy.contiguous()
+            wsink = _grad_sink(w) if need_w else None
+            bsink = _grad_sink(ctx.bias_param) if need_b else None
+            with _on_device(dev):
+                new = lambda *shape: torch.empty(shape, device=dev, dtype=dt)
+                dz = new(M, N) if z is not None and (need_x or need_w) else None
+                gx = new(M, K) if need_x else None
+                gw = (new(N, K) if wsink is None else wsink) if need_w else None
+                gb = (new(N) if bsink is None else bsink) if need_b else None
+                at = lambda t: None if t is None else t.data_ptr()
+                L = _lib.lib(_ELEM_OF[dt])
+                ns = _nsplit(True) if dt == torch.float32 else 1
+                d = _lib.LinearBwd(M, N, K, _lib.TYPES[dt], ns, ctx.code[0], wsink is not None, bsink is not None,
+                                   ctx.code[1], _row_step(x), _row_step(w), g.data_ptr(), x.data_ptr(), w.data_ptr(),
+                                   at(z), at(dz), at(gx), at(gw), at(gb))
+                key = (M, N, K, dt, ns, 'bwd')
+                n = _act_ws.get(key)
+                if n is None:
+                    n = _act_ws[key] = int(L.vca_linear_act_bwd_ws_floats(d))
+                ws = torch.empty(n, device=dev, dtype=torch.float32)
+                check(L.vca_linear_act_bwd(d, ws.data_ptr(), n, stream()), 'linear_act_bwd')
+            gw = gw if wsink is None else None
+            gb = gb if bsink is None else None
+        return gx, gw, gb, gy if need_r else None, None
 
 
 def linear_act(x, w, bias=None, act=None, residual=None):
@@ -923,32 +923,36 @@ def linear_act(x, w, bias=None, act=None, residual=None):
     value under the activation and dz = gy act' are rounded to the tensors' type.  Inside direct_param_grad() the
     gradients of leaf parameters are added straight into their .grad; input_grads_only() leaves them out."""
     code = _linear_act_code(act)
-    if x.dtype not in _lib.TYPES:
-        raise TypeError('linear_act: fp32, bf16 or fp16 tensors, got %s' % x.dtype)
-    if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1] or w.shape[0] < 1 or w.shape[1] < 1:
-        raise ValueError('linear_act: x %s and w %s do not go together' % (tuple(x.shape), tuple(w.shape)))
-    shape = tuple(x.shape[:-1]) + (w.shape[0],)
-    if bias is not None and tuple(bias.shape) != (w.shape[0],):
-        raise ValueError('linear_act: bias of shape %s for %d outputs' % (tuple(bias.shape), w.shape[0]))
-    if residual is not None and tuple(residual.shape) != shape:
-        raise ValueError('linear_act: residual of shape %s for an output of %s' % (tuple(residual.shape), shape))
-    for name, t in (('x', x), ('w', w), ('bias', bias), ('residual', residual)):
-        if t is not None and t.dtype != x.dtype:
-            raise TypeError('linear_act: %s is %s and x is %s' % (name, t.dtype, x.dtype))
-        if t is not None and (not t.is_cuda or t.device != x.device):
-            raise ValueError('linear_act: %s is on %s and x on %s; one GPU is wanted' % (name, t.device, x.device))
+    dt, dev, xs, ws = x.dtype, x.device, x.shape, w.shape
+    if dt not in _lib.TYPES:
+        raise TypeError('linear_act: fp32, bf16 or fp16 tensors, got %s' % dt)
+    if len(ws) != 2 or len(xs) < 1 or xs[-1] != ws[1] or 0 in ws:
+        raise ValueError('linear_act: x %s and w %s do not go together' % (tuple(xs), tuple(ws)))
+    shape = xs[:-1] + ws[:1]
+    if bias is not None and bias.shape != ws[:1]:
+        raise ValueError('linear_act: bias of shape %s for %d outputs' % (tuple(bias.shape), ws[0]))
+    if residual is not None and residual.shape != shape:
+        raise ValueError('linear_act: residual of shape %s for an output of %s' % (tuple(residual.shape), tuple(shape)))
+    tensors = [t for t in (x, w, bias, residual) if t is not None]
+    for t in tensors:
+        if t.dtype != dt:
+            raise TypeError('linear_act: tensors of one type are wanted, got %s and %s' % (dt, t.dtype))
+        if not t.is_cuda or t.device != dev:
+            raise ValueError('linear_act: tensors on one GPU are wanted, got %s and %s' % (dev, t.device))
     if 0 in shape:
         y = x.new_zeros(shape)                  # no rows: an empty result that still hangs on its inputs
-        for t in (x, w, bias, residual):
-            if t is not None:
-                y = y + t.sum() * 0
+        for t in tensors:
+            y = y + t.sum() * 0
         return y
-    with _on_device(x.device):
-        b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-        keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias))
-        y = LinearActFn.apply(_rows_2d(x), _rows_2d(w), b, None if residual is None else _rows_2d(residual, True), code,
-                              keep)
-    return y.view(shape)
+    x2, w2 = _rows_2d(x), _rows_2d(w)
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    r = None if residual is None else _rows_2d(residual, True)
+    with _on_device(dev):
+        if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+            y = LinearActFn.apply(x2, w2, b, r, code)
+        else:
+            y = _linear_act_fwd(x2, w2, b, r, code)
+    return y if len(shape) == 2 else y.view(shape)
 
 
 class StemConvFn(torch.autograd.Function):
