@@ -164,7 +164,7 @@ __device__ __forceinline__ void finish(const MatArgs& g, int m, int n, float (&v
 // ------------------------------------------------------------------------------------------------
 template <int MODE, int R>
 __device__ __forceinline__ int col_swizzle(int k) {       // in 16-byte pieces
-  if (MODE == MODE_16) return ((k & 3) | ((k >> 1) & 4)) << 1;
+  if (MODE == MODE_16) return (R >= 128 ? (k & 3) | ((k >> 1) & 4) : k & 3) << 1;   // (64: a row of k has four blocks)
   return ((MODE == MODE_F32 ? k >> 2 : k >> 3) & 3) << 2;
 }
 
@@ -259,7 +259,7 @@ template <bool KC, int R>
 __device__ __forceinline__ bf16x8 frag16(const char* s, int sub, int kk, int lc, int g) {
   if (KC) return *reinterpret_cast<const bf16x8*>(s + (sub + lc) * 128 + (((kk * 4 + g) ^ (lc & 7)) << 4));
   const int k = kk * 32 + 8 * g + (lc >> 2);
-  const char* p = s + k * (R * 2) + (((sub >> 4) ^ ((k & 3) | ((k >> 1) & 4))) << 5) + (lc & 3) * 8;
+  const char* p = s + k * (R * 2) + (((sub >> 3) ^ col_swizzle<MODE_16, R>(k)) << 4) + (lc & 3) * 8;
   union { s16x4 h[2]; bf16x8 v; } f;
   f.h[0] = read_transposed(p);
   f.h[1] = read_transposed(p + 4 * R * 2);
@@ -273,7 +273,7 @@ __device__ __forceinline__ f32x4 frag32(const char* s, int sub, int kk, int lc, 
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int k = kk * 16 + 4 * g + e;
-    f[e] = *reinterpret_cast<const float*>(s + k * (R * 4) + (((sub >> 4) ^ ((k >> 2) & 3)) << 6) + lc * 4);
+    f[e] = *reinterpret_cast<const float*>(s + k * (R * 4) + (((sub >> 2) ^ col_swizzle<MODE_F32, R>(k)) << 4) + lc * 4);
   }
   return f;
 }
@@ -292,7 +292,7 @@ __device__ __forceinline__ void frag_split(const char* s, int sub, int lc, int g
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int k = 8 * g + e;
-      v[e] = *reinterpret_cast<const float*>(s + k * (R * 4) + (((sub >> 4) ^ ((k >> 3) & 3)) << 6) + lc * 4);
+      v[e] = *reinterpret_cast<const float*>(s + k * (R * 4) + (((sub >> 2) ^ col_swizzle<MODE_S3, R>(k)) << 4) + lc * 4);
     }
   }
 #pragma unroll
@@ -742,7 +742,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_rows_kernel(const MatArgs 
 template <typename T>
 __global__ __launch_bounds__(256) void act_bwd_kernel(int M, int N, int act, float slope, const T* __restrict__ gy,
                                                       const T* __restrict__ z, T* __restrict__ dz,
-                                                      float* __restrict__ part, int rows) {
+                                                      float* __restrict__ part, int rows, T* __restrict__ db,
+                                                      int db_add) {
   constexpr int V = 16 / (int)sizeof(T);
   __shared__ float red[8][32 * V];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -779,7 +780,7 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(int M, int N, int act, flo
         }
     }
   }
-  if (!part) return;
+  if (!db) return;
 #pragma unroll
   for (int e = 0; e < V; ++e) red[ty][tx * V + e] = s[e];
   __syncthreads();
@@ -788,7 +789,9 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(int M, int N, int act, flo
 #pragma unroll
     for (int y = 0; y < 8; ++y) t += red[y][i];
     const int col = blockIdx.x * 32 * V + i;
-    if (col < N) part[(size_t)blockIdx.y * N + col] = t;
+    if (col >= N) continue;
+    if (gridDim.y > 1) part[(size_t)blockIdx.y * N + col] = t;
+    else db[col] = (T)(db_add ? t + (float)db[col] : t);      // the only slab
   }
 }
 
@@ -823,15 +826,57 @@ int mode_of(const vca_matmul_desc& d) {
 
 struct Plan {
   MatArgs g;
-  int mode, tile;                     // 128 or 256; 0: few rows
-  bool dma;
+  int mode, tile;                     // 64, 128 or 256; 0: few rows
+  bool dma, wide;
 };
+
+// Tile and split of a product, by the time the candidates would take.  A tile's chunk costs a CU `work` us of its matrix
+// cores; a workgroup that has a CU to itself cannot go below `wait` us a chunk (LDS and memory latency, one barrier a
+// chunk), a CU with r workgroups takes max(wait, r work).  `ends`: filling the pipeline and storing the tile.  A split
+// adds one launch and a pass over the partial products.  Fitted to launches of 2 to 2000 us on this part; the choice is
+// within 10 % of the best one measured at each.  Where sides change (us): fp32 4800 x 1280, K 512: 64-wide tiles 62, 128
+// 74; 8192 x 4096, K 4096: 2349 against 2043.  16 bits 2048^3: 64 29, 128 30, 256 39 (split); 4800 x 2560, K 5120:
+// 197, 137, 112; 64 x 4096, K 4096: 64-wide unsplit 31, split four ways 15.
+struct TileCost { int tile; double work, wait, ends; };
+constexpr TileCost COST[4][3] = {
+    {{256, 1.55, 1.55, 8.}, {128, 0.53, 0.85, 2.}, {64, 0.20, 0.45, 0.8}},     // 16-bit tensors
+    {{0, 0., 0., 0.}, {128, 1.95, 2.15, 2.5}, {64, 0.56, 0.62, 1.}},           // fp32, exact
+    {{0, 0., 0., 0.}, {128, 0.92, 1.15, 2.5}, {64, 0.36, 0.55, 1.}},           // fp32, three products
+    {{0, 0., 0., 0.}, {128, 0.46, 0.85, 2.5}, {64, 0.22, 0.45, 1.}}};          // fp32, one product
+
+bool pick(Plan& p, int nc) {
+  MatArgs& g = p.g;
+  double best = 0.;
+  p.tile = 0;
+  for (const TileCost& t : COST[p.mode]) {
+    if (!t.tile || (t.tile == 256 && !p.wide)) continue;
+    const long long tiles = ((g.M + (long long)t.tile - 1) / t.tile) * ((g.N + (long long)t.tile - 1) / t.tile);
+    if (tiles >= (1 << 24)) continue;
+    for (int ks = 1; ks <= 32 && ks <= nc; ++ks) {
+      const int chunks = (nc + ks - 1) / ks;
+      if (ks > 1 && (chunks < 2 || tiles * ks > 2048)) break;
+      const double r = (double)((tiles * ks + 255) / 256);
+      double us = chunks * (r * t.work > t.wait ? r * t.work : t.wait) + r * t.ends;
+      if (ks > 1) us += 3. + (double)ks * g.M * g.npad * 1e-6;                 // written and read at 8 bytes / ps
+      if (p.tile && us >= best) continue;
+      best = us;
+      p.tile = t.tile;
+      g.cpz = chunks;
+    }
+  }
+  if (!p.tile) return false;
+  g.ksplit = (nc + g.cpz - 1) / g.cpz;
+  g.ntm = (g.M + p.tile - 1) / p.tile;
+  g.ntn = (g.N + p.tile - 1) / p.tile;
+  return true;
+}
 
 int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p) {
   VCA_CHECK_ARG(dp);
   const vca_matmul_desc& d = *dp;
   p.mode = mode_of(d);
   VCA_CHECK_ARG(p.mode >= 0 && d.M > 0 && d.N > 0 && d.K > 0 && act_ok(d.act));
+  VCA_CHECK_ARG(d.M <= (1 << 30) && d.N <= (1 << 30) && d.K <= (1 << 30));   // (tile edges stay in an int)
   VCA_CHECK_ARG(!(d.a_col && !d.b_col));                   // no product here reads only its rows by columns
   const int esz = d.type == VCA_T_F32 ? 4 : 2, bk = 128 / esz;
   VCA_CHECK_ARG(d.lda >= (d.a_col ? d.M : (d.M > 1 ? d.K : 0)) && d.ldb >= (d.b_col ? d.N : (d.N > 1 ? d.K : 0)) &&
@@ -858,26 +903,19 @@ int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p) {
     p.tile = 0;
     return 0;
   }
-  auto tiles = [&](int t) { return (long long)((d.M + t - 1) / t) * ((d.N + t - 1) / t); };
-  p.tile = p.mode == MODE_16 && p.dma && tiles(256) >= 192 ? 256 : 128;
-  g.ntm = (d.M + p.tile - 1) / p.tile;
-  g.ntn = (d.N + p.tile - 1) / p.tile;
-  VCA_CHECK_ARG(tiles(p.tile) < (1 << 24));
-  const int nt = g.ntm * g.ntn, nc = g.cpz;
-  // few tiles: split the reduction over workgroups until the chip is covered, four chunks a range at least
-  int ks = 1;
-  while (nt * ks < 256 && nc / (ks + 1) >= 4 && ks < 32) ++ks;
-  g.cpz = (nc + ks - 1) / ks;
-  g.ksplit = (nc + g.cpz - 1) / g.cpz;
-  return 0;
+  // the 256-wide kernel addresses its pieces by 32-bit offsets from the tile: 256 rows (64 of k) of at most 4 MB
+  p.wide = p.mode == MODE_16 && p.dma && d.lda <= (1 << 21) && d.ldb <= (1 << 21);
+  return pick(p, g.cpz) ? 0 : -22;
 }
 
-template <int MODE, bool AKC, bool BKC, int BM, int NWM, int NWN, bool DMA>
-int launch_tile(const MatArgs& g, hipStream_t s) {
-  const size_t lds = 2 * (size_t)(BM + BM) * 128;
-  if (lds > 64 * 1024) VCA_MAX_LDS((matmul_kernel<MODE, AKC, BKC, BM, BM, NWM, NWN, DMA>));
-  hipLaunchKernelGGL((matmul_kernel<MODE, AKC, BKC, BM, BM, NWM, NWN, DMA>), dim3(g.ntm * g.ntn * g.ksplit),
-                     dim3(NWM * NWN * 64), lds, s, g);
+template <int MODE, bool AKC, bool BKC, int BM>
+int launch_tile(const Plan& p, hipStream_t s) {
+  const size_t lds = 4 * (size_t)BM * 128;                 // at most 64 KB
+  const dim3 grid(p.g.ntm * p.g.ntn * p.g.ksplit);
+  if (p.dma)
+    hipLaunchKernelGGL((matmul_kernel<MODE, AKC, BKC, BM, BM, 2, 2, true>), grid, dim3(256), lds, s, p.g);
+  else
+    hipLaunchKernelGGL((matmul_kernel<MODE, AKC, BKC, BM, BM, 2, 2, false>), grid, dim3(256), lds, s, p.g);
   return vca_launch_status();
 }
 
@@ -888,8 +926,7 @@ int launch_layout(const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((matmul_wide_kernel<AKC, BKC>), dim3(p.g.ntm * p.g.ntn * p.g.ksplit), dim3(512), 128 * 1024, s, p.g);
     return vca_launch_status();
   }
-  return p.dma ? launch_tile<MODE, AKC, BKC, 128, 2, 2, true>(p.g, s)
-               : launch_tile<MODE, AKC, BKC, 128, 2, 2, false>(p.g, s);
+  return p.tile == 64 ? launch_tile<MODE, AKC, BKC, 64>(p, s) : launch_tile<MODE, AKC, BKC, 128>(p, s);
 }
 
 template <int MODE>
@@ -899,21 +936,26 @@ int launch_mode(const Plan& p, bool a_col, bool b_col, hipStream_t s) {
   return launch_layout<MODE, true, true>(p, s);
 }
 
-// Workspace floats of a product, whatever its operands' alignment.
+long long ws_of(const Plan& p) {
+  return p.tile && p.g.ksplit > 1 ? (long long)p.g.ksplit * p.g.M * p.g.npad : 0;
+}
+
+// Workspace floats of a product whatever its operands' alignment and strides, so that a caller may ask once a size.
 long long ws_floats_of(const vca_matmul_desc* d) {
+  Plan p;
+  if (plan_of(d, nullptr, nullptr, p) != 0 || !p.tile) return 0;
   long long n = 0;
-  for (uintptr_t at : {(uintptr_t)16, (uintptr_t)4}) {
-    Plan p;
-    if (plan_of(d, reinterpret_cast<const void*>(at), reinterpret_cast<const void*>(at), p) != 0) return 0;
-    const long long f = p.tile && p.g.ksplit > 1 ? (long long)p.g.ksplit * p.g.M * p.g.npad : 0;
-    n = f > n ? f : n;
+  for (bool wide : {false, true}) {
+    const int nc = (p.g.K * (d->type == VCA_T_F32 ? 4ll : 2ll) + 127) / 128;
+    p.wide = wide && p.mode == MODE_16;
+    if (pick(p, nc) && ws_of(p) > n) n = ws_of(p);
   }
   return n;
 }
 
 int act_rows(int M, int N, int esz) {                     // rows a workgroup of act_bwd_kernel takes
   const long long strips = ((long long)N * esz + 511) / 512;
-  int rows = 8;
+  int rows = 64;                                          // up to 64 rows: one slab, and no launch to add slabs up
   auto slabs = [&]() { return ((long long)M + rows - 1) / rows; };
   while ((rows < 256 && strips * slabs() > 1024) || slabs() > 65535) rows *= 2;   // (65535: the grid's second dimension)
   return rows;
@@ -950,7 +992,7 @@ extern "C" int vca_matmul_act(const vca_matmul_desc* d, const void* a, const voi
     return vca_launch_status();
   }
   if (g.ksplit > 1) {
-    VCA_CHECK_ARG(ws && ws_floats >= (long long)g.ksplit * g.M * g.npad && (reinterpret_cast<uintptr_t>(ws) & 15) == 0);
+    VCA_CHECK_ARG(ws && ws_floats >= ws_of(p) && (reinterpret_cast<uintptr_t>(ws) & 15) == 0);
     g.part = ws;
   }
   int e = 0;
@@ -986,14 +1028,13 @@ extern "C" int vca_act_bwd(int type, int M, int N, int act, float slope, const v
   VCA_CHECK_ARG(!db || (ws && ws_floats >= (long long)slabs * N && (reinterpret_cast<uintptr_t>(ws) & 3) == 0));
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(((long long)N * esz + 511) / 512), (unsigned)slabs);
-  float* part = db ? ws : nullptr;
   if (esz == 4)
     hipLaunchKernelGGL(act_bwd_kernel<float>, grid, dim3(256), 0, s, M, N, act, slope, (const float*)gy, (const float*)z,
-                       (float*)dz, part, rows);
+                       (float*)dz, ws, rows, (float*)db, db_add);
   else
     hipLaunchKernelGGL(act_bwd_kernel<vca_e16>, grid, dim3(256), 0, s, M, N, act, slope, (const vca_e16*)gy,
-                       (const vca_e16*)z, (vca_e16*)dz, part, rows);
-  if (db) {
+                       (const vca_e16*)z, (vca_e16*)dz, ws, rows, (vca_e16*)db, db_add);
+  if (db && slabs > 1) {
     const dim3 fg((N + 15) / 16);
     if (esz == 4) hipLaunchKernelGGL(bias_fold_kernel<float>, fg, dim3(256), 0, s, N, slabs, ws, (float*)db, db_add);
     else hipLaunchKernelGGL(bias_fold_kernel<vca_e16>, fg, dim3(256), 0, s, N, slabs, ws, (vca_e16*)db, db_add);
@@ -1026,22 +1067,25 @@ extern "C" int vca_linear_act_bwd(const vca_linear_bwd* b, float* ws, long long 
   VCA_CHECK_ARG((!b->dx || b->w) && (!b->dw || b->x) && ((b->act == VCA_ACT_NONE) == !b->dz || !(b->dx || b->dw)));
   // (checked before the first launch: a refused call has written nothing)
   const vca_matmul_desc x = bwd_dx(*b), w = bwd_dw(*b);
+  const void* dz = b->dz ? b->dz : b->gy;
+  long long need = b->db ? vca_act_bwd_ws_floats(b->type, b->M, b->N) : 0;
   Plan p;
   if (b->dx) {
-    const int rc = plan_of(&x, b->gy, b->w, p);
+    const int rc = plan_of(&x, dz, b->w, p);
     if (rc) return rc;
+    need = ws_of(p) > need ? ws_of(p) : need;
   }
   if (b->dw) {
-    const int rc = plan_of(&w, b->gy, b->x, p);
+    const int rc = plan_of(&w, dz, b->x, p);
     if (rc) return rc;
+    need = ws_of(p) > need ? ws_of(p) : need;
   }
-  VCA_CHECK_ARG(ws_floats >= vca_linear_act_bwd_ws_floats(b) && (!ws_floats || (ws && (reinterpret_cast<uintptr_t>(ws) & 15) == 0)));
+  VCA_CHECK_ARG(ws_floats >= need && (!need || (ws && (reinterpret_cast<uintptr_t>(ws) & 15) == 0)));
   if (b->dz || b->db) {
     const int rc = vca_act_bwd(b->type, b->M, b->N, b->act, b->slope, b->gy, b->z, b->dz, b->db, b->db_add, ws, ws_floats,
                                stream);
     if (rc) return rc;
   }
-  const void* dz = b->dz ? b->dz : b->gy;
   if (b->dx) {
     const int rc = vca_matmul_act(&x, dz, b->w, nullptr, nullptr, b->dx, nullptr, ws, ws_floats, stream);
     if (rc) return rc;
