@@ -565,11 +565,12 @@ int vca_linear_act_bwd(const vca_linear_bwd* b, float* ws, long long ws_floats, 
  * reference trains without clipping).  h_ptrs / h_numel / h_types are host arrays, read before the call returns:
  * device pointer (aligned to its element), element count (0 allowed) and VCA_T_* of each tensor, taken as dense memory.
  * scale: {s, 1/s} of a loss scaler whose factor the gradients carry, or NULL.  ws: at least
- * vca_grad_norm_ws_doubles(ntensor) doubles, contents irrelevant, not shared by calls that may overlap in time.
+ * vca_grad_norm_ws_doubles of the list (0 for a short one; with h_ptrs NULL: enough for any list of that many tensors)
+ * doubles, contents irrelevant, not shared by calls that may overlap in time.
  *   vca_grad_norm   out[0] = sqrt(sum g^2) / s
  *   vca_grad_clip   the same, then every g *= min(1, max_norm / (out[0] + 1e-6)) in place; the tensors must not overlap
  * The sum is held in fp64 and in a fixed order: equal inputs give equal bits. */
-long long vca_grad_norm_ws_doubles(int ntensor);
+long long vca_grad_norm_ws_doubles(int ntensor, const void* const* h_ptrs, const long long* h_numel, const int* h_types);
 int vca_grad_norm(int ntensor, const void* const* h_ptrs, const long long* h_numel, const int* h_types,
                   const float* scale, double* ws, long long ws_doubles, float* out, void* stream);
 int vca_grad_clip(int ntensor, const void* const* h_ptrs, const long long* h_numel, const int* h_types, float max_norm,
@@ -578,8 +579,8 @@ int vca_grad_clip(int ntensor, const void* const* h_ptrs, const long long* h_num
 /* The Adam update of an optimizer's flat buffers (vca_adam_f32's arithmetic) on gradients clipped by their joint norm:
  * g enters as g * min(1, max_norm / (norm + 1e-6)) / s and is not written.  Every buffer 16-byte aligned, n % 4 == 0.
  * ++*step_dev happens inside; scale / flag (both or neither) are the loss scaler's: a gradient that is not finite sets
- * *flag, and with *flag up nothing is updated and the count stays.  ws as above for ntensor = ngroup;
- * out[4] = {norm, factor, learning rate / bias correction, root of the second bias correction}. */
+ * *flag, and with *flag up nothing is updated and the count stays.  ws: vca_grad_norm_ws_doubles(ngroup, NULL, ...)
+ * doubles; out: 5 words, {norm, factor, learning rate / bias correction, root of the second bias correction, scratch}. */
 #define VCA_MAX_ADAM_GROUPS 32
 typedef struct {
   float* p;

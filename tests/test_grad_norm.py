@@ -216,7 +216,7 @@ def _check_adam(opt, groups, ref):
 
 @gpu
 @pytest.mark.parametrize('amsgrad', [False, True])
-@pytest.mark.parametrize('sizes', [[4], [100], [4096, 8], [65540, 4, 1000000], [12] * 32])
+@pytest.mark.parametrize('sizes', [[4], [100], [4096, 8], [65540, 4, 1000000], [12] * 32, [3000000, 1200004]])
 def test_adam_with_clipping(sizes, amsgrad):
     opt, groups, ref = _adam_pair(sizes, amsgrad, len(sizes))
     for t in (1, 2, 3):
@@ -391,4 +391,5 @@ def test_entry_points_refuse_before_any_launch():
         assert call(g(**kw)) == -22, kw
     assert call(g(), n=0) == -22 and call(g(), n=33) == -22 and call(g(), mx=-1.0) == -22
     assert call(g(), sc=64) == -22 and call(g(), fl=64) == -22                   # a scale without its flag, and back
-    assert L.vca_grad_norm_ws_doubles(10) >= 10
+    assert L.vca_grad_norm_ws_doubles(10, None, None, None) >= 10
+    assert 0 < L.vca_grad_norm_ws_doubles(*ok) < 2050 and L.vca_grad_norm_ws_doubles(1, P(64), N(9), T(0)) == 0

@@ -127,7 +127,7 @@ def _run(M, K, N, dtype, act, seed, mode='fp32', bias=True, res=True):
 # reductions (split over workgroups), the serving kernel's 16-row edge, the 256-wide tiles with and without a tail
 SHAPES = [(1, 1, 1), (1, 8, 16), (2, 3, 5), (1, 512, 512), (7, 129, 33), (15, 1000, 18), (16, 2048, 40), (17, 2048, 40),
           (64, 64, 64), (127, 32, 129), (128, 64, 128), (129, 65, 127), (200, 1111, 77), (333, 96, 513), (40, 5000, 12),
-          (600, 256, 1280)]
+          (600, 256, 1280), (3, 20000, 70), (16, 9001, 33)]
 
 
 @gpu

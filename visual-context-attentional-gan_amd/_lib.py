@@ -203,7 +203,7 @@ _SIGS = {
     'vca_act_bwd': ([_I, _I, _I, _I, _F, _P, _P, _P, _P, _I, _P, _LL, _P], _I),
     'vca_linear_act_bwd_ws_floats': ([ctypes.POINTER(LinearBwd)], _LL),
     'vca_linear_act_bwd': ([ctypes.POINTER(LinearBwd), _P, _LL, _P], _I),
-    'vca_grad_norm_ws_doubles': ([_I], _LL),
+    'vca_grad_norm_ws_doubles': ([_I, _P, _P, _P], _LL),
     'vca_grad_norm': ([_I, _P, _P, _P, _P, _P, _LL, _P, _P], _I),
     'vca_grad_clip': ([_I, _P, _P, _P, _F, _P, _P, _LL, _P, _P], _I),
     'vca_adam_clip_f32': ([_I, _P, _F, _D, _D, _D, _D, _P, _P, _P, _P, _P, _LL, _P, _P], _I),

@@ -50,14 +50,32 @@ template <typename T> union Vec16 {
 // ------------------------------------------------------------------------------------------------
 constexpr float GELU_C = 0.7978845608028654f, GELU_A = 0.044715f;   // sqrt(2 / pi)
 
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+// 1 / (1 + e^-x): the hardware's exponential and reciprocal, each within an ulp or two; 0 and 1 at the ends
+__device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-x)); }
+
+// e = exp(-z^2 / 2) and erfc(|z| / sqrt 2) by Abramowitz & Stegun 7.1.26 (five-term polynomial in 1 / (1 + p x) times
+// e, off by at most 1.5e-7): a dozen instructions where erff takes four times as many, and at 33 M values that is
+// 30 us of the 8192 x 4096 forward pass
+__device__ __forceinline__ float erfc_half(float z, float& e) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+  e = fast_exp(-x * x);
+  return t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * e;
+}
+
 __device__ __forceinline__ float act_f(float z, int act, float slope) {
   switch (act) {
     case VCA_ACT_LEAKY: return z > 0.f ? z : z * slope;
     case VCA_ACT_RELU: return z <= 0.f ? 0.f : z;            // a NaN stays one
     case VCA_ACT_TANH: return tanhf(z);
-    case VCA_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case VCA_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(GELU_C * (z + GELU_A * z * z * z)));
-    case VCA_ACT_SILU: return z / (1.f + expf(-z));
+    case VCA_ACT_GELU: {                                     // z Phi(z); the small tail is multiplied, never subtracted
+      float e;
+      const float q = 0.5f * erfc_half(z, e);
+      return z > 0.f ? z - z * q : z * q;
+    }
+    case VCA_ACT_GELU_TANH: return z * sigmoid_f(2.f * GELU_C * (z + GELU_A * z * z * z));   // (1 + tanh u) / 2
+    case VCA_ACT_SILU: return z * sigmoid_f(z);
     default: return z;
   }
 }
@@ -92,15 +110,18 @@ __device__ __forceinline__ float act_slope(float z, int act, float slope) {
       const float h = tanhf(z);
       return 1.f - h * h;
     }
-    case VCA_ACT_GELU:
-      return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + c * expf(-0.5f * c * c) * 0.3989422804014327f;
+    case VCA_ACT_GELU: {
+      float e;
+      const float q = 0.5f * erfc_half(z, e);
+      return (z > 0.f ? 1.f - q : q) + c * e * 0.3989422804014327f;
+    }
     case VCA_ACT_GELU_TANH: {
-      const float h = tanhf(GELU_C * (z + GELU_A * z * z * z));
-      return 0.5f * (1.f + h) + 0.5f * c * (1.f - h * h) * GELU_C * (1.f + 3.f * GELU_A * c * c);
+      const float s = sigmoid_f(2.f * GELU_C * (z + GELU_A * z * z * z));
+      return s + c * s * (1.f - s) * 2.f * GELU_C * (1.f + 3.f * GELU_A * c * c);
     }
     case VCA_ACT_SILU: {
-      const float e = 1.f / (1.f + expf(-z));
-      return e * (1.f + c * (1.f - e));
+      const float s = sigmoid_f(z);
+      return s + c * s * (1.f - s);
     }
     default: return 1.f;
   }
@@ -108,43 +129,53 @@ __device__ __forceinline__ float act_slope(float z, int act, float slope) {
 
 template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) AnyVec { T e[V]; };
 
+template <typename T, int V>
+__device__ __forceinline__ AnyVec<T, V> load_any(const T* p, int left) {      // left: columns that exist
+  AnyVec<T, V> q;
+  if (left >= V) return *reinterpret_cast<const AnyVec<T, V>*>(p);
+#pragma unroll
+  for (int r = 0; r < V; ++r) q.e[r] = r < left ? p[r] : (T)0.f;
+  return q;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_any(T* p, int left, const float (&v)[V]) {
+  if (left >= V) {
+    AnyVec<T, V> q;
+#pragma unroll
+    for (int r = 0; r < V; ++r) q.e[r] = (T)v[r];
+    *reinterpret_cast<AnyVec<T, V>*>(p) = q;
+  } else {
+#pragma unroll
+    for (int r = 0; r < V; ++r)
+      if (r < left) p[r] = (T)v[r];
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ AnyVec<T, V> bias_of(const MatArgs& g, int n) {
+  return load_any<T, V>(reinterpret_cast<const T*>(g.bias) + n, g.bias ? g.N - n : 0);
+}
+
+template <typename T, int V>
+__device__ __forceinline__ AnyVec<T, V> res_of(const MatArgs& g, int m, int n) {
+  return load_any<T, V>(reinterpret_cast<const T*>(g.res) + (size_t)m * g.ldr + n, g.res ? g.N - n : 0);
+}
+
 // Bias, activation and residual of V neighbouring columns n .. n + V - 1 of row m; stores y and, if kept, z.
 template <typename T, int V>
-__device__ __forceinline__ void finish(const MatArgs& g, int m, int n, float (&v)[V]) {
-  typedef AnyVec<T, V> Any;
-  const T* bias = reinterpret_cast<const T*>(g.bias);
-  const T* res = reinterpret_cast<const T*>(g.res);
-  T* c = reinterpret_cast<T*>(g.c) + (size_t)m * g.ldc + n;
-  T* z = g.z ? reinterpret_cast<T*>(g.z) + (size_t)m * g.N + n : nullptr;
-  const bool whole = n + V <= g.N;
-  auto add = [&](const T* p) {
-    if (whole) {
-      const Any q = *reinterpret_cast<const Any*>(p);
+__device__ __forceinline__ void finish(const MatArgs& g, int m, int n, float (&v)[V], const AnyVec<T, V>& bias,
+                                       const AnyVec<T, V>& res) {
+  const int left = g.N - n;
 #pragma unroll
-      for (int r = 0; r < V; ++r) v[r] += (float)q.e[r];
-    } else {
-#pragma unroll
-      for (int r = 0; r < V; ++r)
-        if (n + r < g.N) v[r] += (float)p[r];
-    }
-  };
-  auto store = [&](T* p) {
-    if (whole) {
-      Any q;
-#pragma unroll
-      for (int r = 0; r < V; ++r) q.e[r] = (T)v[r];
-      *reinterpret_cast<Any*>(p) = q;
-    } else {
-#pragma unroll
-      for (int r = 0; r < V; ++r)
-        if (n + r < g.N) p[r] = (T)v[r];
-    }
-  };
-  if (bias) add(bias + n);
-  if (z) store(z);
+  for (int r = 0; r < V; ++r) v[r] += (float)bias.e[r];
+  if (g.z) store_any<T, V>(reinterpret_cast<T*>(g.z) + (size_t)m * g.N + n, left, v);
   act_all(v, g.act, g.slope);
-  if (res) add(res + (size_t)m * g.ldr + n);
-  store(c);
+  if (g.res) {
+#pragma unroll
+    for (int r = 0; r < V; ++r) v[r] += (float)res.e[r];
+  }
+  store_any<T, V>(reinterpret_cast<T*>(g.c) + (size_t)m * g.ldc + n, left, v);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -339,8 +370,12 @@ __device__ __forceinline__ void store_tile(const MatArgs& g, const f32x4 (&acc)[
     }
     return;
   }
-  constexpr int V = 16 / (int)sizeof(T), PARTS = BM * BN * 4 / (2 * (BM + BN) * 128) < 1 ? 1 : BM * BN * 4 / (2 * (BM + BN) * 128);
-  constexpr int HM = TM / PARTS, TPR = BN / V;
+  constexpr int V = 16 / (int)sizeof(T), TPR = BN / V;
+  constexpr int PARTS = BM * BN * 4 > 2 * (BM + BN) * 128 ? BM * BN * 4 / (2 * (BM + BN) * 128) : 1, HM = TM / PARTS;
+  constexpr int STEP = NT / TPR, ROWS = NWM * HM * 16;       // a thread keeps its columns and takes every STEP-th row
+  static_assert(NT % TPR == 0 && ROWS % STEP == 0, "");
+  const int col = (tid % TPR) * V, n = n0 + col;
+  const AnyVec<T, V> bias = bias_of<T, V>(g, min(n, g.N));
 #pragma unroll
   for (int h = 0; h < PARTS; ++h) {
     __syncthreads();
@@ -352,19 +387,27 @@ __device__ __forceinline__ void store_tile(const MatArgs& g, const f32x4 (&acc)[
         *reinterpret_cast<f32x4*>(smem + row * (BN * 4) + ((pc ^ lc) << 4)) = acc[h * HM + i][j];
       }
     __syncthreads();
+    if (n >= g.N) continue;
+    auto row_of = [&](int row) { return m0 + (row / (HM * 16) * TM + h * HM) * 16 + row % (HM * 16); };
+    int row = tid / TPR, m = row_of(row);
+    AnyVec<T, V> next = res_of<T, V>(g, min(m, g.M - 1), n);
 #pragma unroll 1
-    for (int q = tid; q < NWM * HM * 16 * TPR; q += NT) {
-      const int row = q / TPR, col = (q % TPR) * V;
-      const int m = m0 + (row / (HM * 16) * TM + h * HM) * 16 + row % (HM * 16), n = n0 + col;
-      if (m >= g.M || n >= g.N) continue;
-      float v[V];
+    for (; row < ROWS; row += STEP) {
+      const AnyVec<T, V> res = next;                         // the next row's residual travels under this row's work
+      const int mn = row_of(row + STEP < ROWS ? row + STEP : row);
+      next = res_of<T, V>(g, min(mn, g.M - 1), n);
+      if (m < g.M) {
+        float v[V];
 #pragma unroll
-      for (int e = 0; e < V; e += 4) {
-        const f32x4 t = *reinterpret_cast<const f32x4*>(smem + row * (BN * 4) + ((((col + e) >> 2) ^ (row & 15)) << 4));
+        for (int e = 0; e < V; e += 4) {
+          const f32x4 t =
+              *reinterpret_cast<const f32x4*>(smem + row * (BN * 4) + ((((col + e) >> 2) ^ (row & 15)) << 4));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[e + r] = t[r];
+          for (int r = 0; r < 4; ++r) v[e + r] = t[r];
+        }
+        finish<T, V>(g, m, n, v, bias, res);
       }
-      finish<T, V>(g, m, n, v);
+      m = mn;
     }
   }
 }
@@ -663,23 +706,26 @@ __global__ __launch_bounds__(256) void matmul_fold_kernel(const MatArgs g) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[e + r] += t[r];
       }
-    finish<T, V>(g, m, n, v);
+    finish<T, V>(g, m, n, v, bias_of<T, V>(g, n), res_of<T, V>(g, m, n));
   }
 }
 
 // ------------------------------------------------------------------------------------------------
 // Few rows (M <= 16, both operands with k contiguous): the product reads W once and does next to nothing with it, so
-// there is no tile to share through LDS.  A workgroup owns 16 columns of C; its waves take the reduction's chunks in
-// turn, each lane streaming its own 16 bytes of a W row (and of an x row, out of the caches) straight into an MFMA
-// operand, UNROLL chunks in flight; the waves' partial tiles meet in LDS.  Rows of x beyond M repeat the last one.
+// there is no tile to share through LDS.  A workgroup owns 16 columns of C (and a range of the reduction where there are
+// few columns); each lane streams 16 bytes of a W row, and of an x row out of the caches, straight into an MFMA operand.
+// A wave takes two neighbouring chunks of 64 bytes at a time, so the line of each of its 16 rows is asked for by one wave
+// in a row (31 us against 35 with single chunks dealt out to the waves, 4096 -> 16384 in bf16, 8 rows), and the next two
+// fly under this pair's products.  More in flight (four chunks: 32 us), 32 columns a workgroup (34) or four waves (33)
+// were longer.  Bound by memory: 5.1 TB/s with one row, 4.4 with eight, whose x fragments pass through L2 as well.  The
+// waves' partial tiles meet in LDS.  Rows of x beyond M repeat the last one.
 // ------------------------------------------------------------------------------------------------
-constexpr int FEW_WAVES = 8;
+constexpr int FEW_WAVES = 8, FEW_PAIR = 2, FEW_GROUP = FEW_WAVES * FEW_PAIR;
 
 template <int MODE>
 __global__ __launch_bounds__(FEW_WAVES * 64) void few_rows_kernel(const MatArgs g) {
   typedef typename ElemOf<MODE>::T T;
   constexpr int EPP = 16 / (int)sizeof(T), CK = 4 * EPP;   // elements a lane and a chunk take
-  constexpr int UNROLL = 8;
   __shared__ f32x4 red[FEW_WAVES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lc = lane & 15, lg = lane >> 4;
@@ -709,30 +755,50 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_rows_kernel(const MatArgs 
       for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(w.f[e], x.f[e], acc, 0, 0, 0);
     }
   };
-  const int nc = (g.K + CK - 1) / CK;
-  int c = wave;
-  for (; c + (UNROLL - 1) * FEW_WAVES < nc - 1; c += UNROLL * FEW_WAVES) {     // whole chunks only
-    uint4 w[UNROLL], x[UNROLL];
+  const int cb = blockIdx.y * g.cpz, ce = min((g.K + CK - 1) / CK, cb + g.cpz);   // this workgroup's chunks
+  const int groups = (ce - cb - 1) / FEW_GROUP;            // groups of whole chunks (the last chunk is never in one)
+  uint4 w[2][FEW_PAIR], x[2][FEW_PAIR];
+  auto fetch = [&](int grp, int s) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int k = (c + u * FEW_WAVES) * CK + lg * EPP;
-      w[u] = reinterpret_cast<const Any16*>(wp + k)->u;
-      x[u] = reinterpret_cast<const Any16*>(xp + k)->u;
+    for (int u = 0; u < FEW_PAIR; ++u) {
+      const int k = (cb + grp * FEW_GROUP + wave * FEW_PAIR + u) * CK + lg * EPP;
+      w[s][u] = reinterpret_cast<const Any16*>(wp + k)->u;
+      x[s][u] = reinterpret_cast<const Any16*>(xp + k)->u;
     }
+  };
+  auto use = [&](int s) {
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) mul(w[u], x[u]);
+    for (int u = 0; u < FEW_PAIR; ++u) mul(w[s][u], x[s][u]);
+  };
+  if (groups > 0) fetch(0, 0);
+  int q = 0;
+  for (; q + 2 < groups; q += 2) {
+    fetch(q + 1, 1);
+    use(0);
+    fetch(q + 2, 0);
+    use(1);
   }
-  for (; c < nc; c += FEW_WAVES) mul(load(wp, c), load(xp, c));
+  if (q + 1 < groups) {
+    fetch(q + 1, 1);
+    use(0);
+    use(1);
+  } else if (q < groups) {
+    use(0);
+  }
+  for (int c = cb + groups * FEW_GROUP + wave; c < ce; c += FEW_WAVES) mul(load(wp, c), load(xp, c));
   red[wave][lane] = acc;
   __syncthreads();
   if (wave) return;
 #pragma unroll
-  for (int w = 1; w < FEW_WAVES; ++w) acc += red[w][lane];
+  for (int v = 1; v < FEW_WAVES; ++v) acc += red[v][lane];
   const int n = n0 + 4 * lg;
-  if (lc < g.M && n < g.N) {
-    float v[4] = {acc[0], acc[1], acc[2], acc[3]};
-    finish<T, 4>(g, lc, n, v);
+  if (lc >= g.M || n >= g.N) return;
+  if (g.ksplit > 1) {
+    *reinterpret_cast<f32x4*>(g.part + ((size_t)blockIdx.y * g.M + lc) * g.npad + n) = acc;
+    return;
   }
+  float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+  finish<T, 4>(g, lc, n, v, bias_of<T, 4>(g, n), res_of<T, 4>(g, lc, n));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -900,7 +966,21 @@ int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p) {
   const int per16 = 16 / esz;
   p.dma = (bits & 15) == 0 && (!d.a_col || d.M % per16 == 0) && (!d.b_col || d.N % per16 == 0);
   if (d.M <= 16 && !d.a_col && !d.b_col && (p.mode == MODE_16 || p.mode == MODE_F32)) {
+    // A workgroup streams its 16 rows of W at some 30 GB/s; where columns alone give too few of them to load the memory,
+    // the reduction is split too, if that saves more than the launch that adds the parts (16384 -> 1024 in bf16, one row:
+    // 20 us unsplit).
     p.tile = 0;
+    const int nc = (d.K * esz + 63) / 64, blocks = (d.N + 15) / 16;
+    double best = 0.;
+    for (int ks = 1; ks <= 16 && (ks == 1 || (blocks * ks <= 512 && nc / ks >= 2 * FEW_GROUP)); ++ks) {
+      const int chunks = (nc + ks - 1) / ks;
+      const double us = chunks * 1024. / 30e3 + (ks > 1 ? 4. : 0.);
+      if (ks == 1 || us < best) {
+        best = us;
+        g.cpz = chunks;
+      }
+    }
+    g.ksplit = (nc + g.cpz - 1) / g.cpz;
     return 0;
   }
   // the 256-wide kernel addresses its pieces by 32-bit offsets from the tile: 256 rows (64 of k) of at most 4 MB
@@ -937,13 +1017,14 @@ int launch_mode(const Plan& p, bool a_col, bool b_col, hipStream_t s) {
 }
 
 long long ws_of(const Plan& p) {
-  return p.tile && p.g.ksplit > 1 ? (long long)p.g.ksplit * p.g.M * p.g.npad : 0;
+  return p.g.ksplit > 1 ? (long long)p.g.ksplit * p.g.M * p.g.npad : 0;
 }
 
 // Workspace floats of a product whatever its operands' alignment and strides, so that a caller may ask once a size.
 long long ws_floats_of(const vca_matmul_desc* d) {
   Plan p;
-  if (plan_of(d, nullptr, nullptr, p) != 0 || !p.tile) return 0;
+  if (plan_of(d, nullptr, nullptr, p) != 0) return 0;
+  if (!p.tile) return ws_of(p);
   long long n = 0;
   for (bool wide : {false, true}) {
     const int nc = (p.g.K * (d->type == VCA_T_F32 ? 4ll : 2ll) + 127) / 128;
@@ -955,7 +1036,7 @@ long long ws_floats_of(const vca_matmul_desc* d) {
 
 int act_rows(int M, int N, int esz) {                     // rows a workgroup of act_bwd_kernel takes
   const long long strips = ((long long)N * esz + 511) / 512;
-  int rows = 64;                                          // up to 64 rows: one slab, and no launch to add slabs up
+  int rows = M <= 64 ? 64 : 8;                            // up to 64 rows: one slab, and no launch to add slabs up
   auto slabs = [&]() { return ((long long)M + rows - 1) / rows; };
   while ((rows < 256 && strips * slabs() > 1024) || slabs() > 65535) rows *= 2;   // (65535: the grid's second dimension)
   return rows;
@@ -985,19 +1066,18 @@ extern "C" int vca_matmul_act(const vca_matmul_desc* d, const void* a, const voi
   g.c = c;
   g.z = z;
   hipStream_t s = (hipStream_t)stream;
-  if (p.tile == 0) {
-    const dim3 grid((g.N + 15) / 16);
-    if (p.mode == MODE_16) hipLaunchKernelGGL(few_rows_kernel<MODE_16>, grid, dim3(FEW_WAVES * 64), 0, s, g);
-    else hipLaunchKernelGGL(few_rows_kernel<MODE_F32>, grid, dim3(FEW_WAVES * 64), 0, s, g);
-    return vca_launch_status();
-  }
   if (g.ksplit > 1) {
     VCA_CHECK_ARG(ws && ws_floats >= ws_of(p) && (reinterpret_cast<uintptr_t>(ws) & 15) == 0);
     g.part = ws;
   }
   int e = 0;
   const bool ac = d->a_col != 0, bc = d->b_col != 0;
-  switch (p.mode) {
+  if (p.tile == 0) {
+    const dim3 grid((g.N + 15) / 16, g.ksplit);
+    if (p.mode == MODE_16) hipLaunchKernelGGL(few_rows_kernel<MODE_16>, grid, dim3(FEW_WAVES * 64), 0, s, g);
+    else hipLaunchKernelGGL(few_rows_kernel<MODE_F32>, grid, dim3(FEW_WAVES * 64), 0, s, g);
+    e = vca_launch_status();
+  } else switch (p.mode) {
     case MODE_16: e = launch_mode<MODE_16>(p, ac, bc, s); break;
     case MODE_F32: e = launch_mode<MODE_F32>(p, ac, bc, s); break;
     case MODE_S3: e = launch_mode<MODE_S3>(p, ac, bc, s); break;

@@ -2314,7 +2314,7 @@ class GradNorm:
         self._ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in ts])
         self._numel = (ctypes.c_longlong * n)(*[t.numel() for t in ts])
         self._types = (ctypes.c_int * n)(*[_lib.TYPES[t.dtype] for t in ts])
-        self._ws = int(_lib.lib().vca_grad_norm_ws_doubles(n))
+        self._ws = int(_lib.lib().vca_grad_norm_ws_doubles(n, self._ptrs, self._numel, self._types))
         self._disjoint = None
 
     def norm(self, scaler=None):
@@ -2322,7 +2322,7 @@ class GradNorm:
         with _on_device(self.device):
             out, ws = self._buffers()
             check(_lib.lib().vca_grad_norm(self._n, self._ptrs, self._numel, self._types,
-                                           None if scaler is None else ptr(scaler.scale), ws.data_ptr(), self._ws,
+                                           None if scaler is None else ptr(scaler.scale), _addr(ws), self._ws,
                                            out.data_ptr(), stream()), 'grad_norm')
         return out
 
@@ -2337,14 +2337,14 @@ class GradNorm:
         with _on_device(self.device):
             out, ws = self._buffers()
             check(_lib.lib().vca_grad_clip(self._n, self._ptrs, self._numel, self._types, max_norm,
-                                           None if scaler is None else ptr(scaler.scale), ws.data_ptr(), self._ws,
+                                           None if scaler is None else ptr(scaler.scale), _addr(ws), self._ws,
                                            out.data_ptr(), stream()), 'grad_clip')
         torch.autograd.graph.increment_version(self.tensors)
         return out
 
     def _buffers(self):
         return (torch.empty((), device=self.device, dtype=torch.float32),
-                torch.empty(self._ws, device=self.device, dtype=torch.float64))
+                torch.empty(self._ws, device=self.device, dtype=torch.float64) if self._ws else None)
 
 
 def grad_norm(tensors, scaler=None):
@@ -2355,6 +2355,10 @@ def grad_norm(tensors, scaler=None):
 def clip_grad_norm_(tensors, max_norm, scaler=None):
     """Clip a list of gradient tensors in place by their global 2-norm and return it; see GradNorm."""
     return GradNorm(tensors).clip_(max_norm, scaler)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _max_norm(v):
@@ -2474,10 +2478,10 @@ class FusedAdam:
         n = len(self.groups)
         tab = (_lib.AdamGroup * n)(*[(ptr(f), ptr(g), ptr(st['m']), ptr(st['v']), ptr(st['vmax']), f.numel())
                                      for (f, g), st in zip(self.groups, self.state)])
-        nws = int(L.vca_grad_norm_ws_doubles(n))
+        nws = int(L.vca_grad_norm_ws_doubles(n, None, None, None))
         dev = self.t_dev.device
         ws = torch.empty(nws, device=dev, dtype=torch.float64)
-        out = torch.empty(4, device=dev, dtype=torch.float32)
+        out = torch.empty(5, device=dev, dtype=torch.float32)
         check(L.vca_adam_clip_f32(n, tab, max_norm, self.betas[0], self.betas[1], self.eps, self.weight_decay,
                                   self.t_dev.data_ptr(), self.lr_dev.data_ptr(),
                                   None if scaler is None else ptr(scaler.scale),
