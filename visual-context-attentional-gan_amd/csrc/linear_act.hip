@@ -12,6 +12,7 @@
 // Arithmetic: 16-bit tensors of the library's element type take one product with fp32 accumulation.  fp32 tensors take
 // the exact fp32 MFMA (nsplit 0) or are split in registers into 16-bit parts (nsplit 3: hi hi + hi lo + lo hi; 1: hi).
 // Bias, activation and residual are applied to the fp32 accumulator, so a result is rounded once.
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.h"
@@ -687,18 +688,20 @@ __global__ __launch_bounds__(512) void matmul_wide_kernel(const MatArgs g) {
   store_tile<vca_e16, BM, BM, 2, 4>(g, acc, smem, m0, n0, kz, wm, wn, lc, lg, tid);
 }
 
-// C from the ksplit partial products, added in order of the reduction, through the same epilogue
+// C from the ksplit partial products, added in order of the reduction, through the same epilogue (workgroup `block` of
+// `blocks`)
 template <typename T>
-__global__ __launch_bounds__(256) void matmul_fold_kernel(const MatArgs g) {
+__device__ __forceinline__ void fold_product(const MatArgs& g, int block, int blocks) {
   constexpr int V = 16 / (int)sizeof(T);
   const int nv = (g.N + V - 1) / V;
   const size_t total = (size_t)g.M * nv, slab = (size_t)g.M * g.npad;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+  for (size_t i = (size_t)block * 256 + threadIdx.x; i < total; i += (size_t)blocks * 256) {
     const int m = (int)(i / nv), n = (int)(i - (size_t)m * nv) * V;
     const float* p = g.part + (size_t)m * g.npad + n;      // npad is a multiple of 8
     float v[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = 0.f;
+#pragma unroll 4
     for (int s = 0; s < g.ksplit; ++s)
 #pragma unroll
       for (int e = 0; e < V; e += 4) {
@@ -708,6 +711,47 @@ __global__ __launch_bounds__(256) void matmul_fold_kernel(const MatArgs g) {
       }
     finish<T, V>(g, m, n, v, bias_of<T, V>(g, n), res_of<T, V>(g, m, n));
   }
+}
+
+// db[n] (+)= sum of the slabs: 16 columns a workgroup, each column's slabs in 16 interleaved runs
+struct BiasArgs {
+  const float* part;
+  void* db;
+  int N, slabs, add;
+};
+
+template <typename T>
+__device__ __forceinline__ void fold_bias(const BiasArgs& b, int block, float (*red)[17]) {
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, n = block * 16 + tx;
+  float t = 0.f;
+  if (n < b.N) {
+#pragma unroll 8
+    for (int s = ty; s < b.slabs; s += 16) t += b.part[(size_t)s * b.N + n];
+  }
+  red[ty][tx] = t;
+  __syncthreads();
+  if (ty || n >= b.N) return;
+#pragma unroll
+  for (int y = 1; y < 16; ++y) t += red[y][tx];
+  T* db = reinterpret_cast<T*>(b.db);
+  db[n] = (T)(b.add ? t + (float)db[n] : t);
+}
+
+// What is left to add up behind a forward pass (one product) or a backward pass (two products and the bias gradient), in
+// one launch: workgroups [0, first[1]) take product 0, [first[1], first[2]) product 1, the rest the bias gradient.
+struct FoldArgs {
+  MatArgs g[2];
+  BiasArgs b;
+  int first[4];
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void fold_kernel(const FoldArgs f) {
+  __shared__ float red[16][17];
+  const int w = blockIdx.x;
+  if (w < f.first[1]) fold_product<T>(f.g[0], w, f.first[1]);
+  else if (w < f.first[2]) fold_product<T>(f.g[1], w - f.first[1], f.first[2] - f.first[1]);
+  else fold_bias<T>(f.b, w - f.first[2], red);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -859,25 +903,6 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(int M, int N, int act, flo
     if (gridDim.y > 1) part[(size_t)blockIdx.y * N + col] = t;
     else db[col] = (T)(db_add ? t + (float)db[col] : t);      // the only slab
   }
-}
-
-// db[n] (+)= sum of the slabs: 16 columns a workgroup, each column's slabs in 16 interleaved runs
-template <typename T>
-__global__ __launch_bounds__(256) void bias_fold_kernel(int N, int slabs, const float* __restrict__ part,
-                                                        T* __restrict__ db, int add) {
-  __shared__ float red[16][17];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, n = blockIdx.x * 16 + tx;
-  float t = 0.f;
-  if (n < N) {
-#pragma unroll 8
-    for (int s = ty; s < slabs; s += 16) t += part[(size_t)s * N + n];
-  }
-  red[ty][tx] = t;
-  __syncthreads();
-  if (ty || n >= N) return;
-#pragma unroll
-  for (int y = 1; y < 16; ++y) t += red[y][tx];
-  db[n] = (T)(add ? t + (float)db[n] : t);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1034,6 +1059,60 @@ long long ws_floats_of(const vca_matmul_desc* d) {
   return n;
 }
 
+bool aligned(int type, std::initializer_list<const void*> ps) {
+  uintptr_t bits = 0;
+  for (const void* p : ps) bits |= reinterpret_cast<uintptr_t>(p);
+  return (bits & (type == VCA_T_F32 ? 3 : 1)) == 0;
+}
+
+// The product itself: into C, or into its partial products in ws where the plan splits it.
+int launch_product(Plan& p, const vca_matmul_desc& d, const void* a, const void* b, const void* bias, const void* res,
+                   void* c, void* z, float* ws, hipStream_t s) {
+  MatArgs& g = p.g;
+  g.a = a;
+  g.b = b;
+  g.bias = bias;
+  g.res = res;
+  g.c = c;
+  g.z = z;
+  g.part = g.ksplit > 1 ? ws : nullptr;
+  const bool ac = d.a_col != 0, bc = d.b_col != 0;
+  if (p.tile == 0) {
+    const dim3 grid((g.N + 15) / 16, g.ksplit);
+    if (p.mode == MODE_16) hipLaunchKernelGGL(few_rows_kernel<MODE_16>, grid, dim3(FEW_WAVES * 64), 0, s, g);
+    else hipLaunchKernelGGL(few_rows_kernel<MODE_F32>, grid, dim3(FEW_WAVES * 64), 0, s, g);
+    return vca_launch_status();
+  }
+  switch (p.mode) {
+    case MODE_16: return launch_mode<MODE_16>(p, ac, bc, s);
+    case MODE_F32: return launch_mode<MODE_F32>(p, ac, bc, s);
+    case MODE_S3: return launch_mode<MODE_S3>(p, ac, bc, s);
+    default: return launch_mode<MODE_S1>(p, ac, bc, s);
+  }
+}
+
+void clear(FoldArgs& f) {
+  f.first[0] = f.first[1] = f.first[2] = f.first[3] = 0;
+  f.b = {nullptr, nullptr, 0, 0, 0};
+}
+
+// Adds up what is split: up to two products and the bias gradient in f.b (slabs 0: none).
+int launch_folds(FoldArgs& f, const MatArgs* g0, const MatArgs* g1, int type, hipStream_t s) {
+  auto blocks = [&](const MatArgs& g) {
+    const long long n = ((long long)g.M * (g.npad / (type == VCA_T_F32 ? 4 : 8)) + 255) / 256;
+    return (int)(n > 4096 ? 4096 : n);
+  };
+  if (g0) f.g[0] = *g0;
+  if (g1) f.g[1] = *g1;
+  f.first[1] = g0 ? blocks(*g0) : 0;
+  f.first[2] = f.first[1] + (g1 ? blocks(*g1) : 0);
+  f.first[3] = f.first[2] + (f.b.slabs ? (f.b.N + 15) / 16 : 0);
+  if (!f.first[3]) return 0;
+  if (type == VCA_T_F32) hipLaunchKernelGGL(fold_kernel<float>, dim3(f.first[3]), dim3(256), 0, s, f);
+  else hipLaunchKernelGGL(fold_kernel<vca_e16>, dim3(f.first[3]), dim3(256), 0, s, f);
+  return vca_launch_status();
+}
+
 int act_rows(int M, int N, int esz) {                     // rows a workgroup of act_bwd_kernel takes
   const long long strips = ((long long)N * esz + 511) / 512;
   int rows = M <= 64 ? 64 : 8;                            // up to 64 rows: one slab, and no launch to add slabs up
@@ -1054,41 +1133,12 @@ extern "C" int vca_matmul_act(const vca_matmul_desc* d, const void* a, const voi
   VCA_CHECK_ARG(a && b && c);
   const int rc = plan_of(d, a, b, p);
   if (rc) return rc;
-  const int esz = d->type == VCA_T_F32 ? 4 : 2;
-  VCA_CHECK_ARG(((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(bias) |
-                  reinterpret_cast<uintptr_t>(res) | reinterpret_cast<uintptr_t>(c) | reinterpret_cast<uintptr_t>(z)) &
-                 (esz - 1)) == 0);
-  MatArgs& g = p.g;
-  g.a = a;
-  g.b = b;
-  g.bias = bias;
-  g.res = res;
-  g.c = c;
-  g.z = z;
-  hipStream_t s = (hipStream_t)stream;
-  if (g.ksplit > 1) {
-    VCA_CHECK_ARG(ws && ws_floats >= ws_of(p) && (reinterpret_cast<uintptr_t>(ws) & 15) == 0);
-    g.part = ws;
-  }
-  int e = 0;
-  const bool ac = d->a_col != 0, bc = d->b_col != 0;
-  if (p.tile == 0) {
-    const dim3 grid((g.N + 15) / 16, g.ksplit);
-    if (p.mode == MODE_16) hipLaunchKernelGGL(few_rows_kernel<MODE_16>, grid, dim3(FEW_WAVES * 64), 0, s, g);
-    else hipLaunchKernelGGL(few_rows_kernel<MODE_F32>, grid, dim3(FEW_WAVES * 64), 0, s, g);
-    e = vca_launch_status();
-  } else switch (p.mode) {
-    case MODE_16: e = launch_mode<MODE_16>(p, ac, bc, s); break;
-    case MODE_F32: e = launch_mode<MODE_F32>(p, ac, bc, s); break;
-    case MODE_S3: e = launch_mode<MODE_S3>(p, ac, bc, s); break;
-    default: e = launch_mode<MODE_S1>(p, ac, bc, s); break;
-  }
-  if (e || g.ksplit == 1) return e;
-  const size_t nv = (size_t)g.M * (g.npad / (16 / esz));
-  const dim3 grid((unsigned)(nv / 256 + 1 > 4096 ? 4096 : nv / 256 + 1));
-  if (esz == 4) hipLaunchKernelGGL(matmul_fold_kernel<float>, grid, dim3(256), 0, s, g);
-  else hipLaunchKernelGGL(matmul_fold_kernel<vca_e16>, grid, dim3(256), 0, s, g);
-  return vca_launch_status();
+  VCA_CHECK_ARG(aligned(d->type, {a, b, bias, res, c, z}));
+  VCA_CHECK_ARG(ws_of(p) == 0 || (ws && ws_floats >= ws_of(p) && (reinterpret_cast<uintptr_t>(ws) & 15) == 0));
+  const int e = launch_product(p, *d, a, b, bias, res, c, z, ws, (hipStream_t)stream);
+  FoldArgs f;
+  clear(f);
+  return e ? e : launch_folds(f, p.g.ksplit > 1 ? &p.g : nullptr, nullptr, d->type, (hipStream_t)stream);
 }
 
 extern "C" long long vca_act_bwd_ws_floats(int type, int M, int N) {
@@ -1097,16 +1147,10 @@ extern "C" long long vca_act_bwd_ws_floats(int type, int M, int N) {
   return ((long long)M + rows - 1) / rows * N;
 }
 
-extern "C" int vca_act_bwd(int type, int M, int N, int act, float slope, const void* gy, const void* z, void* dz, void* db,
-                           int db_add, float* ws, long long ws_floats, void* stream) {
-  const int own16 = VCA_ELEM_TYPE ? VCA_T_F16 : VCA_T_BF16;
-  VCA_CHECK_ARG((type == VCA_T_F32 || type == own16) && M > 0 && N > 0 && act_ok(act) && gy && (dz || db));
-  VCA_CHECK_ARG((act == VCA_ACT_NONE) == !z && (!dz || z));
+// Launches dz and the slabs of db; leaves in f what of db is left to add up.
+static int act_bwd(int type, int M, int N, int act, float slope, const void* gy, const void* z, void* dz, void* db,
+                   int db_add, float* ws, FoldArgs& f, hipStream_t s) {
   const int esz = type == VCA_T_F32 ? 4 : 2, rows = act_rows(M, N, esz), slabs = (int)(((long long)M + rows - 1) / rows);
-  VCA_CHECK_ARG(((reinterpret_cast<uintptr_t>(gy) | reinterpret_cast<uintptr_t>(z) | reinterpret_cast<uintptr_t>(dz) |
-                  reinterpret_cast<uintptr_t>(db)) & (esz - 1)) == 0);
-  VCA_CHECK_ARG(!db || (ws && ws_floats >= (long long)slabs * N && (reinterpret_cast<uintptr_t>(ws) & 3) == 0));
-  hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)(((long long)N * esz + 511) / 512), (unsigned)slabs);
   if (esz == 4)
     hipLaunchKernelGGL(act_bwd_kernel<float>, grid, dim3(256), 0, s, M, N, act, slope, (const float*)gy, (const float*)z,
@@ -1114,12 +1158,24 @@ extern "C" int vca_act_bwd(int type, int M, int N, int act, float slope, const v
   else
     hipLaunchKernelGGL(act_bwd_kernel<vca_e16>, grid, dim3(256), 0, s, M, N, act, slope, (const vca_e16*)gy,
                        (const vca_e16*)z, (vca_e16*)dz, ws, rows, (vca_e16*)db, db_add);
-  if (db && slabs > 1) {
-    const dim3 fg((N + 15) / 16);
-    if (esz == 4) hipLaunchKernelGGL(bias_fold_kernel<float>, fg, dim3(256), 0, s, N, slabs, ws, (float*)db, db_add);
-    else hipLaunchKernelGGL(bias_fold_kernel<vca_e16>, fg, dim3(256), 0, s, N, slabs, ws, (vca_e16*)db, db_add);
-  }
+  if (db && slabs > 1) f.b = {ws, db, N, slabs, db_add};
   return vca_launch_status();
+}
+
+static bool act_bwd_ok(int type, int M, int N, int act, const void* gy, const void* z, const void* dz, const void* db) {
+  const int own16 = VCA_ELEM_TYPE ? VCA_T_F16 : VCA_T_BF16;
+  return (type == VCA_T_F32 || type == own16) && M > 0 && N > 0 && act_ok(act) && gy && (act == VCA_ACT_NONE) == !z &&
+         (!dz || z) && aligned(type, {gy, z, dz, db});
+}
+
+extern "C" int vca_act_bwd(int type, int M, int N, int act, float slope, const void* gy, const void* z, void* dz, void* db,
+                           int db_add, float* ws, long long ws_floats, void* stream) {
+  VCA_CHECK_ARG(act_bwd_ok(type, M, N, act, gy, z, dz, db) && (dz || db));
+  VCA_CHECK_ARG(!db || (ws && ws_floats >= vca_act_bwd_ws_floats(type, M, N) && (reinterpret_cast<uintptr_t>(ws) & 3) == 0));
+  FoldArgs f;
+  clear(f);
+  const int e = act_bwd(type, M, N, act, slope, gy, z, dz, db, db_add, ws, f, (hipStream_t)stream);
+  return e ? e : launch_folds(f, nullptr, nullptr, type, (hipStream_t)stream);
 }
 
 // The three products' descriptors of a backward pass.
@@ -1133,43 +1189,41 @@ static vca_matmul_desc bwd_dw(const vca_linear_bwd& b) {
   return d;
 }
 
+static long long up4(long long n) { return (n + 3) / 4 * 4; }   // each part of the workspace starts at 16 bytes
+
 extern "C" long long vca_linear_act_bwd_ws_floats(const vca_linear_bwd* b) {
   if (!b || b->M <= 0 || b->N <= 0 || b->K <= 0) return 0;
   const vca_matmul_desc x = bwd_dx(*b), w = bwd_dw(*b);
-  long long n = vca_act_bwd_ws_floats(b->type, b->M, b->N);
-  const long long nx = ws_floats_of(&x), nw = ws_floats_of(&w);
-  n = nx > n ? nx : n;
-  return nw > n ? nw : n;
+  return up4(vca_act_bwd_ws_floats(b->type, b->M, b->N)) + up4(ws_floats_of(&x)) + ws_floats_of(&w);
 }
 
 extern "C" int vca_linear_act_bwd(const vca_linear_bwd* b, float* ws, long long ws_floats, void* stream) {
-  VCA_CHECK_ARG(b && b->gy && b->M > 0 && b->N > 0 && b->K > 0 && (b->act == VCA_ACT_NONE) == !b->z);
-  VCA_CHECK_ARG((!b->dx || b->w) && (!b->dw || b->x) && ((b->act == VCA_ACT_NONE) == !b->dz || !(b->dx || b->dw)));
-  // (checked before the first launch: a refused call has written nothing)
+  VCA_CHECK_ARG(b && b->K > 0 && act_bwd_ok(b->type, b->M, b->N, b->act, b->gy, b->z, b->dz, b->db));
+  VCA_CHECK_ARG((!b->dx || b->w) && (!b->dw || b->x) && (b->act == VCA_ACT_NONE || b->dz || !(b->dx || b->dw)));
+  VCA_CHECK_ARG(aligned(b->type, {b->x, b->w, b->dx, b->dw}));
+  // (everything is checked before the first launch: a refused call has written nothing)
   const vca_matmul_desc x = bwd_dx(*b), w = bwd_dw(*b);
   const void* dz = b->dz ? b->dz : b->gy;
-  long long need = b->db ? vca_act_bwd_ws_floats(b->type, b->M, b->N) : 0;
-  Plan p;
+  Plan px, pw;
+  px.g.ksplit = pw.g.ksplit = 1;
   if (b->dx) {
-    const int rc = plan_of(&x, dz, b->w, p);
+    const int rc = plan_of(&x, dz, b->w, px);
     if (rc) return rc;
-    need = ws_of(p) > need ? ws_of(p) : need;
   }
   if (b->dw) {
-    const int rc = plan_of(&w, dz, b->x, p);
+    const int rc = plan_of(&w, dz, b->x, pw);
     if (rc) return rc;
-    need = ws_of(p) > need ? ws_of(p) : need;
   }
+  // one part of the workspace for each of db, dx and dw, so that what is split is added up by one launch at the end
+  const long long at_x = b->db ? up4(vca_act_bwd_ws_floats(b->type, b->M, b->N)) : 0;
+  const long long at_w = at_x + (b->dx ? up4(ws_of(px)) : 0), need = at_w + (b->dw ? ws_of(pw) : 0);
   VCA_CHECK_ARG(ws_floats >= need && (!need || (ws && (reinterpret_cast<uintptr_t>(ws) & 15) == 0)));
-  if (b->dz || b->db) {
-    const int rc = vca_act_bwd(b->type, b->M, b->N, b->act, b->slope, b->gy, b->z, b->dz, b->db, b->db_add, ws, ws_floats,
-                               stream);
-    if (rc) return rc;
-  }
-  if (b->dx) {
-    const int rc = vca_matmul_act(&x, dz, b->w, nullptr, nullptr, b->dx, nullptr, ws, ws_floats, stream);
-    if (rc) return rc;
-  }
-  if (b->dw) return vca_matmul_act(&w, dz, b->x, nullptr, b->dw_add ? b->dw : nullptr, b->dw, nullptr, ws, ws_floats, stream);
-  return 0;
+  hipStream_t s = (hipStream_t)stream;
+  FoldArgs f;
+  clear(f);
+  int e = 0;
+  if (b->dz || b->db) e = act_bwd(b->type, b->M, b->N, b->act, b->slope, b->gy, b->z, b->dz, b->db, b->db_add, ws, f, s);
+  if (!e && b->dx) e = launch_product(px, x, dz, b->w, nullptr, nullptr, b->dx, nullptr, ws + at_x, s);
+  if (!e && b->dw) e = launch_product(pw, w, dz, b->x, nullptr, b->dw_add ? b->dw : nullptr, b->dw, nullptr, ws + at_w, s);
+  return e ? e : launch_folds(f, px.g.ksplit > 1 ? &px.g : nullptr, pw.g.ksplit > 1 ? &pw.g : nullptr, b->type, s);
 }

@@ -874,39 +874,42 @@ class LinearActFn(torch.autograd.Function):
         return _linear_act_fwd(x, w, bias, res, code, z)
 
     @staticmethod
-    @once
     def backward(ctx, gy):
-        x, w, z = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        if _inputs_only[0]:
-            need_w = need_b = False
-        gx = gw = gb = None
-        if need_x or need_w or need_b:
-            (M, K), N, dt, dev = x.shape, w.shape[0], x.dtype, x.device
-            g = gy.contiguous()
-            wsink = _grad_sink(w) if need_w else None
-            bsink = _grad_sink(ctx.bias_param) if need_b else None
-            with _on_device(dev):
-                new = lambda *shape: torch.empty(shape, device=dev, dtype=dt)
-                dz = new(M, N) if z is not None and (need_x or need_w) else None
-                gx = new(M, K) if need_x else None
-                gw = (new(N, K) if wsink is None else wsink) if need_w else None
-                gb = (new(N) if bsink is None else bsink) if need_b else None
-                at = lambda t: None if t is None else t.data_ptr()
-                L = _lib.lib(_ELEM_OF[dt])
-                ns = _nsplit(True) if dt == torch.float32 else 1
-                d = _lib.LinearBwd(M, N, K, _lib.TYPES[dt], ns, ctx.code[0], wsink is not None, bsink is not None,
-                                   ctx.code[1], _row_step(x), _row_step(w), g.data_ptr(), x.data_ptr(), w.data_ptr(),
-                                   at(z), at(dz), at(gx), at(gw), at(gb))
-                key = (M, N, K, dt, ns, 'bwd')
-                n = _act_ws.get(key)
-                if n is None:
-                    n = _act_ws[key] = int(L.vca_linear_act_bwd_ws_floats(d))
-                ws = torch.empty(n, device=dev, dtype=torch.float32)
-                check(L.vca_linear_act_bwd(d, ws.data_ptr(), n, stream()), 'linear_act_bwd')
-            gw = gw if wsink is None else None
-            gb = gb if bsink is None else None
-        return gx, gw, gb, gy if need_r else None, None
+        # (the decorator only matters under create_graph, where it makes a second differentiation an error)
+        return _linear_act_bwd_once(ctx, gy) if torch.is_grad_enabled() else _linear_act_bwd(ctx, gy)
+
+
+def _linear_act_bwd(ctx, gy):
+    x, w, z = ctx.saved_tensors
+    need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+    if _inputs_only[0]:
+        need_w = need_b = False
+    if not (need_x or need_w or need_b):
+        return None, None, None, gy if need_r else None, None
+    (M, K), N, dt, dev = x.shape, w.shape[0], x.dtype, x.device
+    g = gy.contiguous()
+    wsink = _grad_sink(w) if need_w else None
+    bsink = _grad_sink(ctx.bias_param) if need_b else None
+    with _on_device(dev):
+        dz = torch.empty((M, N), device=dev, dtype=dt) if z is not None and (need_x or need_w) else None
+        gx = torch.empty((M, K), device=dev, dtype=dt) if need_x else None
+        gw = (torch.empty((N, K), device=dev, dtype=dt) if wsink is None else wsink) if need_w else None
+        gb = (torch.empty(N, device=dev, dtype=dt) if bsink is None else bsink) if need_b else None
+        L = _lib.lib(_ELEM_OF[dt])
+        ns = _nsplit(True) if dt == torch.float32 else 1
+        d = _lib.LinearBwd(M, N, K, _lib.TYPES[dt], ns, ctx.code[0], wsink is not None, bsink is not None, ctx.code[1],
+                           _row_step(x), _row_step(w), g.data_ptr(), x.data_ptr(), w.data_ptr(), _addr(z), _addr(dz),
+                           _addr(gx), _addr(gw), _addr(gb))
+        key = (M, N, K, dt, ns, 'bwd')
+        n = _act_ws.get(key)
+        if n is None:
+            n = _act_ws[key] = int(L.vca_linear_act_bwd_ws_floats(d))
+        ws = torch.empty(n, device=dev, dtype=torch.float32)
+        check(L.vca_linear_act_bwd(d, ws.data_ptr(), n, stream()), 'linear_act_bwd')
+    return gx, gw if wsink is None else None, gb if bsink is None else None, gy if need_r else None, None
+
+
+_linear_act_bwd_once = once(_linear_act_bwd)
 
 
 def linear_act(x, w, bias=None, act=None, residual=None):
