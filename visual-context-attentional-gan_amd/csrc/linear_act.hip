@@ -373,12 +373,20 @@ __device__ __forceinline__ void store_tile(const MatArgs& g, const f32x4 (&acc)[
   }
   constexpr int V = 16 / (int)sizeof(T), TPR = BN / V;
   constexpr int PARTS = BM * BN * 4 > 2 * (BM + BN) * 128 ? BM * BN * 4 / (2 * (BM + BN) * 128) : 1, HM = TM / PARTS;
-  constexpr int STEP = NT / TPR, ROWS = NWM * HM * 16;       // a thread keeps its columns and takes every STEP-th row
-  static_assert(NT % TPR == 0 && ROWS % STEP == 0, "");
+  constexpr int STEP = NT / TPR, ROWS = NWM * HM * 16, ITER = ROWS / STEP;   // a thread keeps its columns and takes
+  static_assert(NT % TPR == 0 && ROWS % STEP == 0, "");                      // every STEP-th row
   const int col = (tid % TPR) * V, n = n0 + col;
   const AnyVec<T, V> bias = bias_of<T, V>(g, min(n, g.N));
 #pragma unroll
   for (int h = 0; h < PARTS; ++h) {
+    auto row_of = [&](int row) { return m0 + (row / (HM * 16) * TM + h * HM) * 16 + row % (HM * 16); };
+    // All of the part's residual is asked for at once, under the turn through LDS.  The counter that loads and stores
+    // share is in order, so a load between the rows' stores would wait for memory twice a row.
+    AnyVec<T, V> res[ITER];
+    if (g.res && n < g.N) {
+#pragma unroll
+      for (int k = 0; k < ITER; ++k) res[k] = res_of<T, V>(g, min(row_of(tid / TPR + k * STEP), g.M - 1), n);
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < HM; ++i)
@@ -389,14 +397,9 @@ __device__ __forceinline__ void store_tile(const MatArgs& g, const f32x4 (&acc)[
       }
     __syncthreads();
     if (n >= g.N) continue;
-    auto row_of = [&](int row) { return m0 + (row / (HM * 16) * TM + h * HM) * 16 + row % (HM * 16); };
-    int row = tid / TPR, m = row_of(row);
-    AnyVec<T, V> next = res_of<T, V>(g, min(m, g.M - 1), n);
 #pragma unroll 1
-    for (; row < ROWS; row += STEP) {
-      const AnyVec<T, V> res = next;                         // the next row's residual travels under this row's work
-      const int mn = row_of(row + STEP < ROWS ? row + STEP : row);
-      next = res_of<T, V>(g, min(mn, g.M - 1), n);
+    for (int row = tid / TPR; row < ROWS; row += STEP) {
+      const int m = row_of(row);
       if (m < g.M) {
         float v[V];
 #pragma unroll
@@ -406,9 +409,10 @@ __device__ __forceinline__ void store_tile(const MatArgs& g, const f32x4 (&acc)[
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[e + r] = t[r];
         }
-        finish<T, V>(g, m, n, v, bias, res);
+        finish<T, V>(g, m, n, v, bias, res[0]);
       }
-      m = mn;
+#pragma unroll
+      for (int k = 0; k + 1 < ITER; ++k) res[k] = res[k + 1];      // (a rolled loop: the rows share one copy of the code)
     }
   }
 }
