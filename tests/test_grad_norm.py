@@ -124,6 +124,17 @@ def test_dense_layouts_and_an_integer_number_of_bits():
 
 
 @gpu
+def test_elements_beyond_32_bits():
+    from vcagan_amd import ops
+    n = 2 ** 31 + 12345
+    t = torch.zeros(n + 1, device='cuda', dtype=torch.bfloat16)[1:]
+    t[0], t[2 ** 31 + 5], t[-1] = 3.0, 4.0, 12.0
+    assert float(ops.clip_grad_norm_([t], 6.5)) == 13.0
+    assert [float(t[i]) for i in (0, 2 ** 31 + 5, n - 1)] == [1.5, 2.0, 6.0]
+    assert int((t != 0).sum()) == 3
+
+
+@gpu
 def test_scaled_gradients():
     from vcagan_amd import ops
     ts = _list([777, 50001], (torch.float32,), 2)

@@ -6,8 +6,9 @@ Tolerances (u = 2^-24, e = half an ulp of the tensors' type, finfo.eps / 2; |.| 
          16-bit parts of half-ulp h: the dropped lo lo and the rounding of the two lo parts, 3 h^2, single product:
          2 h + h^2) and (K + 8) u (|x| |w|^T + |b|) for fp32 accumulation in any order
   y      |act'| <= 1.13 times that, 8 u (|z| + 1) for the activation's own evaluation, 2 u (|act| + |r|), and e |y|
-  dz     |gy| |act''| (dz + e |z|) with |act''| <= 1.13 for the smooth activations, 16 u |gy|; where a kinked
-         activation's |z| is within dz + e |z| of its kink the slope may be the other one; and e |dz|
+  dz     |gy| |act''| (dz + k |z|) with |act''| <= 1.13 for the smooth activations and k half an ulp of the type z is
+         kept in (half for bf16, fp32 for fp32 and half), 16 u |gy|; where a kinked activation's |z| is within that of
+         its kink the slope may be the other one; and e |dz|
   dx     dz's error times |w|, the product's own error as above, and e |dx|; dw likewise with |x|; db = sum |gy| ... of
          dz before its rounding, M u sum |dz|, and e |db|
 Half precision adds its smallest subnormal's half, 2^-25, per rounding."""
@@ -81,7 +82,7 @@ def _reference(x, w, b, r, gy, act, mode):
     if act is None:
         eu = torch.zeros_like(dz)
     else:
-        off = ez + e * z.abs() + tiny
+        off = ez + (2.0 ** -11 * z.abs() + 2.0 ** -25 if t == torch.bfloat16 else U * z.abs())
         eu = (G.abs() * torch.where(z.abs() <= off, 1.0, 0.0) if act in ('relu', 'leaky0.2')
               else 1.13 * G.abs() * off) + 16 * U * G.abs()
     ed = eu + (0.0 if act is None else e * (dz.abs() + eu) + tiny)
@@ -264,6 +265,7 @@ def test_rows_of_the_output_beyond_it_stay():
         x, w, _, _, _ = _inputs(M, K, N, torch.float32, 4)
         c = torch.full((M + 2, N + 5), 7.5, device='cuda')
         d = _lib.MatmulDesc(M, N, K, 0, 0, 0, 0, 0, 0.0, K, K, N + 5, 0)
+        d = ctypes.byref(d)
         n = L.vca_matmul_act_ws_floats(d)
         ws = torch.empty(n + 4, device='cuda')
         ws[n:] = 3.25
@@ -323,6 +325,45 @@ def test_streams_and_graph_replay():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(out, want)), rep
+
+
+@gpu
+def test_elements_beyond_32_bits():
+    """2.2e9 elements of x, y and dz: the last rows come out as the same rows alone do."""
+    from vcagan_amd import ops
+    M, K, N = 2_800_000, 768, 776
+    x = torch.zeros(M, K, device='cuda', dtype=torch.bfloat16)
+    g = torch.Generator().manual_seed(1)
+    tail = torch.randn(300, K, generator=g).to(torch.bfloat16).cuda()
+    x[-300:] = tail
+    w = (torch.randn(N, K, generator=g) / 28).to(torch.bfloat16).cuda().requires_grad_(True)
+    small = ops.linear_act(tail, w, act='silu')
+    y = ops.linear_act(x, w, act='silu')
+    # (another tile may add up in another order, and a rounding to bf16 then fall the other way: one ulp, 2^-7)
+    assert float((y[-300:] - small).detach().abs().max()) <= 2.0 ** -7 * float(small.detach().abs().max())
+    assert float(y[:-300].detach().abs().max()) == 0.0
+    gw, = torch.autograd.grad(y, w, torch.ones_like(y))
+    ws, = torch.autograd.grad(small, w, torch.ones_like(small))
+    assert float((gw - ws).abs().max()) <= 2.0 ** -7 * float(ws.abs().max())      # likewise
+
+
+@gpu
+def test_two_streams_at_once():
+    """Calls on two streams share no workspace: interleaved, each gives what it gives alone."""
+    from vcagan_amd import ops
+    a, b = _inputs(60, 4000, 50, torch.float32, 1), _inputs(60, 4000, 50, torch.float32, 2)
+    want = [ops.linear_act(v[0], v[1], v[2], act='gelu', residual=v[3]) for v in (a, b)]
+    norms = [ops.grad_norm([v[0], v[1]]) for v in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i, (s, v) in enumerate(zip(streams, (a, b))):
+            with torch.cuda.stream(s):
+                got[i].append((ops.linear_act(v[0], v[1], v[2], act='gelu', residual=v[3]), ops.grad_norm([v[0], v[1]])))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) and torch.equal(n, norms[i]) for y, n in got[i])
 
 
 @gpu
@@ -395,6 +436,14 @@ def test_refusals_on_device_tensors():
         g.sum().backward()
 
 
+def test_packed_structures_are_the_declared_ones():
+    from vcagan_amd import _lib
+    v = [3, 5, 7, 1, 1, 0, 1, 6, 0.25, 11, 13, 17, 19]
+    assert bytes(_lib.MatmulDesc(*v)) == _lib.pack_matmul(*v)
+    v = [3, 5, 7, 1, 1, 6, 1, 0, 0.25, 11, 13, 64, 128, 192, 0, 320, 384, 448, 512]
+    assert bytes(_lib.LinearBwd(*[None if x == 0 and i > 10 else x for i, x in enumerate(v)])) == _lib.pack_linear_bwd(*v)
+
+
 def test_refusals_without_a_gpu():
     from vcagan_amd import ops
     with pytest.raises(ValueError):
@@ -409,7 +458,7 @@ def test_entry_points_refuse_before_any_launch():
         L = _lib.lib(elem)
         ok = dict(M=64, N=64, K=64, type=0, nsplit=0, a_col=0, b_col=0, act=0, slope=0.0, lda=64, ldb=64, ldc=64, ldr=64)
         call = lambda a=64, b=64, c=64, ws=64, n=1 << 30, bias=None, **kw: L.vca_matmul_act(
-            _lib.MatmulDesc(**dict(ok, **kw)), a, b, bias, None, c, None, ws, n, None)
+            ctypes.byref(_lib.MatmulDesc(**dict(ok, **kw))), a, b, bias, None, c, None, ws, n, None)
         for kw in (dict(M=0), dict(N=0), dict(K=0), dict(K=-5), dict(type=3), dict(type=other, nsplit=1),
                    dict(type=own, nsplit=0), dict(type=own, nsplit=3), dict(nsplit=2), dict(act=2), dict(act=8),
                    dict(lda=63), dict(ldb=63), dict(ldc=63), dict(ldr=-1), dict(a_col=1, b_col=0),
@@ -417,7 +466,7 @@ def test_entry_points_refuse_before_any_launch():
                    dict(a=66), dict(bias=65)):
             assert call(**kw) == -22, kw
         long = dict(K=1 << 16, lda=1 << 16, ldb=1 << 16)
-        n = L.vca_matmul_act_ws_floats(_lib.MatmulDesc(**dict(ok, **long)))
+        n = L.vca_matmul_act_ws_floats(ctypes.byref(_lib.MatmulDesc(**dict(ok, **long))))
         assert n > 0 and n % (64 * 64) == 0
         assert call(ws=None, **long) == -22 and call(n=n - 1, **long) == -22 and call(ws=68, **long) == -22
         f = lambda type=0, M=4, N=4, act=6, gy=64, z=64, dz=64, db=64, ws=64, n=1 << 20: L.vca_act_bwd(
@@ -428,9 +477,9 @@ def test_entry_points_refuse_before_any_launch():
         assert L.vca_act_bwd_ws_floats(0, 0, 4) == 0
         bwd = dict(M=64, N=64, K=64, type=0, nsplit=0, act=6, dw_add=0, db_add=0, slope=0.0, ldx=64, ldw=64, gy=64, x=64,
                    w=64, z=64, dz=64, dx=64, dw=64, db=64)
-        n = L.vca_linear_act_bwd_ws_floats(_lib.LinearBwd(**bwd))
+        n = L.vca_linear_act_bwd_ws_floats(ctypes.byref(_lib.LinearBwd(**bwd)))
         assert n > 0
-        g = lambda ws=64, n=n, **kw: L.vca_linear_act_bwd(_lib.LinearBwd(**dict(bwd, **kw)), ws, n, None)
+        g = lambda ws=64, n=n, **kw: L.vca_linear_act_bwd(ctypes.byref(_lib.LinearBwd(**dict(bwd, **kw))), ws, n, None)
         for kw in (dict(gy=None), dict(M=0), dict(K=0), dict(act=0), dict(act=2), dict(z=None), dict(dz=None),
                    dict(type=other, nsplit=1), dict(nsplit=2), dict(w=None), dict(x=None), dict(ldx=63), dict(ldw=63),
                    dict(n=n - 1), dict(ws=None), dict(ws=72)):

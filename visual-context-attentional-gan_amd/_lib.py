@@ -10,6 +10,7 @@ entry point without matrix products is the same code in both.
 import concurrent.futures
 import ctypes
 import os
+import struct
 import subprocess
 
 import torch
@@ -98,6 +99,11 @@ class LinearBwd(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in ('M', 'N', 'K', 'type', 'nsplit', 'act', 'dw_add', 'db_add')] + \
         [('slope', ctypes.c_float)] + [(n, ctypes.c_longlong) for n in ('ldx', 'ldw')] + \
         [(n, ctypes.c_void_p) for n in ('gy', 'x', 'w', 'z', 'dz', 'dx', 'dw', 'db')]
+
+
+# The two structures above as bytes: packing one takes a fifth of the time of filling a ctypes.Structure.
+pack_matmul = struct.Struct('8if4q').pack
+pack_linear_bwd = struct.Struct('8if2q8P').pack
 
 
 class AdamGroup(ctypes.Structure):
@@ -197,12 +203,12 @@ _SIGS = {
     'vca_loss_scale_count': ([_P, _P, _P], _I),
     'vca_adam_scaled_f32': ([_LL, _P, _P, _P, _P, _P, _F, _F, _F, _F, _P, _P, _P, _P, _P], _I),
     'vca_loss_scale_update': ([_P, _P, _F, _F, _I, _P], _I),
-    'vca_matmul_act_ws_floats': ([ctypes.POINTER(MatmulDesc)], _LL),
-    'vca_matmul_act': ([ctypes.POINTER(MatmulDesc)] + [_P] * 7 + [_LL, _P], _I),
+    'vca_matmul_act_ws_floats': ([_P], _LL),
+    'vca_matmul_act': ([_P] * 8 + [_LL, _P], _I),
     'vca_act_bwd_ws_floats': ([_I, _I, _I], _LL),
     'vca_act_bwd': ([_I, _I, _I, _I, _F, _P, _P, _P, _P, _I, _P, _LL, _P], _I),
-    'vca_linear_act_bwd_ws_floats': ([ctypes.POINTER(LinearBwd)], _LL),
-    'vca_linear_act_bwd': ([ctypes.POINTER(LinearBwd), _P, _LL, _P], _I),
+    'vca_linear_act_bwd_ws_floats': ([_P], _LL),
+    'vca_linear_act_bwd': ([_P, _P, _LL, _P], _I),
     'vca_grad_norm_ws_doubles': ([_I, _P, _P, _P], _LL),
     'vca_grad_norm': ([_I, _P, _P, _P, _P, _P, _LL, _P, _P], _I),
     'vca_grad_clip': ([_I, _P, _P, _P, _F, _P, _P, _LL, _P, _P], _I),

@@ -24,6 +24,17 @@ enum { MODE_16 = 0, MODE_F32 = 1, MODE_S3 = 2, MODE_S1 = 3 };   // 16-bit tensor
 template <int MODE> struct ElemOf { typedef float T; };
 template <> struct ElemOf<MODE_16> { typedef vca_e16 T; };
 
+// What the value under the activation is kept in for the backward pass.  Its rounding enters dz next to dz's own, so it
+// has to be the smaller of the two: three more bits than bf16 in the same room (the slopes are 0, 1 or flat long before
+// half's range ends, an infinity included), fp32 beside half.
+#ifdef VCA_E16_FP16
+typedef float vca_z16;
+#else
+typedef _Float16 vca_z16;
+#endif
+template <typename T> struct ZOf { typedef float type; };
+template <> struct ZOf<vca_e16> { typedef vca_z16 type; };
+
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 struct MatArgs {
@@ -170,7 +181,8 @@ __device__ __forceinline__ void finish(const MatArgs& g, int m, int n, float (&v
   const int left = g.N - n;
 #pragma unroll
   for (int r = 0; r < V; ++r) v[r] += (float)bias.e[r];
-  if (g.z) store_any<T, V>(reinterpret_cast<T*>(g.z) + (size_t)m * g.N + n, left, v);
+  typedef typename ZOf<T>::type Z;
+  if (g.z) store_any<Z, V>(reinterpret_cast<Z*>(g.z) + (size_t)m * g.N + n, left, v);
   act_all(v, g.act, g.slope);
   if (g.res) {
 #pragma unroll
@@ -855,7 +867,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_rows_kernel(const MatArgs 
 // ------------------------------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void act_bwd_kernel(int M, int N, int act, float slope, const T* __restrict__ gy,
-                                                      const T* __restrict__ z, T* __restrict__ dz,
+                                                      const typename ZOf<T>::type* __restrict__ z, T* __restrict__ dz,
                                                       float* __restrict__ part, int rows, T* __restrict__ db,
                                                       int db_add) {
   constexpr int V = 16 / (int)sizeof(T);
@@ -869,9 +881,10 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(int M, int N, int act, flo
   if (n + V <= N) {
     for (int r = r0 + ty; r < r1; r += 8) {
       const size_t o = (size_t)r * N + n;
-      Vec16<T> a, b, d;
+      Vec16<T> a, d;
+      AnyVec<typename ZOf<T>::type, V> b;
       a.u = reinterpret_cast<const Any16*>(gy + o)->u;
-      if (z) b.u = reinterpret_cast<const Any16*>(z + o)->u;
+      if (z) b = *reinterpret_cast<const AnyVec<typename ZOf<T>::type, V>*>(z + o);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float v = (float)a.e[e];
@@ -1063,6 +1076,8 @@ long long ws_floats_of(const vca_matmul_desc* d) {
   return n;
 }
 
+int z_type(int type) { return type == VCA_T_BF16 ? VCA_T_F16 : VCA_T_F32; }
+
 bool aligned(int type, std::initializer_list<const void*> ps) {
   uintptr_t bits = 0;
   for (const void* p : ps) bits |= reinterpret_cast<uintptr_t>(p);
@@ -1137,7 +1152,7 @@ extern "C" int vca_matmul_act(const vca_matmul_desc* d, const void* a, const voi
   VCA_CHECK_ARG(a && b && c);
   const int rc = plan_of(d, a, b, p);
   if (rc) return rc;
-  VCA_CHECK_ARG(aligned(d->type, {a, b, bias, res, c, z}));
+  VCA_CHECK_ARG(aligned(d->type, {a, b, bias, res, c}) && aligned(z_type(d->type), {z}));
   VCA_CHECK_ARG(ws_of(p) == 0 || (ws && ws_floats >= ws_of(p) && (reinterpret_cast<uintptr_t>(ws) & 15) == 0));
   const int e = launch_product(p, *d, a, b, bias, res, c, z, ws, (hipStream_t)stream);
   FoldArgs f;
@@ -1161,7 +1176,7 @@ static int act_bwd(int type, int M, int N, int act, float slope, const void* gy,
                        (float*)dz, ws, rows, (float*)db, db_add);
   else
     hipLaunchKernelGGL(act_bwd_kernel<vca_e16>, grid, dim3(256), 0, s, M, N, act, slope, (const vca_e16*)gy,
-                       (const vca_e16*)z, (vca_e16*)dz, ws, rows, (vca_e16*)db, db_add);
+                       (const vca_z16*)z, (vca_e16*)dz, ws, rows, (vca_e16*)db, db_add);
   if (db && slabs > 1) f.b = {ws, db, N, slabs, db_add};
   return vca_launch_status();
 }
@@ -1169,7 +1184,7 @@ static int act_bwd(int type, int M, int N, int act, float slope, const void* gy,
 static bool act_bwd_ok(int type, int M, int N, int act, const void* gy, const void* z, const void* dz, const void* db) {
   const int own16 = VCA_ELEM_TYPE ? VCA_T_F16 : VCA_T_BF16;
   return (type == VCA_T_F32 || type == own16) && M > 0 && N > 0 && act_ok(act) && gy && (act == VCA_ACT_NONE) == !z &&
-         (!dz || z) && aligned(type, {gy, z, dz, db});
+         (!dz || z) && aligned(type, {gy, dz, db}) && aligned(z_type(type), {z});
 }
 
 extern "C" int vca_act_bwd(int type, int M, int N, int act, float slope, const void* gy, const void* z, void* dz, void* db,

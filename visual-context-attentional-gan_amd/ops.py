@@ -836,6 +836,8 @@ def _rows_2d(t, broadcast=False):
 
 
 _ELEM_OF = {torch.float32: None, torch.bfloat16: 'bf16', torch.float16: 'fp16'}   # 16-bit products are compiled per type
+# what the value under the activation is kept in: rounded less than dz, next to whose rounding its own comes
+_KEPT_IN = {torch.float32: torch.float32, torch.bfloat16: torch.float16, torch.float16: torch.float32}
 _act_ws = {}     # sizes and types of a forward or backward pass -> workspace floats
 
 
@@ -843,21 +845,24 @@ def _row_step(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]               # a single row's stride may be anything
 
 
+def _at(t):
+    return 0 if t is None else t.data_ptr()
+
+
 def _linear_act_fwd(x, w, bias, res, code, z=None):
-    (M, K), N, dt = x.shape, w.shape[0], x.dtype
-    y = torch.empty((M, N), device=x.device, dtype=dt)
+    (M, K), N, dt, dev = x.shape, w.shape[0], x.dtype, x.device
+    y = torch.empty((M, N), device=dev, dtype=dt)
     L = _lib.lib(_ELEM_OF[dt])
     ns = _nsplit() if dt == torch.float32 else 1
-    d = _lib.MatmulDesc(M, N, K, _lib.TYPES[dt], ns, 0, 0, code[0], code[1], _row_step(x), _row_step(w), N,
-                        0 if res is None else _row_step(res))
+    d = _lib.pack_matmul(M, N, K, _lib.TYPES[dt], ns, 0, 0, code[0], code[1], _row_step(x), _row_step(w), N,
+                         0 if res is None else _row_step(res))
     key = (M, N, K, dt, ns)
     n = _act_ws.get(key)
     if n is None:
         n = _act_ws[key] = int(L.vca_matmul_act_ws_floats(d))
-    ws = torch.empty(n, device=x.device, dtype=torch.float32) if n else None
-    check(L.vca_matmul_act(d, x.data_ptr(), w.data_ptr(), None if bias is None else bias.data_ptr(),
-                           None if res is None else res.data_ptr(), y.data_ptr(), None if z is None else z.data_ptr(),
-                           None if ws is None else ws.data_ptr(), n, stream()), 'matmul_act')
+    ws = torch.empty(n, device=dev, dtype=torch.float32) if n else None
+    check(L.vca_matmul_act(d, x.data_ptr(), w.data_ptr(), _at(bias), _at(res), y.data_ptr(), _at(z), _at(ws), n, stream()),
+          'matmul_act')
     return y
 
 
@@ -866,15 +871,20 @@ class LinearActFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, bias, res, code):
+        need = ctx.needs_input_grad
         z = None
-        if code[0] != ACT_NONE and any(ctx.needs_input_grad[:3]):
-            z = torch.empty((x.shape[0], w.shape[0]), device=x.device, dtype=x.dtype)
+        if code[0] != ACT_NONE and (need[0] or need[1] or need[2]):
+            z = torch.empty((x.shape[0], w.shape[0]), device=x.device, dtype=_KEPT_IN[x.dtype])
         ctx.save_for_backward(x, w, z)
         ctx.code, ctx.bias_param = code, bias
         return _linear_act_fwd(x, w, bias, res, code, z)
 
     @staticmethod
     def backward(ctx, gy):
+        dev = gy.device
+        if dev.index != torch._C._cuda_getDevice():
+            with torch.cuda.device(dev):
+                return LinearActFn.backward(ctx, gy)
         # (the decorator only matters under create_graph, where it makes a second differentiation an error)
         return _linear_act_bwd_once(ctx, gy) if torch.is_grad_enabled() else _linear_act_bwd(ctx, gy)
 
@@ -890,22 +900,22 @@ def _linear_act_bwd(ctx, gy):
     g = gy.contiguous()
     wsink = _grad_sink(w) if need_w else None
     bsink = _grad_sink(ctx.bias_param) if need_b else None
-    with _on_device(dev):
-        dz = torch.empty((M, N), device=dev, dtype=dt) if z is not None and (need_x or need_w) else None
-        gx = torch.empty((M, K), device=dev, dtype=dt) if need_x else None
-        gw = (torch.empty((N, K), device=dev, dtype=dt) if wsink is None else wsink) if need_w else None
-        gb = (torch.empty(N, device=dev, dtype=dt) if bsink is None else bsink) if need_b else None
-        L = _lib.lib(_ELEM_OF[dt])
-        ns = _nsplit(True) if dt == torch.float32 else 1
-        d = _lib.LinearBwd(M, N, K, _lib.TYPES[dt], ns, ctx.code[0], wsink is not None, bsink is not None, ctx.code[1],
-                           _row_step(x), _row_step(w), g.data_ptr(), x.data_ptr(), w.data_ptr(), _addr(z), _addr(dz),
-                           _addr(gx), _addr(gw), _addr(gb))
-        key = (M, N, K, dt, ns, 'bwd')
-        n = _act_ws.get(key)
-        if n is None:
-            n = _act_ws[key] = int(L.vca_linear_act_bwd_ws_floats(d))
-        ws = torch.empty(n, device=dev, dtype=torch.float32)
-        check(L.vca_linear_act_bwd(d, ws.data_ptr(), n, stream()), 'linear_act_bwd')
+    L = _lib.lib(_ELEM_OF[dt])
+    ns = _nsplit(True) if dt == torch.float32 else 1
+    code = ctx.code
+    dz = torch.empty((M, N), device=dev, dtype=dt) if z is not None and (need_x or need_w) else None
+    gx = torch.empty((M, K), device=dev, dtype=dt) if need_x else None
+    gw = (torch.empty((N, K), device=dev, dtype=dt) if wsink is None else wsink) if need_w else None
+    gb = (torch.empty(N, device=dev, dtype=dt) if bsink is None else bsink) if need_b else None
+    d = _lib.pack_linear_bwd(M, N, K, _lib.TYPES[dt], ns, code[0], wsink is not None, bsink is not None, code[1],
+                             _row_step(x), _row_step(w), g.data_ptr(), x.data_ptr(), w.data_ptr(), _at(z), _at(dz),
+                             _at(gx), _at(gw), _at(gb))
+    key = (M, N, K, dt, ns, 'bwd')
+    n = _act_ws.get(key)
+    if n is None:
+        n = _act_ws[key] = int(L.vca_linear_act_bwd_ws_floats(d))
+    ws = torch.empty(n, device=dev, dtype=torch.float32)
+    check(L.vca_linear_act_bwd(d, ws.data_ptr(), n, stream()), 'linear_act_bwd')
     return gx, gw if wsink is None else None, gb if bsink is None else None, gy if need_r else None, None
 
 
@@ -922,8 +932,8 @@ def linear_act(x, w, bias=None, act=None, residual=None):
 
     fp32 tensors are multiplied as set_precision() says ('fp32': exact; the split and single-product modes like every
     other product, 'mixed' with single products in the gradients); 16-bit tensors take one product of their own type in
-    every mode.  Sums, bias, activation and residual are fp32, and the result is rounded once; for the gradients the
-    value under the activation and dz = gy act' are rounded to the tensors' type.  Inside direct_param_grad() the
+    every mode.  Sums, bias, activation and residual are fp32, and the result is rounded once; for the gradients dz =
+    gy act' is rounded to the tensors' type (the value under the activation is kept in more bits than that).  Inside direct_param_grad() the
     gradients of leaf parameters are added straight into their .grad; input_grads_only() leaves them out."""
     code = _linear_act_code(act)
     dt, dev, xs, ws = x.dtype, x.device, x.shape, w.shape
@@ -947,14 +957,16 @@ def linear_act(x, w, bias=None, act=None, residual=None):
         for t in tensors:
             y = y + t.sum() * 0
         return y
+    if dev.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return linear_act(x, w, bias, act, residual)
     x2, w2 = _rows_2d(x), _rows_2d(w)
     b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     r = None if residual is None else _rows_2d(residual, True)
-    with _on_device(dev):
-        if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-            y = LinearActFn.apply(x2, w2, b, r, code)
-        else:
-            y = _linear_act_fwd(x2, w2, b, r, code)
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
+        y = LinearActFn.apply(x2, w2, b, r, code)
+    else:
+        y = _linear_act_fwd(x2, w2, b, r, code)
     return y if len(shape) == 2 else y.view(shape)
 
 
@@ -2320,12 +2332,19 @@ class GradNorm:
         self._ws = int(_lib.lib().vca_grad_norm_ws_doubles(n, self._ptrs, self._numel, self._types))
         self._disjoint = None
 
+    def _scale(self, scaler):
+        if scaler is None:
+            return None
+        if scaler.scale.device != self.device:
+            raise ValueError('GradNorm: gradients on %s and a loss scale on %s' % (self.device, scaler.scale.device))
+        return ptr(scaler.scale)
+
     def norm(self, scaler=None):
         """sqrt(sum of squares of all elements) (divided by the loss scale)."""
         with _on_device(self.device):
             out, ws = self._buffers()
             check(_lib.lib().vca_grad_norm(self._n, self._ptrs, self._numel, self._types,
-                                           None if scaler is None else ptr(scaler.scale), _addr(ws), self._ws,
+                                           self._scale(scaler), _at(ws), self._ws,
                                            out.data_ptr(), stream()), 'grad_norm')
         return out
 
@@ -2340,7 +2359,7 @@ class GradNorm:
         with _on_device(self.device):
             out, ws = self._buffers()
             check(_lib.lib().vca_grad_clip(self._n, self._ptrs, self._numel, self._types, max_norm,
-                                           None if scaler is None else ptr(scaler.scale), _addr(ws), self._ws,
+                                           self._scale(scaler), _at(ws), self._ws,
                                            out.data_ptr(), stream()), 'grad_clip')
         torch.autograd.graph.increment_version(self.tensors)
         return out
@@ -2358,10 +2377,6 @@ def grad_norm(tensors, scaler=None):
 def clip_grad_norm_(tensors, max_norm, scaler=None):
     """Clip a list of gradient tensors in place by their global 2-norm and return it; see GradNorm."""
     return GradNorm(tensors).clip_(max_norm, scaler)
-
-
-def _addr(t):
-    return None if t is None else t.data_ptr()
 
 
 def _max_norm(v):
@@ -2387,7 +2402,7 @@ class _on_device:
     """Make `device` current for the enclosed launches (which go to its current stream); free where it is already."""
 
     def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        self.guard = None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
     def __enter__(self):
         if self.guard is not None:
