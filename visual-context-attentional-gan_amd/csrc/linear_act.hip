@@ -164,14 +164,19 @@ __device__ __forceinline__ void store_any(T* p, int left, const float (&v)[V]) {
   }
 }
 
+// (a missing bias or residual takes no part in this: the branch is the same for the whole launch)
 template <typename T, int V>
 __device__ __forceinline__ AnyVec<T, V> bias_of(const MatArgs& g, int n) {
-  return load_any<T, V>(reinterpret_cast<const T*>(g.bias) + n, g.bias ? g.N - n : 0);
+  AnyVec<T, V> q = {};
+  if (g.bias) q = load_any<T, V>(reinterpret_cast<const T*>(g.bias) + n, g.N - n);
+  return q;
 }
 
 template <typename T, int V>
 __device__ __forceinline__ AnyVec<T, V> res_of(const MatArgs& g, int m, int n) {
-  return load_any<T, V>(reinterpret_cast<const T*>(g.res) + (size_t)m * g.ldr + n, g.res ? g.N - n : 0);
+  AnyVec<T, V> q = {};
+  if (g.res) q = load_any<T, V>(reinterpret_cast<const T*>(g.res) + (size_t)m * g.ldr + n, g.N - n);
+  return q;
 }
 
 // Bias, activation and residual of V neighbouring columns n .. n + V - 1 of row m; stores y and, if kept, z.
@@ -179,8 +184,10 @@ template <typename T, int V>
 __device__ __forceinline__ void finish(const MatArgs& g, int m, int n, float (&v)[V], const AnyVec<T, V>& bias,
                                        const AnyVec<T, V>& res) {
   const int left = g.N - n;
+  if (g.bias) {
 #pragma unroll
-  for (int r = 0; r < V; ++r) v[r] += (float)bias.e[r];
+    for (int r = 0; r < V; ++r) v[r] += (float)bias.e[r];
+  }
   typedef typename ZOf<T>::type Z;
   if (g.z) store_any<Z, V>(reinterpret_cast<Z*>(g.z) + (size_t)m * g.N + n, left, v);
   act_all(v, g.act, g.slope);
