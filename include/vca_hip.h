@@ -540,17 +540,11 @@ long long vca_matmul_act_ws_floats(const vca_matmul_desc* d);
 int vca_matmul_act(const vca_matmul_desc* d, const void* a, const void* b, const void* bias, const void* res, void* c,
                    void* z, float* ws, long long ws_floats, void* stream);
 
-/* dz = gy act'(z) and db[n] (+)= sum_m dz[m][n] (of the unrounded dz) in one pass over dense [M][N] matrices.  Without an
- * activation (act 0, z and dz NULL) only db is formed, from gy.  db may be NULL; db_add: add to it.
- * ws: vca_act_bwd_ws_floats floats, needed with db. */
-long long vca_act_bwd_ws_floats(int type, int M, int N);
-int vca_act_bwd(int type, int M, int N, int act, float slope, const void* gy, const void* z, void* dz, void* db,
-                int db_add, float* ws, long long ws_floats, void* stream);
-
-/* The backward pass of y = act(x W^T + bias) + res in one call: dz and db as vca_act_bwd (with act 0, z and dz are NULL
- * and dz is gy), then dx = dz W and dw = dz^T x as vca_matmul_act.  gy, z, dz [M][N], dx [M][K], dw [N][K] dense, x and w
- * with row strides ldx and ldw.  dx, dw, db may be NULL; dw_add / db_add: add to what is there.  ws: at least
- * vca_linear_act_bwd_ws_floats(b) floats (its pointers are not looked at by the query), used by the launches in turn. */
+/* The backward pass of y = act(x W^T + bias) + res in one call: dz = gy act'(z) and db[n] (+)= sum_m dz[m][n] (of the
+ * unrounded dz) in one pass over gy and z (with act 0, z and dz are NULL and dz is gy), then dx = dz W and dw = dz^T x as
+ * vca_matmul_act.  gy, z, dz [M][N], dx [M][K], dw [N][K] dense, x and w with row strides ldx and ldw.  dx, dw, db may be
+ * NULL; dw_add / db_add: add to what is there.  ws: at least vca_linear_act_bwd_ws_floats(b) floats (its pointers are not
+ * looked at by the query), a part for each of db, dx and dw. */
 typedef struct {
   int M, N, K, type, nsplit, act, dw_add, db_add;
   float slope;

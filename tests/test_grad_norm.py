@@ -124,6 +124,18 @@ def test_dense_layouts_and_an_integer_number_of_bits():
 
 
 @gpu
+def test_the_memory_of_a_list_stays_when_a_tensor_gets_other_data():
+    from vcagan_amd import ops
+    t = torch.full((100000,), 2.0, device='cuda')
+    n = ops.GradNorm([t])
+    t.data = torch.zeros(100000, device='cuda')
+    fill = [torch.full((100000,), 9.0, device='cuda') for _ in range(8)]
+    assert float(n.norm()) == float(torch.tensor(400000.0).double().sqrt().float())
+    n.clip_(1.0)
+    assert bool((t == 0).all()) and all(bool((f == 9).all()) for f in fill)
+
+
+@gpu
 def test_elements_beyond_32_bits():
     from vcagan_amd import ops
     n = 2 ** 31 + 12345

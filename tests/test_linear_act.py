@@ -1,4 +1,4 @@
-"""ops.linear_act (vca_matmul_act / vca_act_bwd: a linear layer with bias, activation and residual in the product's
+"""ops.linear_act (vca_matmul_act / vca_linear_act_bwd: a linear layer with bias, activation and residual in the product's
 epilogue, forward and gradients) against 64-bit arithmetic, element by element.
 
 Tolerances (u = 2^-24, e = half an ulp of the tensors' type, finfo.eps / 2; |.| of matrices element by element):
@@ -125,10 +125,12 @@ def _run(M, K, N, dtype, act, seed, mode='fp32', bias=True, res=True):
 
 
 # rows, reduction, columns: single ones, below and just over every tile and chunk, odd and even, few rows with long
-# reductions (split over workgroups), the serving kernel's 16-row edge, the 256-wide tiles with and without a tail
+# reductions (split over workgroups), the serving kernel's 16-row edge and wide weights beyond it, the 32-row tiles, 64-row
+# tiles with four stages
 SHAPES = [(1, 1, 1), (1, 8, 16), (2, 3, 5), (1, 512, 512), (7, 129, 33), (15, 1000, 18), (16, 2048, 40), (17, 2048, 40),
           (64, 64, 64), (127, 32, 129), (128, 64, 128), (129, 65, 127), (200, 1111, 77), (333, 96, 513), (40, 5000, 12),
-          (600, 256, 1280), (3, 20000, 70), (16, 9001, 33)]
+          (600, 256, 1280), (3, 20000, 70), (16, 9001, 33), (24, 4096, 300), (32, 512, 1280), (31, 1000, 70), (20, 8256, 72),
+          (17, 40, 2000), (100, 640, 1300), (128, 72, 136), (9, 8192, 8200)]
 
 
 @gpu
@@ -254,6 +256,22 @@ def test_slopes_far_out():
         hi = 0.0 if act == 'tanh' else 1.0
         assert bool((gz[:4].abs() < 1e-24).all()) and torch.equal(gz[4:], torch.full_like(gz[4:], hi)), (act, gz)
         assert bool(y.isfinite().all())
+
+
+@gpu
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+def test_activations_of_infinity(dtype):
+    """+infinity under a smooth activation stays infinity with slope one (tanh: 1 and 0), never infinity x 0."""
+    from vcagan_amd import ops
+    t = TYPES[dtype]
+    x = torch.tensor([[math.inf], [1.0], [math.nan]], dtype=t).cuda().requires_grad_(True)
+    one = torch.ones(1, 1, dtype=t).cuda()
+    for act in ACTS:
+        y = ops.linear_act(x, one, act=act)
+        gx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        top, slope = (1.0, 0.0) if act == 'tanh' else (math.inf, 1.0)
+        assert float(y[0]) == top and float(gx[0]) == slope and bool(y[1].isfinite().all()), (act, y, gx)
+        assert bool(y[2].isnan().all()), (act, y)
 
 
 @gpu
@@ -469,12 +487,6 @@ def test_entry_points_refuse_before_any_launch():
         n = L.vca_matmul_act_ws_floats(ctypes.byref(_lib.MatmulDesc(**dict(ok, **long))))
         assert n > 0 and n % (64 * 64) == 0
         assert call(ws=None, **long) == -22 and call(n=n - 1, **long) == -22 and call(ws=68, **long) == -22
-        f = lambda type=0, M=4, N=4, act=6, gy=64, z=64, dz=64, db=64, ws=64, n=1 << 20: L.vca_act_bwd(
-            type, M, N, act, 0.0, gy, z, dz, db, 0, ws, n, None)
-        for kw in (dict(type=other), dict(M=0), dict(N=0), dict(act=2), dict(act=9), dict(gy=None), dict(z=None),
-                   dict(dz=None, db=None), dict(ws=None), dict(n=3), dict(act=0), dict(act=0, z=None), dict(z=66)):
-            assert f(**kw) == -22, kw
-        assert L.vca_act_bwd_ws_floats(0, 0, 4) == 0
         bwd = dict(M=64, N=64, K=64, type=0, nsplit=0, act=6, dw_add=0, db_add=0, slope=0.0, ldx=64, ldw=64, gy=64, x=64,
                    w=64, z=64, dz=64, dx=64, dw=64, db=64)
         n = L.vca_linear_act_bwd_ws_floats(ctypes.byref(_lib.LinearBwd(**bwd)))
@@ -482,5 +494,8 @@ def test_entry_points_refuse_before_any_launch():
         g = lambda ws=64, n=n, **kw: L.vca_linear_act_bwd(ctypes.byref(_lib.LinearBwd(**dict(bwd, **kw))), ws, n, None)
         for kw in (dict(gy=None), dict(M=0), dict(K=0), dict(act=0), dict(act=2), dict(z=None), dict(dz=None),
                    dict(type=other, nsplit=1), dict(nsplit=2), dict(w=None), dict(x=None), dict(ldx=63), dict(ldw=63),
-                   dict(n=n - 1), dict(ws=None), dict(ws=72)):
+                   dict(n=n - 1), dict(ws=None), dict(ws=72), dict(N=0), dict(act=9), dict(z=66),
+                   dict(type=other, nsplit=1, dx=None, dw=None), dict(act=0, z=None), dict(act=0, dz=None),
+                   dict(n=3, dx=None, dw=None), dict(ws=None, n=0, dx=None, dw=None)):
             assert g(**kw) == -22, kw
+        assert L.vca_linear_act_bwd_ws_floats(ctypes.byref(_lib.LinearBwd(**dict(bwd, M=0)))) == 0

@@ -205,8 +205,6 @@ _SIGS = {
     'vca_loss_scale_update': ([_P, _P, _F, _F, _I, _P], _I),
     'vca_matmul_act_ws_floats': ([_P], _LL),
     'vca_matmul_act': ([_P] * 8 + [_LL, _P], _I),
-    'vca_act_bwd_ws_floats': ([_I, _I, _I], _LL),
-    'vca_act_bwd': ([_I, _I, _I, _I, _F, _P, _P, _P, _P, _I, _P, _LL, _P], _I),
     'vca_linear_act_bwd_ws_floats': ([_P], _LL),
     'vca_linear_act_bwd': ([_P, _P, _LL, _P], _I),
     'vca_grad_norm_ws_doubles': ([_I, _P, _P, _P], _LL),

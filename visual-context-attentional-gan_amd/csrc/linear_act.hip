@@ -1,7 +1,7 @@
 // Linear layers with bias, activation and residual in the product's epilogue, forward and gradients, on fp32 and 16-bit
 // tensors of any size, row stride and alignment:
 //
-//   z = x W^T + b     y = act(z) + r          (one pass over the product: z is rounded and kept for the backward pass)
+//   z = x W^T + b     y = act(z) + r          (one pass over the product; training keeps z, see ZOf)
 //   dz = gy act'(z)   db = sum_m dz           (one pass over gy and z)
 //   dx = dz W         dW = dz^T x             (products with one or both operands read along their columns)
 //
@@ -84,7 +84,7 @@ __device__ __forceinline__ float act_f(float z, int act, float slope) {
     case VCA_ACT_GELU: {                                     // z Phi(z); the small tail is multiplied, never subtracted
       float e;
       const float q = 0.5f * erfc_half(z, e);
-      return z > 0.f ? z - z * q : z * q;
+      return z * (z > 0.f ? 1.f - q : q);
     }
     case VCA_ACT_GELU_TANH: return z * sigmoid_f(2.f * GELU_C * (z + GELU_A * z * z * z));   // (1 + tanh u) / 2
     case VCA_ACT_SILU: return z * sigmoid_f(z);
@@ -200,9 +200,14 @@ __device__ __forceinline__ void finish(const MatArgs& g, int m, int n, float (&v
 
 // ------------------------------------------------------------------------------------------------
 // The tiled product.  A workgroup owns a BM x BN tile of C and walks the reduction in chunks of 128 bytes of a row
-// (64 16-bit or 32 fp32 elements) through two LDS stages: chunk c + 1 travels while chunk c feeds the matrix cores, one
-// barrier a chunk.  DMA: whole chunks go straight from memory to LDS (16-byte pieces, operands 16-byte aligned); the
-// reduction's last, partial chunk, and every chunk of operands of another alignment, go through registers with masks.
+// (64 16-bit or 32 fp32 elements) through two LDS stages (four where memory has to be waited for, see launch_layout):
+// chunk c + 1 travels while chunk c feeds the matrix cores, one barrier a chunk.  DMA: whole chunks go straight from memory
+// to LDS (16-byte pieces, operands 16-byte aligned); the reduction's last, partial chunk, and every chunk of operands of
+// another alignment, go through registers with masks.
+//
+// fp32 is bound by the matrix cores: 8192^3 at 139 TFLOP/s of the library's 154 (128-wide tiles); 2400 x 2560 -> 512, whose
+// 228 workgroups leave a tenth of the CUs idle, 68 us = 92 TFLOP/s.  16 bits with these tiles are bound by LDS and by the
+// wait for a chunk: 2048^3 29 us = 590 TFLOP/s.
 //
 // LDS images of an operand with R rows in the tile:
 //   k contiguous      [R][128 B], 16-byte pieces of a row XOR-ed with row & 7: the 16 rows a fragment load touches
@@ -436,7 +441,7 @@ __device__ __forceinline__ void store_tile(const MatArgs& g, const f32x4 (&acc)[
   }
 }
 
-template <int MODE, bool AKC, bool BKC, int BM, int BN, int NWM, int NWN, bool DMA>
+template <int MODE, bool AKC, bool BKC, int BM, int BN, int NWM, int NWN, bool DMA, int STAGES>
 __global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef typename ElemOf<MODE>::T T;
@@ -517,17 +522,28 @@ __global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g)
   if (c0 < whole) {
     A.start(c0);
     B.start(c0);
-    A.dma(smem);
-    B.dma(smem + BM * 128);
-    for (int c = c0; c < whole; ++c) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // chunk c has landed, in every wave behind the barrier
-      __syncthreads();
-      char* next = smem + ((c - c0 + 1) & 1) * STAGE;     // every wave has left this stage: it is behind chunk c - 1
-      if (c + 1 < whole) {
-        A.dma(next);
-        B.dma(next + BM * 128);
-      }
-      compute(smem + ((c - c0) & 1) * STAGE);
+    int at = 0, to = 0;                                   // stages of chunk c and of the next chunk to send
+    auto turn = [](int s) { return s + 1 == STAGES ? 0 : s + 1; };
+    auto send = [&]() {
+      A.dma(smem + to * STAGE);
+      B.dma(smem + to * STAGE + BM * 128);
+      to = turn(to);
+    };
+    for (int c = c0; c < min(whole, c0 + STAGES - 1); ++c) send();
+    // Chunk c has landed (in every wave behind the barrier) when at most the STAGES - 2 later chunks' pieces are under
+    // way; every wave has left the stage that is sent to next, chunk c - 1's, with its reads done.
+    int c = c0;
+    for (; c + STAGES - 1 < whole; ++c) {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * (A.PIECES + B.PIECES)) : "memory");
+      send();
+      compute(smem + at * STAGE);
+      at = turn(at);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the rest is all under way
+    __syncthreads();
+    for (; c < whole; ++c) {
+      compute(smem + at * STAGE);
+      at = turn(at);
     }
   }
   if (whole < c1) {                                       // not by DMA: chunk c + 1 waits in registers under chunk c
@@ -552,13 +568,18 @@ __global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g)
 }
 
 // ------------------------------------------------------------------------------------------------
-// The tiled product for large 16-bit ones: 256 x 256 tiles, four waves of 128 x 128 each.  LDS carries 2 x 64 KB stages
-// and feeds each wave 2 x 16 KB of fragments a chunk: half of what eight waves of 128 x 64 would read, and three
-// quarters of the time the matrix cores need for the chunk.  One wave a SIMD has nobody to hide behind, so the wave
-// overlaps by itself: while the 64 MFMAs of one half chunk run, the 16 fragments of the next half are read (the second
-// half of chunk c, then the first of chunk c + 1), an LDS read between every few MFMAs.  The chunk's only barrier sits
-// in its middle: there every wave has its last fragments of chunk c in registers, chunk c + 1 has landed (it was sent a
-// whole chunk earlier), and chunk c's stage is free to be refilled with chunk c + 2.
+// The tiled product for large 16-bit ones: 256 x 256 tiles, eight waves of 128 x 64 each, two to a SIMD, one workgroup to
+// a CU.  LDS carries 2 x 64 KB stages and feeds the waves 192 KB of fragments a chunk, under the time the matrix cores need
+// for it.  The waves overlap by themselves: while the 32 MFMAs of one half chunk run, the 12 fragments of the next half are
+// read (the second half of chunk c, then the first of chunk c + 1) and, in the second half, a piece of chunk c + 2 is sent
+// behind each row of MFMAs.  The chunk's only barrier sits in its middle: there every wave has its last fragments of chunk
+// c in registers, chunk c + 1 has landed (it was sent a whole chunk earlier), and chunk c's stage is free to be refilled.
+//
+// Bound by the matrix cores: 8192^3 in bf16 at 1390 (x W^T), 1447 (dx) and 1465 TFLOP/s (dW), where the library's
+// product reaches 1485; with few chunks a tile the pipeline's ends show, 8192 x 4096 x 4096: 1270, 1300, 1408.  Tried and
+// slower: four waves of 128 x 128 (fewer fragment reads, but accumulators that do not fit the registers next to the
+// fragments: 459 us against 339), touching the next chunk's lines in L2, the barrier shifted by a quarter chunk, chunks
+// visited in an order that differs between tiles.
 // ------------------------------------------------------------------------------------------------
 template <bool KC>
 struct WideOperand {
@@ -784,8 +805,9 @@ __global__ __launch_bounds__(256) void fold_kernel(const FoldArgs f) {
 // A wave takes two neighbouring chunks of 64 bytes at a time, so the line of each of its 16 rows is asked for by one wave
 // in a row (31 us against 35 with single chunks dealt out to the waves, 4096 -> 16384 in bf16, 8 rows), and the next two
 // fly under this pair's products.  More in flight (four chunks: 32 us), 32 columns a workgroup (34) or four waves (33)
-// were longer.  Bound by memory: 5.1 TB/s with one row, 4.4 with eight, whose x fragments pass through L2 as well.  The
-// waves' partial tiles meet in LDS.  Rows of x beyond M repeat the last one.
+// were longer.  Bound by memory: 5.3 TB/s with one row, 4.9 with four (4096 -> 16384), whose x fragments pass through L2 as
+// well: with more rows the tiles above take over (FEW_BYTES).  The waves' partial tiles meet in LDS.  Rows of x beyond M
+// repeat the last one.
 // ------------------------------------------------------------------------------------------------
 constexpr int FEW_WAVES = 8, FEW_PAIR = 2, FEW_GROUP = FEW_WAVES * FEW_PAIR;
 
@@ -870,7 +892,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_rows_kernel(const MatArgs 
 
 // ------------------------------------------------------------------------------------------------
 // dz = gy act'(z) and the columns' sums of it.  A workgroup takes a strip of 32 x 16 bytes of columns and a range of
-// rows (8 at a time); its column sums (of the unrounded dz, fp32) go to a slab, slabs are added in order.
+// rows (8 at a time); its column sums (of the unrounded dz, fp32) go to a slab, slabs are added in order.  Bound by memory:
+// 8192 x 4096 bf16, gelu: 39 us, 5.1 TB/s.
 // ------------------------------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void act_bwd_kernel(int M, int N, int act, float slope, const T* __restrict__ gy,
@@ -941,9 +964,15 @@ int mode_of(const vca_matmul_desc& d) {
 
 struct Plan {
   MatArgs g;
-  int mode, tile;                     // 64, 128 or 256; 0: few rows
-  bool dma, wide;
+  int mode, tile;                     // 32 (x 64), 64, 128 or 256; 0: few rows
+  bool dma, wide, low;                // low, wide: the 32 and 256 tiles may be taken
 };
+
+// Rows of x times bytes of W up to which few_rows_kernel takes a product of at most 16 rows: every workgroup of 16 columns
+// reads x again, a tile of 64 columns a quarter of that.  us, few_rows_kernel and tiles: bf16 4096 -> 16384, 1 row 25 / 30,
+// 4 rows 27.6 / 29.6, 8 rows 31 / 29.7, 16 rows 39 / 30; 4096 -> 4096, 16 rows 11.6 / 12.9; fp32 4096 -> 4096, 16 rows
+// 25 / 21; 512 -> 512, 16 rows 4.2 / 6.6.
+constexpr double FEW_BYTES = 600e6;
 
 // Tile and split of a product, by the time the candidates would take.  A tile's chunk costs a CU `work` us of its matrix
 // cores; a workgroup that has a CU to itself cannot go below `wait` us a chunk (LDS and memory latency, one barrier a
@@ -951,21 +980,23 @@ struct Plan {
 // adds one launch and a pass over the partial products.  Fitted to launches of 2 to 2000 us on this part; the choice is
 // within 10 % of the best one measured at each.  Where sides change (us): fp32 4800 x 1280, K 512: 64-wide tiles 62, 128
 // 74; 8192 x 4096, K 4096: 2349 against 2043.  16 bits 2048^3: 64 29, 128 30, 256 39 (split); 4800 x 2560, K 5120:
-// 197, 137, 112; 64 x 4096, K 4096: 64-wide unsplit 31, split four ways 15.
+// 197, 137, 112; 64 x 4096, K 4096: 64-wide unsplit 31, split four ways 15.  Up to 32 rows tiles of 32 x 64 (whose work is
+// the memory's, not the matrix cores'), against 64 x 64: 32 x 4096 -> 4096 13.4 / 14.5, fp32 21.6 / 25.8.
 struct TileCost { int tile; double work, wait, ends; };
-constexpr TileCost COST[4][3] = {
-    {{256, 1.55, 1.55, 8.}, {128, 0.53, 0.85, 2.}, {64, 0.20, 0.45, 0.8}},     // 16-bit tensors
-    {{0, 0., 0., 0.}, {128, 1.95, 2.15, 2.5}, {64, 0.56, 0.62, 1.}},           // fp32, exact
-    {{0, 0., 0., 0.}, {128, 0.92, 1.15, 2.5}, {64, 0.36, 0.55, 1.}},           // fp32, three products
-    {{0, 0., 0., 0.}, {128, 0.46, 0.85, 2.5}, {64, 0.22, 0.45, 1.}}};          // fp32, one product
+constexpr TileCost COST[4][4] = {
+    {{256, 1.55, 1.55, 8.}, {128, 0.53, 0.85, 2.}, {64, 0.20, 0.45, 0.8}, {32, 0.42, 0.24, 2.}},     // 16-bit tensors
+    {{0, 0., 0., 0.}, {128, 1.95, 2.15, 2.5}, {64, 0.56, 0.62, 1.}, {32, 0.42, 0.44, 2.}},           // fp32, exact
+    {{0, 0., 0., 0.}, {128, 0.92, 1.15, 2.5}, {64, 0.36, 0.55, 1.}, {32, 0.42, 0.40, 2.}},           // fp32, three products
+    {{0, 0., 0., 0.}, {128, 0.46, 0.85, 2.5}, {64, 0.22, 0.45, 1.}, {32, 0.42, 0.35, 2.}}};          // fp32, one product
 
 bool pick(Plan& p, int nc) {
   MatArgs& g = p.g;
   double best = 0.;
   p.tile = 0;
   for (const TileCost& t : COST[p.mode]) {
-    if (!t.tile || (t.tile == 256 && !p.wide)) continue;
-    const long long tiles = ((g.M + (long long)t.tile - 1) / t.tile) * ((g.N + (long long)t.tile - 1) / t.tile);
+    if (!t.tile || (t.tile == 256 && !p.wide) || (t.tile == 32 && !p.low)) continue;
+    const long long cols = t.tile == 32 ? 64 : t.tile;
+    const long long tiles = ((g.M + (long long)t.tile - 1) / t.tile) * ((g.N + cols - 1) / cols);
     if (tiles >= (1 << 24)) continue;
     for (int ks = 1; ks <= 32 && ks <= nc; ++ks) {
       const int chunks = (nc + ks - 1) / ks;
@@ -982,7 +1013,7 @@ bool pick(Plan& p, int nc) {
   if (!p.tile) return false;
   g.ksplit = (nc + g.cpz - 1) / g.cpz;
   g.ntm = (g.M + p.tile - 1) / p.tile;
-  g.ntn = (g.N + p.tile - 1) / p.tile;
+  g.ntn = p.tile == 32 ? (g.N + 63) / 64 : (g.N + p.tile - 1) / p.tile;
   return true;
 }
 
@@ -1014,16 +1045,19 @@ int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p) {
                          (uintptr_t)(d.lda * esz) | (uintptr_t)(d.ldb * esz);
   const int per16 = 16 / esz;
   p.dma = (bits & 15) == 0 && (!d.a_col || d.M % per16 == 0) && (!d.b_col || d.N % per16 == 0);
-  if (d.M <= 16 && !d.a_col && !d.b_col && (p.mode == MODE_16 || p.mode == MODE_F32)) {
-    // A workgroup streams its 16 rows of W at some 30 GB/s; where columns alone give too few of them to load the memory,
-    // the reduction is split too, if that saves more than the launch that adds the parts (16384 -> 1024 in bf16, one row:
-    // 20 us unsplit).
+  const double wbytes = (double)d.N * d.K * esz;
+  if (d.M <= 16 && d.N <= (1 << 26) && !d.a_col && !d.b_col && (p.mode == MODE_16 || p.mode == MODE_F32) &&
+      d.M * wbytes <= FEW_BYTES) {
+    // A workgroup streams its 16 rows of W at some 30 GB/s, all of them at most at 5 TB/s; where columns alone give too few
+    // of them to load the memory, the reduction is split too, if that saves more than the launch that adds the parts (one
+    // row, split and unsplit: bf16 16384 -> 1024 12.9 / 21.7 us, fp32 2560 -> 512 7.2 / 9.6, fp32 4096^2 21.2 / 20.3).
     p.tile = 0;
     const int nc = (d.K * esz + 63) / 64, blocks = (d.N + 15) / 16;
     double best = 0.;
     for (int ks = 1; ks <= 16 && (ks == 1 || (blocks * ks <= 512 && nc / ks >= 2 * FEW_GROUP)); ++ks) {
       const int chunks = (nc + ks - 1) / ks;
-      const double us = chunks * 1024. / 30e3 + (ks > 1 ? 4. : 0.);
+      const double stream = chunks * 1024. / 30e3, memory = wbytes / 5e6;
+      const double us = (stream > memory ? stream : memory) + (ks > 1 ? 4. : 0.);
       if (ks == 1 || us < best) {
         best = us;
         g.cpz = chunks;
@@ -1033,18 +1067,17 @@ int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p) {
     return 0;
   }
   // the 256-wide kernel addresses its pieces by 32-bit offsets from the tile: 256 rows (64 of k) of at most 4 MB
+  p.low = p.dma && d.M <= 32 && !d.a_col && !d.b_col;
   p.wide = p.mode == MODE_16 && p.dma && d.lda <= (1 << 21) && d.ldb <= (1 << 21);
   return pick(p, g.cpz) ? 0 : -22;
 }
 
-template <int MODE, bool AKC, bool BKC, int BM>
-int launch_tile(const Plan& p, hipStream_t s) {
-  const size_t lds = 4 * (size_t)BM * 128;                 // at most 64 KB
-  const dim3 grid(p.g.ntm * p.g.ntn * p.g.ksplit);
-  if (p.dma)
-    hipLaunchKernelGGL((matmul_kernel<MODE, AKC, BKC, BM, BM, 2, 2, true>), grid, dim3(256), lds, s, p.g);
-  else
-    hipLaunchKernelGGL((matmul_kernel<MODE, AKC, BKC, BM, BM, 2, 2, false>), grid, dim3(256), lds, s, p.g);
+template <int MODE, bool AKC, bool BKC, int BM, int BN, int NWM, bool DMA, int STAGES>
+int launch_kernel(const Plan& p, hipStream_t s) {
+  constexpr int LDS = STAGES * (BM + BN) * 128;            // at most 64 KB
+  static_assert(LDS <= 64 * 1024, "");
+  hipLaunchKernelGGL((matmul_kernel<MODE, AKC, BKC, BM, BN, NWM, 4 / NWM, DMA, STAGES>),
+                     dim3(p.g.ntm * p.g.ntn * p.g.ksplit), dim3(256), LDS, s, p.g);
   return vca_launch_status();
 }
 
@@ -1055,7 +1088,19 @@ int launch_layout(const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((matmul_wide_kernel<AKC, BKC>), dim3(p.g.ntm * p.g.ntn * p.g.ksplit), dim3(512), 128 * 1024, s, p.g);
     return vca_launch_status();
   }
-  return p.tile == 64 ? launch_tile<MODE, AKC, BKC, 64>(p, s) : launch_tile<MODE, AKC, BKC, 128>(p, s);
+  if (p.tile == 32) return launch_kernel<MODE, true, true, 32, 64, 1, true, 4>(p, s);
+  if (p.tile == 128)
+    return p.dma ? launch_kernel<MODE, AKC, BKC, 128, 128, 2, true, 2>(p, s)
+                 : launch_kernel<MODE, AKC, BKC, 128, 128, 2, false, 2>(p, s);
+  if (!p.dma) return launch_kernel<MODE, AKC, BKC, 64, 64, 2, false, 2>(p, s);
+  // Up to 128 rows the weights come from memory, not from another workgroup's lines in L2: three chunks under way instead
+  // of one (16 bits 4096 -> 16384, 64 rows: 37 us against 40, 128: 48 against 56; fp32 4096^2, 64: 28 against 32).  Larger
+  // products only lose workgroups a CU by it (2000 x 2048 -> 512: 15.5 against 14.9), column-major operands too
+  // (64 x 4096 x 4096, dx: 15.5 against 13.6).
+  if constexpr (AKC && BKC) {
+    if (p.g.ntm <= 2) return launch_kernel<MODE, true, true, 64, 64, 2, true, 4>(p, s);
+  }
+  return launch_kernel<MODE, AKC, BKC, 64, 64, 2, true, 2>(p, s);
 }
 
 template <int MODE>
@@ -1075,9 +1120,11 @@ long long ws_floats_of(const vca_matmul_desc* d) {
   if (plan_of(d, nullptr, nullptr, p) != 0) return 0;
   if (!p.tile) return ws_of(p);
   long long n = 0;
-  for (bool wide : {false, true}) {
-    const int nc = (p.g.K * (d->type == VCA_T_F32 ? 4ll : 2ll) + 127) / 128;
-    p.wide = wide && p.mode == MODE_16;
+  const int nc = (p.g.K * (d->type == VCA_T_F32 ? 4ll : 2ll) + 127) / 128;
+  const bool low = d->M <= 32 && !d->a_col && !d->b_col;
+  for (int form = 0; form < 4; ++form) {
+    p.wide = (form & 1) && p.mode == MODE_16;
+    p.low = (form & 2) && low;
     if (pick(p, nc) && ws_of(p) > n) n = ws_of(p);
   }
   return n;
@@ -1141,7 +1188,7 @@ int launch_folds(FoldArgs& f, const MatArgs* g0, const MatArgs* g1, int type, hi
 
 int act_rows(int M, int N, int esz) {                     // rows a workgroup of act_bwd_kernel takes
   const long long strips = ((long long)N * esz + 511) / 512;
-  int rows = M <= 64 ? 64 : 8;                            // up to 64 rows: one slab, and no launch to add slabs up
+  int rows = M <= 16 ? 16 : 8;     // up to 16 rows one slab, and no launch to add slabs up (16 x 512: 3.9 us, 4.9 with two)
   auto slabs = [&]() { return ((long long)M + rows - 1) / rows; };
   while ((rows < 256 && strips * slabs() > 1024) || slabs() > 65535) rows *= 2;   // (65535: the grid's second dimension)
   return rows;
@@ -1167,8 +1214,7 @@ extern "C" int vca_matmul_act(const vca_matmul_desc* d, const void* a, const voi
   return e ? e : launch_folds(f, p.g.ksplit > 1 ? &p.g : nullptr, nullptr, d->type, (hipStream_t)stream);
 }
 
-extern "C" long long vca_act_bwd_ws_floats(int type, int M, int N) {
-  if (M <= 0 || N <= 0 || type < VCA_T_F32 || type > VCA_T_F16) return 0;
+static long long act_bwd_ws(int type, int M, int N) {
   const int rows = act_rows(M, N, type == VCA_T_F32 ? 4 : 2);
   return ((long long)M + rows - 1) / rows * N;
 }
@@ -1194,16 +1240,6 @@ static bool act_bwd_ok(int type, int M, int N, int act, const void* gy, const vo
          (!dz || z) && aligned(type, {gy, dz, db}) && aligned(z_type(type), {z});
 }
 
-extern "C" int vca_act_bwd(int type, int M, int N, int act, float slope, const void* gy, const void* z, void* dz, void* db,
-                           int db_add, float* ws, long long ws_floats, void* stream) {
-  VCA_CHECK_ARG(act_bwd_ok(type, M, N, act, gy, z, dz, db) && (dz || db));
-  VCA_CHECK_ARG(!db || (ws && ws_floats >= vca_act_bwd_ws_floats(type, M, N) && (reinterpret_cast<uintptr_t>(ws) & 3) == 0));
-  FoldArgs f;
-  clear(f);
-  const int e = act_bwd(type, M, N, act, slope, gy, z, dz, db, db_add, ws, f, (hipStream_t)stream);
-  return e ? e : launch_folds(f, nullptr, nullptr, type, (hipStream_t)stream);
-}
-
 // The three products' descriptors of a backward pass.
 static vca_matmul_desc bwd_dx(const vca_linear_bwd& b) {
   vca_matmul_desc d = {b.M, b.K, b.N, b.type, b.nsplit, 0, 1, VCA_ACT_NONE, 0.f, b.N, b.ldw, b.K, 0};
@@ -1220,7 +1256,7 @@ static long long up4(long long n) { return (n + 3) / 4 * 4; }   // each part of 
 extern "C" long long vca_linear_act_bwd_ws_floats(const vca_linear_bwd* b) {
   if (!b || b->M <= 0 || b->N <= 0 || b->K <= 0) return 0;
   const vca_matmul_desc x = bwd_dx(*b), w = bwd_dw(*b);
-  return up4(vca_act_bwd_ws_floats(b->type, b->M, b->N)) + up4(ws_floats_of(&x)) + ws_floats_of(&w);
+  return up4(act_bwd_ws(b->type, b->M, b->N)) + up4(ws_floats_of(&x)) + ws_floats_of(&w);
 }
 
 extern "C" int vca_linear_act_bwd(const vca_linear_bwd* b, float* ws, long long ws_floats, void* stream) {
@@ -1241,7 +1277,7 @@ extern "C" int vca_linear_act_bwd(const vca_linear_bwd* b, float* ws, long long 
     if (rc) return rc;
   }
   // one part of the workspace for each of db, dx and dw, so that what is split is added up by one launch at the end
-  const long long at_x = b->db ? up4(vca_act_bwd_ws_floats(b->type, b->M, b->N)) : 0;
+  const long long at_x = b->db ? up4(act_bwd_ws(b->type, b->M, b->N)) : 0;
   const long long at_w = at_x + (b->dx ? up4(ws_of(px)) : 0), need = at_w + (b->dw ? ws_of(pw) : 0);
   VCA_CHECK_ARG(ws_floats >= need && (!need || (ws && (reinterpret_cast<uintptr_t>(ws) & 15) == 0)));
   hipStream_t s = (hipStream_t)stream;

@@ -927,14 +927,15 @@ def linear_act(x, w, bias=None, act=None, residual=None):
 
     x: (..., K); w: (N, K); bias: (N,); residual: (..., N), the output's shape; all of one type, fp32, bf16 or fp16, and
     on one device.  act: None, 'relu', 'leaky0.2' (LEAKY), 'tanh', 'gelu', 'gelu_tanh', 'silu', or the torch.nn module
-    of one of them.  Any sizes (no rows gives an empty result) and any strides: rows that are dense and equally spaced
-    are read in place, others are copied first.
+    of one of them.  Any number of rows (none gives an empty result), any K and N from one, any strides: rows that are
+    dense and equally spaced are read in place, others are copied first.
 
     fp32 tensors are multiplied as set_precision() says ('fp32': exact; the split and single-product modes like every
     other product, 'mixed' with single products in the gradients); 16-bit tensors take one product of their own type in
     every mode.  Sums, bias, activation and residual are fp32, and the result is rounded once; for the gradients dz =
-    gy act' is rounded to the tensors' type (the value under the activation is kept in more bits than that).  Inside direct_param_grad() the
-    gradients of leaf parameters are added straight into their .grad; input_grads_only() leaves them out."""
+    gy act' is rounded to the tensors' type (the value under the activation is kept in more bits than that).  Inside
+    direct_param_grad() the gradients of leaf parameters are added straight into their .grad; input_grads_only() leaves
+    them out."""
     code = _linear_act_code(act)
     dt, dev, xs, ws = x.dtype, x.device, x.shape, w.shape
     if dt not in _lib.TYPES:
@@ -2299,8 +2300,8 @@ class GradNorm:
     the same for a list that is used once.
 
     tensors: fp32 / bf16 / fp16 in any mixture, any sizes (empty ones too), any alignment, dense (contiguous up to a
-    permutation of the dimensions), all on one device.  The object holds references to them, so their memory stays
-    valid; it does not notice when a parameter is given another .grad.
+    permutation of the dimensions), all on one device.  The object keeps the memory they have now alive and works on that
+    memory: it does not notice when a parameter is given another .grad or a tensor other .data.
 
     norm and clip_ return the norm before clipping as a 0-dim fp32 device tensor, without a host synchronisation; both
     can be captured into a HIP graph, and two calls may run on two streams at once (each has its own workspace) as far
@@ -2326,6 +2327,7 @@ class GradNorm:
         n = len(ts)
         self.device = dev
         self._n = n
+        self._memory = [t.untyped_storage() for t in ts]    # (the pointers below stay good if a tensor's .data is replaced)
         self._ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in ts])
         self._numel = (ctypes.c_longlong * n)(*[t.numel() for t in ts])
         self._types = (ctypes.c_int * n)(*[_lib.TYPES[t.dtype] for t in ts])
