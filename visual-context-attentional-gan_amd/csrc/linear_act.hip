@@ -522,28 +522,24 @@ __global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g)
   if (c0 < whole) {
     A.start(c0);
     B.start(c0);
-    int at = 0, to = 0;                                   // stages of chunk c and of the next chunk to send
-    auto turn = [](int s) { return s + 1 == STAGES ? 0 : s + 1; };
-    auto send = [&]() {
-      A.dma(smem + to * STAGE);
-      B.dma(smem + to * STAGE + BM * 128);
-      to = turn(to);
+    static_assert((STAGES & (STAGES - 1)) == 0, "");
+    auto stage = [&](int c) { return smem + ((c - c0) & (STAGES - 1)) * STAGE; };
+    auto send = [&](int c) {
+      A.dma(stage(c));
+      B.dma(stage(c) + BM * 128);
     };
-    for (int c = c0; c < min(whole, c0 + STAGES - 1); ++c) send();
-    // Chunk c has landed (in every wave behind the barrier) when at most the STAGES - 2 later chunks' pieces are under
-    // way; every wave has left the stage that is sent to next, chunk c - 1's, with its reads done.
-    int c = c0;
-    for (; c + STAGES - 1 < whole; ++c) {
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * (A.PIECES + B.PIECES)) : "memory");
-      send();
-      compute(smem + at * STAGE);
-      at = turn(at);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the rest is all under way
-    __syncthreads();
-    for (; c < whole; ++c) {
-      compute(smem + at * STAGE);
-      at = turn(at);
+    for (int c = c0; c < min(whole, c0 + STAGES - 1); ++c) send(c);
+    for (int c = c0; c < whole; ++c) {
+      // Chunk c has landed, in every wave behind the barrier: at most the STAGES - 2 chunks behind it are under way.  Every
+      // wave has left the stage that is sent to next, chunk c - 1's, with its reads done.
+      if (STAGES > 2 && c + STAGES - 2 < whole) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * (A.PIECES + B.PIECES)) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+      }
+      if (c + STAGES - 1 < whole) send(c + STAGES - 1);
+      compute(stage(c));
     }
   }
   if (whole < c1) {                                       // not by DMA: chunk c + 1 waits in registers under chunk c
@@ -1094,7 +1090,7 @@ int launch_layout(const Plan& p, hipStream_t s) {
                  : launch_kernel<MODE, AKC, BKC, 128, 128, 2, false, 2>(p, s);
   if (!p.dma) return launch_kernel<MODE, AKC, BKC, 64, 64, 2, false, 2>(p, s);
   // Up to 128 rows the weights come from memory, not from another workgroup's lines in L2: three chunks under way instead
-  // of one (16 bits 4096 -> 16384, 64 rows: 37 us against 40, 128: 48 against 56; fp32 4096^2, 64: 28 against 32).  Larger
+  // of one (16 bits 4096 -> 16384, 64 rows: 38 us against 40, 128: 48 against 56; fp32 4096^2, 64: 28 against 32).  Larger
   // products only lose workgroups a CU by it (2000 x 2048 -> 512: 15.5 against 14.9), column-major operands too
   // (64 x 4096 x 4096, dx: 15.5 against 13.6).
   if constexpr (AKC && BKC) {
