@@ -139,14 +139,22 @@ __device__ __forceinline__ float act_slope(float z, int act, float slope) {
   }
 }
 
-template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) AnyVec { T e[V]; };
+// V neighbouring elements from any address (a vector, not an array: the compiler keeps that in registers)
+template <typename T, int V> struct AnyVec {
+  typedef T Vec __attribute__((ext_vector_type(V)));
+  Vec e;
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(&e, p, sizeof(e)); }
+};
 
 template <typename T, int V>
 __device__ __forceinline__ AnyVec<T, V> load_any(const T* p, int left) {      // left: columns that exist
   AnyVec<T, V> q;
-  if (left >= V) return *reinterpret_cast<const AnyVec<T, V>*>(p);
+  if (left >= V) {
+    q.load(p);
+  } else {
 #pragma unroll
-  for (int r = 0; r < V; ++r) q.e[r] = r < left ? p[r] : (T)0.f;
+    for (int r = 0; r < V; ++r) q.e[r] = r < left ? p[r] : (T)0.f;
+  }
   return q;
 }
 
@@ -156,7 +164,7 @@ __device__ __forceinline__ void store_any(T* p, int left, const float (&v)[V]) {
     AnyVec<T, V> q;
 #pragma unroll
     for (int r = 0; r < V; ++r) q.e[r] = (T)v[r];
-    *reinterpret_cast<AnyVec<T, V>*>(p) = q;
+    __builtin_memcpy(p, &q.e, sizeof(q.e));
   } else {
 #pragma unroll
     for (int r = 0; r < V; ++r)
@@ -910,7 +918,7 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(int M, int N, int act, flo
       Vec16<T> a, d;
       AnyVec<typename ZOf<T>::type, V> b;
       a.u = reinterpret_cast<const Any16*>(gy + o)->u;
-      if (z) b = *reinterpret_cast<const AnyVec<typename ZOf<T>::type, V>*>(z + o);
+      if (z) b.load(z + o);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         float v = (float)a.e[e];
