@@ -236,7 +236,8 @@ template <int MODE, bool KC, int R, int NT>
 struct Operand {
   typedef typename ElemOf<MODE>::T T;
   static constexpr int ESZ = sizeof(T), EPP = 16 / ESZ, BK = 128 / ESZ;
-  static constexpr int PIECES = R * 8 / NT;               // 16-byte pieces a thread stages
+  static constexpr int PIECES = (R * 8 + NT - 1) / NT;    // 16-byte pieces a thread stages (the last one: some waves)
+  __device__ __forceinline__ static bool mine(int it, int thread) { return R * 8 % NT == 0 || it * NT + thread < R * 8; }
   static constexpr int PPR = R * ESZ / 16;                // pieces of a row of k (index contiguous)
   const char* src[PIECES];                                // this thread's pieces of the next chunk to fetch (DMA)
   const char* base;
@@ -279,6 +280,7 @@ struct Operand {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 #pragma unroll
     for (int it = 0; it < PIECES; ++it) {
+      if (!mine(it, wave * 64)) continue;
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[it],
                                        (__attribute__((address_space(3))) void*)(stage + (it * NT + wave * 64) * 16), 16,
                                        0, 0);
@@ -293,7 +295,7 @@ struct Operand {
       piece(it, row, pc);
       r[it] = make_uint4(0, 0, 0, 0);
       const int o = o0 + (KC ? row : pc * EPP), k = c * BK + (KC ? pc * EPP : row);
-      if (o >= outer || k >= K) continue;
+      if (o >= outer || k >= K || !mine(it, tid)) continue;
       const int left = KC ? K - k : outer - o;            // elements of the piece that exist
       const char* p = base + (KC ? (long long)o * ldb + (long long)k * ESZ : (long long)k * ldb + (long long)o * ESZ);
       if (left >= EPP) {
@@ -309,7 +311,8 @@ struct Operand {
 
   __device__ __forceinline__ void put(char* stage, const uint4 (&r)[PIECES]) const {
 #pragma unroll
-    for (int it = 0; it < PIECES; ++it) *reinterpret_cast<uint4*>(stage + (it * NT + tid) * 16) = r[it];
+    for (int it = 0; it < PIECES; ++it)
+      if (mine(it, tid)) *reinterpret_cast<uint4*>(stage + (it * NT + tid) * 16) = r[it];
   }
 };
 
@@ -968,8 +971,8 @@ int mode_of(const vca_matmul_desc& d) {
 
 struct Plan {
   MatArgs g;
-  int mode, tile;                     // 32 (x 64), 64, 128 or 256; 0: few rows
-  bool dma, wide, low;                // low, wide: the 32 and 256 tiles may be taken
+  int mode, bm, bn;                   // the tile; 0: few rows
+  bool dma, wide, low, tall;          // may be taken: the 256-wide tiles, the 32-row ones, those with more rows than columns
 };
 
 // Rows of x times bytes of W up to which few_rows_kernel takes a product of at most 16 rows: every workgroup of 16 columns
@@ -985,22 +988,26 @@ constexpr double FEW_BYTES = 600e6;
 // within 10 % of the best one measured at each.  Where sides change (us): fp32 4800 x 1280, K 512: 64-wide tiles 62, 128
 // 74; 8192 x 4096, K 4096: 2349 against 2043.  16 bits 2048^3: 64 29, 128 30, 256 39 (split); 4800 x 2560, K 5120:
 // 197, 137, 112; 64 x 4096, K 4096: 64-wide unsplit 31, split four ways 15.  Up to 32 rows tiles of 32 x 64 (whose work is
-// the memory's, not the matrix cores'), against 64 x 64: 32 x 4096 -> 4096 13.4 / 14.5, fp32 21.6 / 25.8.
-struct TileCost { int tile; double work, wait, ends; };
-constexpr TileCost COST[4][4] = {
-    {{256, 1.55, 1.55, 8.}, {128, 0.53, 0.85, 2.}, {64, 0.20, 0.45, 0.8}, {32, 0.42, 0.24, 2.}},     // 16-bit tensors
-    {{0, 0., 0., 0.}, {128, 1.95, 2.15, 2.5}, {64, 0.56, 0.62, 1.}, {32, 0.42, 0.44, 2.}},           // fp32, exact
-    {{0, 0., 0., 0.}, {128, 0.92, 1.15, 2.5}, {64, 0.36, 0.55, 1.}, {32, 0.42, 0.40, 2.}},           // fp32, three products
-    {{0, 0., 0., 0.}, {128, 0.46, 0.85, 2.5}, {64, 0.22, 0.45, 1.}, {32, 0.42, 0.35, 2.}}};          // fp32, one product
+// the memory's, not the matrix cores'), against 64 x 64: 32 x 4096 -> 4096 13.4 / 14.5, fp32 21.6 / 25.8.  Tall tiles of
+// fp32 products, whose counts of tiles fall between those of the square ones: 4800 x 512 -> 1280 128 x 64 63 / 64 x 64 69;
+// 4800 x 1280 -> 512 80 x 64 62 / 73; 900 x 700 -> 1300 23 / 29; 2400 x 2560 -> 512 160 x 64 split four ways 65 / 128 x 128
+// split three ways 68; but 1500 x 2048 -> 2048 80 x 64 147 / 114.
+struct TileCost { int bm, bn; double work, wait, ends; };
+constexpr TileCost COST[4][6] = {
+    {{256, 256, 1.55, 1.55, 8.}, {128, 128, 0.53, 0.85, 2.}, {64, 64, 0.20, 0.45, 0.8}, {32, 64, 0.42, 0.24, 2.}},   // 16 bits
+    {{128, 128, 1.95, 2.15, 5.5}, {64, 64, 0.56, 0.62, 2.}, {32, 64, 0.42, 0.44, 2.},                          // fp32, exact
+     {160, 64, 1.22, 1.50, 4.5}, {128, 64, 1.05, 1.15, 3.3}, {80, 64, 0.73, 0.82, 2.}},
+    {{128, 128, 0.92, 1.15, 4.}, {64, 64, 0.36, 0.55, 1.}, {32, 64, 0.42, 0.40, 2.},                  // fp32, three products
+     {160, 64, 0.68, 1.05, 4.}, {128, 64, 0.63, 0.87, 2.3}},
+    {{128, 128, 0.46, 0.85, 2.5}, {64, 64, 0.22, 0.45, 1.}, {32, 64, 0.42, 0.35, 2.}}};                 // fp32, one product
 
 bool pick(Plan& p, int nc) {
   MatArgs& g = p.g;
   double best = 0.;
-  p.tile = 0;
+  p.bm = 0;
   for (const TileCost& t : COST[p.mode]) {
-    if (!t.tile || (t.tile == 256 && !p.wide) || (t.tile == 32 && !p.low)) continue;
-    const long long cols = t.tile == 32 ? 64 : t.tile;
-    const long long tiles = ((g.M + (long long)t.tile - 1) / t.tile) * ((g.N + cols - 1) / cols);
+    if (!t.bm || (t.bm == 256 && !p.wide) || (t.bm == 32 && !p.low) || (t.bm > t.bn && !p.tall)) continue;
+    const long long tiles = ((g.M + (long long)t.bm - 1) / t.bm) * ((g.N + (long long)t.bn - 1) / t.bn);
     if (tiles >= (1 << 24)) continue;
     for (int ks = 1; ks <= 32 && ks <= nc; ++ks) {
       const int chunks = (nc + ks - 1) / ks;
@@ -1008,16 +1015,17 @@ bool pick(Plan& p, int nc) {
       const double r = (double)((tiles * ks + 255) / 256);
       double us = chunks * (r * t.work > t.wait ? r * t.work : t.wait) + r * t.ends;
       if (ks > 1) us += 3. + (double)ks * g.M * g.npad * 1e-6;                 // written and read at 8 bytes / ps
-      if (p.tile && us >= best) continue;
+      if (p.bm && us >= best) continue;
       best = us;
-      p.tile = t.tile;
+      p.bm = t.bm;
+      p.bn = t.bn;
       g.cpz = chunks;
     }
   }
-  if (!p.tile) return false;
+  if (!p.bm) return false;
   g.ksplit = (nc + g.cpz - 1) / g.cpz;
-  g.ntm = (g.M + p.tile - 1) / p.tile;
-  g.ntn = p.tile == 32 ? (g.N + 63) / 64 : (g.N + p.tile - 1) / p.tile;
+  g.ntm = (g.M + p.bm - 1) / p.bm;
+  g.ntn = (g.N + p.bn - 1) / p.bn;
   return true;
 }
 
@@ -1055,7 +1063,7 @@ int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p) {
     // A workgroup streams its 16 rows of W at some 30 GB/s, all of them at most at 5 TB/s; where columns alone give too few
     // of them to load the memory, the reduction is split too, if that saves more than the launch that adds the parts (one
     // row, split and unsplit: bf16 16384 -> 1024 12.9 / 21.7 us, fp32 2560 -> 512 7.2 / 9.6, fp32 4096^2 21.2 / 20.3).
-    p.tile = 0;
+    p.bm = 0;
     const int nc = (d.K * esz + 63) / 64, blocks = (d.N + 15) / 16;
     double best = 0.;
     for (int ks = 1; ks <= 16 && (ks == 1 || (blocks * ks <= 512 && nc / ks >= 2 * FEW_GROUP)); ++ks) {
@@ -1072,6 +1080,7 @@ int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p) {
   }
   // the 256-wide kernel addresses its pieces by 32-bit offsets from the tile: 256 rows (64 of k) of at most 4 MB
   p.low = p.dma && d.M <= 32 && !d.a_col && !d.b_col;
+  p.tall = p.dma && !d.a_col;
   p.wide = p.mode == MODE_16 && p.dma && d.lda <= (1 << 21) && d.ldb <= (1 << 21);
   return pick(p, g.cpz) ? 0 : -22;
 }
@@ -1087,13 +1096,22 @@ int launch_kernel(const Plan& p, hipStream_t s) {
 
 template <int MODE, bool AKC, bool BKC>
 int launch_layout(const Plan& p, hipStream_t s) {
-  if (MODE == MODE_16 && p.tile == 256) {
+  if (MODE == MODE_16 && p.bm == 256) {
     VCA_MAX_LDS((matmul_wide_kernel<AKC, BKC>));
     hipLaunchKernelGGL((matmul_wide_kernel<AKC, BKC>), dim3(p.g.ntm * p.g.ntn * p.g.ksplit), dim3(512), 128 * 1024, s, p.g);
     return vca_launch_status();
   }
-  if (p.tile == 32) return launch_kernel<MODE, true, true, 32, 64, 1, true, 4>(p, s);
-  if (p.tile == 128)
+  if constexpr (AKC && BKC) {
+    if (p.bm == 32) return launch_kernel<MODE, true, true, 32, 64, 1, true, 4>(p, s);
+  }
+  if constexpr (AKC && (MODE == MODE_F32 || MODE == MODE_S3)) {
+    if (p.bm == 160) return launch_kernel<MODE, true, BKC, 160, 64, 2, true, 2>(p, s);
+    if (p.bm == 128 && p.bn == 64) return launch_kernel<MODE, true, BKC, 128, 64, 2, true, 2>(p, s);
+  }
+  if constexpr (AKC && MODE == MODE_F32) {
+    if (p.bm == 80) return launch_kernel<MODE, true, BKC, 80, 64, 1, true, 2>(p, s);
+  }
+  if (p.bm == 128)
     return p.dma ? launch_kernel<MODE, AKC, BKC, 128, 128, 2, true, 2>(p, s)
                  : launch_kernel<MODE, AKC, BKC, 128, 128, 2, false, 2>(p, s);
   if (!p.dma) return launch_kernel<MODE, AKC, BKC, 64, 64, 2, false, 2>(p, s);
@@ -1122,13 +1140,14 @@ long long ws_of(const Plan& p) {
 long long ws_floats_of(const vca_matmul_desc* d) {
   Plan p;
   if (plan_of(d, nullptr, nullptr, p) != 0) return 0;
-  if (!p.tile) return ws_of(p);
+  if (!p.bm) return ws_of(p);
   long long n = 0;
   const int nc = (p.g.K * (d->type == VCA_T_F32 ? 4ll : 2ll) + 127) / 128;
   const bool low = d->M <= 32 && !d->a_col && !d->b_col;
-  for (int form = 0; form < 4; ++form) {
-    p.wide = (form & 1) && p.mode == MODE_16;
-    p.low = (form & 2) && low;
+  for (int form = 0; form < 3; ++form) {                   // not by DMA, by DMA, and with the 256-wide tiles
+    p.low = form && low;
+    p.tall = form && !d->a_col;
+    p.wide = form == 2 && p.mode == MODE_16;
     if (pick(p, nc) && ws_of(p) > n) n = ws_of(p);
   }
   return n;
@@ -1154,7 +1173,7 @@ int launch_product(Plan& p, const vca_matmul_desc& d, const void* a, const void*
   g.z = z;
   g.part = g.ksplit > 1 ? ws : nullptr;
   const bool ac = d.a_col != 0, bc = d.b_col != 0;
-  if (p.tile == 0) {
+  if (p.bm == 0) {
     const dim3 grid((g.N + 15) / 16, g.ksplit);
     if (p.mode == MODE_16) hipLaunchKernelGGL(few_rows_kernel<MODE_16>, grid, dim3(FEW_WAVES * 64), 0, s, g);
     else hipLaunchKernelGGL(few_rows_kernel<MODE_F32>, grid, dim3(FEW_WAVES * 64), 0, s, g);
