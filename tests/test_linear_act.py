@@ -126,11 +126,12 @@ def _run(M, K, N, dtype, act, seed, mode='fp32', bias=True, res=True):
 
 # rows, reduction, columns: single ones, below and just over every tile and chunk, odd and even, few rows with long
 # reductions (split over workgroups), the serving kernel's 16-row edge and wide weights beyond it, the 32-row tiles, 64-row
-# tiles with four stages
+# tiles with four stages, reductions that each tile begins elsewhere
 SHAPES = [(1, 1, 1), (1, 8, 16), (2, 3, 5), (1, 512, 512), (7, 129, 33), (15, 1000, 18), (16, 2048, 40), (17, 2048, 40),
           (64, 64, 64), (127, 32, 129), (128, 64, 128), (129, 65, 127), (200, 1111, 77), (333, 96, 513), (40, 5000, 12),
           (600, 256, 1280), (3, 20000, 70), (16, 9001, 33), (24, 4096, 300), (32, 512, 1280), (31, 1000, 70), (20, 8256, 72),
-          (17, 40, 2000), (100, 640, 1300), (128, 72, 136), (9, 8192, 8200)]
+          (17, 40, 2000), (100, 640, 1300), (128, 72, 136), (9, 8192, 8200), (60, 1064, 8200), (33, 128, 8200), (32, 64, 8256),
+          (24, 200, 16384)]
 
 
 @gpu

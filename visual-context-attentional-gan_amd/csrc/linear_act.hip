@@ -288,6 +288,11 @@ struct Operand {
     }
   }
 
+  __device__ __forceinline__ void back(int chunks) {       // from the end of the whole chunks to their first
+#pragma unroll
+    for (int it = 0; it < PIECES; ++it) src[it] -= chunks * (KC ? 128ll : BK * ldb);
+  }
+
   __device__ __forceinline__ void fetch(int c, uint4 (&r)[PIECES]) const {
 #pragma unroll
     for (int it = 0; it < PIECES; ++it) {
@@ -452,7 +457,8 @@ __device__ __forceinline__ void store_tile(const MatArgs& g, const f32x4 (&acc)[
   }
 }
 
-template <int MODE, bool AKC, bool BKC, int BM, int BN, int NWM, int NWN, bool DMA, int STAGES>
+template <int MODE, bool AKC, bool BKC, int BM, int BN, int NWM, int NWN, bool DMA, int STAGES,
+          bool TURN>
 __global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef typename ElemOf<MODE>::T T;
@@ -531,11 +537,19 @@ __global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g)
   };
 
   if (c0 < whole) {
-    A.start(c0);
-    B.start(c0);
+    // TURN: each tile starts at a chunk of its own.  Where every CU walks through its rows of W at the same column and the
+    // rows lie a power of two apart, few of the memory's channels are asked at a time (4096 -> 16384 in bf16, 8 rows 29.8 ->
+    // 25.8 us, 64 rows 31.6 -> 27.5; with less than half the CUs at work it changes nothing).
+    const int turn = TURN ? tn % (whole - c0) : 0;
+    A.start(c0 + turn);
+    B.start(c0 + turn);
     static_assert((STAGES & (STAGES - 1)) == 0, "");
     auto stage = [&](int c) { return smem + ((c - c0) & (STAGES - 1)) * STAGE; };
     auto send = [&](int c) {
+      if (TURN && c == whole - turn) {
+        A.back(whole - c0);
+        B.back(whole - c0);
+      }
       A.dma(stage(c));
       B.dma(stage(c) + BM * 128);
     };
@@ -972,48 +986,54 @@ int mode_of(const vca_matmul_desc& d) {
 struct Plan {
   MatArgs g;
   int mode, bm, bn;                   // the tile; 0: few rows
-  bool dma, wide, low, tall;          // may be taken: the 256-wide tiles, the 32-row ones, those with more rows than columns
+  bool dma, wide, low, tall;          // may be taken: the 256-wide tiles, the 32-row ones and four stages, those with more
+                                      // rows than columns
 };
 
 // Rows of x times bytes of W up to which few_rows_kernel takes a product of at most 16 rows: every workgroup of 16 columns
-// reads x again, a tile of 64 columns a quarter of that.  us, few_rows_kernel and tiles: bf16 4096 -> 16384, 1 row 25 / 30,
-// 4 rows 27.6 / 29.6, 8 rows 31 / 29.7, 16 rows 39 / 30; 4096 -> 4096, 16 rows 11.6 / 12.9; fp32 4096 -> 4096, 16 rows
-// 25 / 21; 512 -> 512, 16 rows 4.2 / 6.6.
-constexpr double FEW_BYTES = 600e6;
+// reads x again, a tile of 64 columns a quarter of that.  us, few_rows_kernel and tiles: bf16 4096 -> 16384, 1 row
+// 25.1 / 26.2, 4 rows 27.6 / 26, 8 rows 31 / 25.8, 16 rows 39 / 26; 4096 -> 4096, 8 rows 10.2 / 11.9; fp32 4096 -> 4096,
+// 16 rows 25 / 21; 512 -> 512, 16 rows 4.2 / 6.6.
+constexpr double FEW_BYTES = 500e6;
+constexpr int LOW_ROWS = 128;         // see launch_layout
 
 // Tile and split of a product, by the time the candidates would take.  A tile's chunk costs a CU `work` us of its matrix
 // cores; a workgroup that has a CU to itself cannot go below `wait` us a chunk (LDS and memory latency, one barrier a
-// chunk), a CU with r workgroups takes max(wait, r work).  `ends`: filling the pipeline and storing the tile.  A split
-// adds one launch and a pass over the partial products.  Fitted to launches of 2 to 2000 us on this part; the choice is
-// within 10 % of the best one measured at each.  Where sides change (us): fp32 4800 x 1280, K 512: 64-wide tiles 62, 128
-// 74; 8192 x 4096, K 4096: 2349 against 2043.  16 bits 2048^3: 64 29, 128 30, 256 39 (split); 4800 x 2560, K 5120:
-// 197, 137, 112; 64 x 4096, K 4096: 64-wide unsplit 31, split four ways 15.  Up to 32 rows tiles of 32 x 64 (whose work is
-// the memory's, not the matrix cores'), against 64 x 64: 32 x 4096 -> 4096 13.4 / 14.5, fp32 21.6 / 25.8.  Tall tiles of
-// fp32 products, whose counts of tiles fall between those of the square ones: 4800 x 512 -> 1280 128 x 64 63 / 64 x 64 69;
-// 4800 x 1280 -> 512 80 x 64 62 / 73; 900 x 700 -> 1300 23 / 29; 2400 x 2560 -> 512 160 x 64 split four ways 65 / 128 x 128
-// split three ways 68; but 1500 x 2048 -> 2048 80 x 64 147 / 114.
+// chunk), a CU with r workgroups takes max(wait, r work), and all of them together no less than the operands' trip from
+// memory.  `ends`: filling the pipeline and storing the tile.  A split adds one launch and a pass over the partial products.
+// Fitted to launches of 2 to 2000 us on this part; the choice is within some 10 % of the best one measured at each.  Where
+// sides change (us): fp32 8192 x 4096, K 4096: 64-wide tiles 2349, 128 2043.  16 bits 2048^3: 64 29, 128 30, 256 39 (split);
+// 4800 x 2560, K 5120: 197, 137, 112; 64 x 4096, K 4096: 64-wide unsplit 23, split four ways 13.  Up to 32 rows tiles of
+// 32 x 64, against 64 x 64: 32 x 4096 -> 4096 12.2 / 13.5, fp32 21.3 / 25.8.  Tall tiles of fp32 products, whose counts fall
+// between those of the square ones: 4800 x 512 -> 1280 128 x 64 63 / 64 x 64 69; 4800 x 1280 -> 512 80 x 64 62 / 73;
+// 900 x 700 -> 1300 23 / 29; 2400 x 2560 -> 512 160 x 64 split four ways 65 / 128 x 128 split three ways 68; but
+// 1500 x 2048 -> 2048 80 x 64 147 / 114.  (In 16 bits they gain 2 us at the most: 4800 x 512 -> 1280 11.9 / 13.6.)
 struct TileCost { int bm, bn; double work, wait, ends; };
 constexpr TileCost COST[4][6] = {
-    {{256, 256, 1.55, 1.55, 8.}, {128, 128, 0.53, 0.85, 2.}, {64, 64, 0.20, 0.45, 0.8}, {32, 64, 0.42, 0.24, 2.}},   // 16 bits
-    {{128, 128, 1.95, 2.15, 5.5}, {64, 64, 0.56, 0.62, 2.}, {32, 64, 0.42, 0.44, 2.},                          // fp32, exact
+    {{256, 256, 1.55, 1.55, 8.}, {128, 128, 0.53, 0.85, 2.}, {64, 64, 0.20, 0.45, 0.8}, {32, 64, 0.12, 0.24, 2.}},   // 16 bits
+    {{128, 128, 1.95, 2.15, 5.5}, {64, 64, 0.56, 0.62, 2.}, {32, 64, 0.22, 0.44, 2.},                          // fp32, exact
      {160, 64, 1.22, 1.50, 4.5}, {128, 64, 1.05, 1.15, 3.3}, {80, 64, 0.73, 0.82, 2.}},
-    {{128, 128, 0.92, 1.15, 4.}, {64, 64, 0.36, 0.55, 1.}, {32, 64, 0.42, 0.40, 2.},                  // fp32, three products
+    {{128, 128, 0.92, 1.15, 4.}, {64, 64, 0.36, 0.55, 1.}, {32, 64, 0.15, 0.40, 2.},                  // fp32, three products
      {160, 64, 0.68, 1.05, 4.}, {128, 64, 0.63, 0.87, 2.3}},
-    {{128, 128, 0.46, 0.85, 2.5}, {64, 64, 0.22, 0.45, 1.}, {32, 64, 0.42, 0.35, 2.}}};                 // fp32, one product
+    {{128, 128, 0.46, 0.85, 2.5}, {64, 64, 0.22, 0.45, 1.}, {32, 64, 0.12, 0.35, 2.}}};                 // fp32, one product
 
 bool pick(Plan& p, int nc) {
   MatArgs& g = p.g;
+  const double memory = ((double)g.M + g.N) * g.K * (p.mode == MODE_16 ? 2 : 4) / 5e6;   // both operands once, at 5 TB/s
   double best = 0.;
   p.bm = 0;
   for (const TileCost& t : COST[p.mode]) {
-    if (!t.bm || (t.bm == 256 && !p.wide) || (t.bm == 32 && !p.low) || (t.bm > t.bn && !p.tall)) continue;
+    if (!t.bm || (t.bm == 256 && !p.wide) || (t.bm == 32 && !(p.low && g.M <= 32)) || (t.bm > t.bn && !p.tall)) continue;
     const long long tiles = ((g.M + (long long)t.bm - 1) / t.bm) * ((g.N + (long long)t.bn - 1) / t.bn);
     if (tiles >= (1 << 24)) continue;
+    const double wait = t.wait * (p.low && g.M <= 64 && t.bm == 64 && p.mode == MODE_16 ? 0.75 : 1.);   // (four stages)
     for (int ks = 1; ks <= 32 && ks <= nc; ++ks) {
       const int chunks = (nc + ks - 1) / ks;
       if (ks > 1 && (chunks < 2 || tiles * ks > 2048)) break;
       const double r = (double)((tiles * ks + 255) / 256);
-      double us = chunks * (r * t.work > t.wait ? r * t.work : t.wait) + r * t.ends;
+      double us = chunks * (r * t.work > wait ? r * t.work : wait);
+      if (us < memory) us = memory;
+      us += r * t.ends;
       if (ks > 1) us += 3. + (double)ks * g.M * g.npad * 1e-6;                 // written and read at 8 bytes / ps
       if (p.bm && us >= best) continue;
       best = us;
@@ -1079,17 +1099,17 @@ int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p) {
     return 0;
   }
   // the 256-wide kernel addresses its pieces by 32-bit offsets from the tile: 256 rows (64 of k) of at most 4 MB
-  p.low = p.dma && d.M <= 32 && !d.a_col && !d.b_col;
+  p.low = p.dma && d.M <= LOW_ROWS && !d.a_col && !d.b_col;
   p.tall = p.dma && !d.a_col;
   p.wide = p.mode == MODE_16 && p.dma && d.lda <= (1 << 21) && d.ldb <= (1 << 21);
   return pick(p, g.cpz) ? 0 : -22;
 }
 
-template <int MODE, bool AKC, bool BKC, int BM, int BN, int NWM, bool DMA, int STAGES>
+template <int MODE, bool AKC, bool BKC, int BM, int BN, int NWM, bool DMA, int STAGES, bool TURN = false>
 int launch_kernel(const Plan& p, hipStream_t s) {
   constexpr int LDS = STAGES * (BM + BN) * 128;            // at most 64 KB
   static_assert(LDS <= 64 * 1024, "");
-  hipLaunchKernelGGL((matmul_kernel<MODE, AKC, BKC, BM, BN, NWM, 4 / NWM, DMA, STAGES>),
+  hipLaunchKernelGGL((matmul_kernel<MODE, AKC, BKC, BM, BN, NWM, 4 / NWM, DMA, STAGES, TURN>),
                      dim3(p.g.ntm * p.g.ntn * p.g.ksplit), dim3(256), LDS, s, p.g);
   return vca_launch_status();
 }
@@ -1101,8 +1121,11 @@ int launch_layout(const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((matmul_wide_kernel<AKC, BKC>), dim3(p.g.ntm * p.g.ntn * p.g.ksplit), dim3(512), 128 * 1024, s, p.g);
     return vca_launch_status();
   }
+  const bool turn = p.g.ksplit == 1 && p.g.ntm * p.g.ntn >= 128;
   if constexpr (AKC && BKC) {
-    if (p.bm == 32) return launch_kernel<MODE, true, true, 32, 64, 1, true, 4>(p, s);
+    if (p.bm == 32)
+      return turn ? launch_kernel<MODE, true, true, 32, 64, 1, true, 4, true>(p, s)
+                  : launch_kernel<MODE, true, true, 32, 64, 1, true, 4>(p, s);
   }
   if constexpr (AKC && (MODE == MODE_F32 || MODE == MODE_S3)) {
     if (p.bm == 160) return launch_kernel<MODE, true, BKC, 160, 64, 2, true, 2>(p, s);
@@ -1120,7 +1143,9 @@ int launch_layout(const Plan& p, hipStream_t s) {
   // products only lose workgroups a CU by it (2000 x 2048 -> 512: 15.5 against 14.9), column-major operands too
   // (64 x 4096 x 4096, dx: 15.5 against 13.6).
   if constexpr (AKC && BKC) {
-    if (p.g.ntm <= 2) return launch_kernel<MODE, true, true, 64, 64, 2, true, 4>(p, s);
+    if (p.low)
+      return turn ? launch_kernel<MODE, true, true, 64, 64, 2, true, 4, true>(p, s)
+                  : launch_kernel<MODE, true, true, 64, 64, 2, true, 4>(p, s);
   }
   return launch_kernel<MODE, AKC, BKC, 64, 64, 2, true, 2>(p, s);
 }
@@ -1143,7 +1168,7 @@ long long ws_floats_of(const vca_matmul_desc* d) {
   if (!p.bm) return ws_of(p);
   long long n = 0;
   const int nc = (p.g.K * (d->type == VCA_T_F32 ? 4ll : 2ll) + 127) / 128;
-  const bool low = d->M <= 32 && !d->a_col && !d->b_col;
+  const bool low = d->M <= LOW_ROWS && !d->a_col && !d->b_col;
   for (int form = 0; form < 3; ++form) {                   // not by DMA, by DMA, and with the 256-wide tiles
     p.low = form && low;
     p.tall = form && !d->a_col;
