@@ -213,8 +213,8 @@ __device__ __forceinline__ void finish(const MatArgs& g, int m, int n, float (&v
 // to LDS (16-byte pieces, operands 16-byte aligned); the reduction's last, partial chunk, and every chunk of operands of
 // another alignment, go through registers with masks.
 //
-// fp32 is bound by the matrix cores: 8192^3 at 139 TFLOP/s of the library's 154 (128-wide tiles); 2400 x 2560 -> 512, whose
-// 228 workgroups leave a tenth of the CUs idle, 68 us = 92 TFLOP/s.  16 bits with these tiles are bound by LDS and by the
+// fp32 is bound by the matrix cores: 8192^3 at 139 TFLOP/s of the library's 154 (128-wide tiles); smaller ones lose to
+// tiles that do not divide over the CUs and to the ends of short reductions, 2400 x 2560 -> 512 64 us = 98 TFLOP/s.  16 bits with these tiles are bound by LDS and by the
 // wait for a chunk: 2048^3 29 us = 590 TFLOP/s.
 //
 // LDS images of an operand with R rows in the tile:
