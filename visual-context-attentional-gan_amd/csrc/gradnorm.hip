@@ -26,8 +26,9 @@ constexpr int FUSED_PARTS = 256;         // partial sums up to which the Adam up
                                          // by 6000 workgroups): 140 and 136
 constexpr int SMALL_WAVES = 16;
 constexpr long long SMALL_CHUNK = 4096;  // bytes a wave takes at a time in the single-workgroup form
-constexpr int SMALL_ITEMS = 32;          // chunks up to which one workgroup does everything: 64 KB 3.2 us, two launches
-                                         // 4.5; 128 KB 4.3 and 4.7; 256 KB would be 6.4 and 4.6
+// Chunks up to which one workgroup does everything; us, one workgroup and two launches, norm: 64 KB 3.2 / 4.6, 128 KB
+// 4.2 / 4.5, 256 KB 6.4 / 4.7; clipping: 64 KB 5.7 / 6.7, 96 KB 6.6 / 6.8, 128 KB 8.5 / 6.8.
+constexpr int SMALL_NORM = 32, SMALL_CLIP = 24;
 
 struct Table {
   const void* p[TABLE];
@@ -477,8 +478,8 @@ int norm_partials(bool once, int n, const void* const* p, const long long* numel
 }
 
 // One workgroup is enough: the whole list in one table and few chunks.
-bool small_list(int n, const void* const* p, const long long* numel, const int* type, Table& t) {
-  if (total_chunks(n, p, numel, type, SMALL_CHUNK) > SMALL_ITEMS) return false;
+bool small_list(int n, const void* const* p, const long long* numel, const int* type, int items, Table& t) {
+  if (total_chunks(n, p, numel, type, SMALL_CHUNK) > items) return false;
   return fill(t, 0, n, p, numel, type, SMALL_CHUNK, 0) == n;
 }
 
@@ -491,7 +492,7 @@ extern "C" long long vca_grad_norm_ws_doubles(int ntensor, const void* const* h_
   if (!h_ptrs) return MAX_CHUNKS + 2ll * ntensor;
   if (!list_ok(ntensor, h_ptrs, h_numel, h_types, bytes)) return 0;
   Table t;
-  if (small_list(ntensor, h_ptrs, h_numel, h_types, t)) return 0;
+  if (small_list(ntensor, h_ptrs, h_numel, h_types, SMALL_CLIP, t)) return 0;   // (the smaller of the two)
   return total_chunks(ntensor, h_ptrs, h_numel, h_types, chunk_bytes(bytes));
 }
 
@@ -501,7 +502,7 @@ extern "C" int vca_grad_norm(int ntensor, const void* const* h_ptrs, const long 
   VCA_CHECK_ARG(out && list_ok(ntensor, h_ptrs, h_numel, h_types, bytes));
   hipStream_t s = (hipStream_t)stream;
   Table t;
-  if (small_list(ntensor, h_ptrs, h_numel, h_types, t)) {
+  if (small_list(ntensor, h_ptrs, h_numel, h_types, SMALL_NORM, t)) {
     hipLaunchKernelGGL(norm_small_kernel<false>, dim3(1), dim3(SMALL_WAVES * 64), 0, s, t, 0.f, scale, out);
     return vca_launch_status();
   }
@@ -519,7 +520,7 @@ extern "C" int vca_grad_clip(int ntensor, const void* const* h_ptrs, const long 
   VCA_CHECK_ARG(out && max_norm >= 0.f && list_ok(ntensor, h_ptrs, h_numel, h_types, bytes));
   hipStream_t s = (hipStream_t)stream;
   Table t;
-  if (small_list(ntensor, h_ptrs, h_numel, h_types, t)) {
+  if (small_list(ntensor, h_ptrs, h_numel, h_types, SMALL_CLIP, t)) {
     hipLaunchKernelGGL(norm_small_kernel<true>, dim3(1), dim3(SMALL_WAVES * 64), 0, s, t, max_norm, scale, out);
     return vca_launch_status();
   }
