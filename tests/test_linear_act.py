@@ -326,6 +326,28 @@ def test_direct_gradients_and_input_grads_only():
 
 
 @gpu
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+@pytest.mark.parametrize('M,K,N', [(60, 64, 48), (600, 600, 600), (300, 1111, 77), (100, 1000, 4000), (1024, 1024, 1024)])
+def test_each_gradient_is_the_same_whichever_are_wanted(M, K, N, dtype):
+    """dx and dw by one launch or by their own, and with an operand that starts off the other's alignment."""
+    from vcagan_amd import ops
+    x, w, b, _, gy = _inputs(M, K, N, TYPES[dtype], 12)
+    want = _reference(x, w, b, None, gy, 'silu', 'fp32')
+    shifted = torch.empty(M * K + 1, dtype=x.dtype, device='cuda')[1:].view(M, K).copy_(x)
+    for x1 in (x, shifted):
+        x1 = x1.detach().requires_grad_(True)
+        w1, b1 = w.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        grads = lambda *leaves: torch.autograd.grad(ops.linear_act(x1, w1, b1, act='silu'), leaves, gy)
+        gx, gw, gb = grads(x1, w1, b1)
+        for g, n in ((gx, 'dx'), (gw, 'dw'), (gb, 'db')):
+            _check(g, want[n], (n, M, K, N))
+        assert torch.equal(grads(x1)[0], gx) and torch.equal(grads(w1)[0], gw) and torch.equal(grads(b1)[0], gb)
+        x2 = x1.detach()
+        gw2, gb2 = torch.autograd.grad(ops.linear_act(x2, w1, b1, act='silu'), (w1, b1), gy)
+        assert torch.equal(gw2, gw) and torch.equal(gb2, gb)
+
+
+@gpu
 def test_streams_and_graph_replay():
     """Forward and backward captured together and replayed on new inputs beside eager work of the same shapes."""
     from vcagan_amd import ops

@@ -239,7 +239,7 @@ struct Operand {
   static constexpr int PIECES = (R * 8 + NT - 1) / NT;    // 16-byte pieces a thread stages (the last one: some waves)
   __device__ __forceinline__ static bool mine(int it, int thread) { return R * 8 % NT == 0 || it * NT + thread < R * 8; }
   static constexpr int PPR = R * ESZ / 16;                // pieces of a row of k (index contiguous)
-  const char* src[PIECES];                                // this thread's pieces of the next chunk to fetch (DMA)
+  const char* src[PIECES];                                // this thread's pieces of chunk 0 (DMA)
   const char* base;
   long long ldb;                                          // bytes
   int o0, outer, K, tid;
@@ -264,33 +264,28 @@ struct Operand {
     tid = tid_;
   }
 
-  // addresses of the first chunk's pieces, clamped into the operand (rows and columns of C beyond its edge are computed
-  // from repeated values and never stored)
-  __device__ __forceinline__ void start(int c) {
+  // addresses of chunk 0's pieces, clamped into the operand (rows and columns of C beyond its edge are computed from
+  // repeated values and never stored)
+  __device__ __forceinline__ void start() {
 #pragma unroll
     for (int it = 0; it < PIECES; ++it) {
       int row, pc;
       piece(it, row, pc);
-      if (KC) src[it] = base + (long long)min(o0 + row, outer - 1) * ldb + (long long)c * 128 + pc * 16;
-      else src[it] = base + (long long)(c * BK + row) * ldb + (long long)min(o0 + pc * EPP, outer - EPP) * ESZ;
+      if (KC) src[it] = base + (long long)min(o0 + row, outer - 1) * ldb + pc * 16;
+      else src[it] = base + (long long)row * ldb + (long long)min(o0 + pc * EPP, outer - EPP) * ESZ;
     }
   }
 
-  __device__ __forceinline__ void dma(char* stage) {
+  __device__ __forceinline__ void dma(char* stage, int c) {      // (a chunk's distance is uniform: no state but src)
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const long long at = c * (KC ? 128ll : BK * ldb);
 #pragma unroll
     for (int it = 0; it < PIECES; ++it) {
       if (!mine(it, wave * 64)) continue;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[it],
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[it] + at),
                                        (__attribute__((address_space(3))) void*)(stage + (it * NT + wave * 64) * 16), 16,
                                        0, 0);
-      src[it] += KC ? 128ll : BK * ldb;
     }
-  }
-
-  __device__ __forceinline__ void back(int chunks) {       // from the end of the whole chunks to their first
-#pragma unroll
-    for (int it = 0; it < PIECES; ++it) src[it] -= chunks * (KC ? 128ll : BK * ldb);
   }
 
   __device__ __forceinline__ void fetch(int c, uint4 (&r)[PIECES]) const {
@@ -377,8 +372,7 @@ __device__ __forceinline__ void frag_split(const char* s, int sub, int lc, int g
 
 // Workgroup -> tile.  Consecutive workgroups go to the 8 XCDs in turn; each XCD gets a contiguous range of the tiles,
 // and those run through groups of 8 tile rows column by column, so the tiles an XCD's L2 holds share operands.
-__device__ __forceinline__ void tile_of(const MatArgs& g, int& tm, int& tn, int& kz) {
-  const int total = gridDim.x, id = blockIdx.x;
+__device__ __forceinline__ void tile_of(const MatArgs& g, int id, int total, int& tm, int& tn, int& kz) {
   const int x = id & 7, per = total >> 3, rem = total & 7;
   int t = x * per + min(x, rem) + (id >> 3);
   const int tiles = g.ntm * g.ntn;
@@ -459,7 +453,7 @@ __device__ __forceinline__ void store_tile(const MatArgs& g, const f32x4 (&acc)[
 
 template <int MODE, bool AKC, bool BKC, int BM, int BN, int NWM, int NWN, bool DMA, int STAGES,
           bool TURN>
-__global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g) {
+__device__ __forceinline__ void product_block(const MatArgs& g, int id, int total) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typedef typename ElemOf<MODE>::T T;
   constexpr int NT = NWM * NWN * 64, BK = 128 / (int)sizeof(T);
@@ -469,7 +463,7 @@ __global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g)
   const int lc = lane & 15, lg = lane >> 4;
   const int wm = wave / NWN, wn = wave % NWN;
   int tm, tn, kz;
-  tile_of(g, tm, tn, kz);
+  tile_of(g, id, total, tm, tn, kz);
   const int m0 = tm * BM, n0 = tn * BN;
   const int c0 = kz * g.cpz, c1 = min((g.K + BK - 1) / BK, c0 + g.cpz);
   const int whole = DMA ? max(c0, min(c1, g.K / BK)) : c0;   // chunks [c0, whole) travel by DMA, the rest through registers
@@ -541,17 +535,14 @@ __global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g)
     // rows lie a power of two apart, few of the memory's channels are asked at a time (4096 -> 16384 in bf16, 8 rows 29.8 ->
     // 25.8 us, 64 rows 31.6 -> 27.5; with less than half the CUs at work it changes nothing).
     const int turn = TURN ? tn % (whole - c0) : 0;
-    A.start(c0 + turn);
-    B.start(c0 + turn);
+    A.start();
+    B.start();
     static_assert((STAGES & (STAGES - 1)) == 0, "");
     auto stage = [&](int c) { return smem + ((c - c0) & (STAGES - 1)) * STAGE; };
     auto send = [&](int c) {
-      if (TURN && c == whole - turn) {
-        A.back(whole - c0);
-        B.back(whole - c0);
-      }
-      A.dma(stage(c));
-      B.dma(stage(c) + BM * 128);
+      const int k = !TURN ? c : c + turn < whole ? c + turn : c + turn - (whole - c0);
+      A.dma(stage(c), k);
+      B.dma(stage(c) + BM * 128, k);
     };
     for (int c = c0; c < min(whole, c0 + STAGES - 1); ++c) send(c);
     for (int c = c0; c < whole; ++c) {
@@ -586,6 +577,18 @@ __global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g)
   }
 
   store_tile<T, BM, BN, NWM, NWN>(g, acc, smem, m0, n0, kz, wm, wn, lc, lg, tid);
+}
+
+template <int MODE, bool AKC, bool BKC, int BM, int BN, int NWM, int NWN, bool DMA, int STAGES, bool TURN>
+__global__ __launch_bounds__(NWM * NWN * 64) void matmul_kernel(const MatArgs g) {
+  product_block<MODE, AKC, BKC, BM, BN, NWM, NWN, DMA, STAGES, TURN>(g, blockIdx.x, gridDim.x);
+}
+
+// dx = dz W and dW = dz^T x in one launch, by 64 x 64 tiles: workgroups [0, first) take dx.
+template <int MODE, bool DMA>
+__global__ __launch_bounds__(256) void matmul_pair_kernel(const MatArgs x, const MatArgs w, int first) {
+  if ((int)blockIdx.x < first) product_block<MODE, true, false, 64, 64, 2, 2, DMA, 2, false>(x, blockIdx.x, first);
+  else product_block<MODE, false, false, 64, 64, 2, 2, DMA, 2, false>(w, blockIdx.x - first, gridDim.x - first);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -640,7 +643,7 @@ __global__ __launch_bounds__(512) void matmul_wide_kernel(const MatArgs g) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lc = lane & 15, lg = lane >> 4, wm = wave >> 2, wn = wave & 3;
   int tm, tn, kz;
-  tile_of(g, tm, tn, kz);
+  tile_of(g, blockIdx.x, gridDim.x, tm, tn, kz);
   const int m0 = tm * BM, n0 = tn * BM;
   const int c0 = kz * g.cpz, c1 = min((g.K + 63) / 64, c0 + g.cpz), whole = max(c0, min(c1, g.K / 64));
 
@@ -988,6 +991,7 @@ struct Plan {
   int mode, bm, bn;                   // the tile; 0: few rows
   bool dma, wide, low, tall;          // may be taken: the 256-wide tiles, the 32-row ones and four stages, those with more
                                       // rows than columns
+  bool pair;                          // only the 64 x 64 tiles may
 };
 
 // Rows of x times bytes of W up to which few_rows_kernel takes a product of at most 16 rows: every workgroup of 16 columns
@@ -1023,7 +1027,7 @@ bool pick(Plan& p, int nc) {
   double best = 0.;
   p.bm = 0;
   for (const TileCost& t : COST[p.mode]) {
-    if (!t.bm || (t.bm == 256 && !p.wide) || (t.bm == 32 && !(p.low && g.M <= 32)) || (t.bm > t.bn && !p.tall)) continue;
+    if (!t.bm || (p.pair && t.bm != 64) || (t.bm == 256 && !p.wide) || (t.bm == 32 && !(p.low && g.M <= 32)) || (t.bm > t.bn && !p.tall)) continue;
     const long long tiles = ((g.M + (long long)t.bm - 1) / t.bm) * ((g.N + (long long)t.bn - 1) / t.bn);
     if (tiles >= (1 << 24)) continue;
     const double wait = t.wait * (p.low && g.M <= 64 && t.bm == 64 && p.mode == MODE_16 ? 0.75 : 1.);   // (four stages)
@@ -1049,10 +1053,11 @@ bool pick(Plan& p, int nc) {
   return true;
 }
 
-int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p) {
+int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p, bool pair = false) {
   VCA_CHECK_ARG(dp);
   const vca_matmul_desc& d = *dp;
   p.mode = mode_of(d);
+  p.pair = pair;
   VCA_CHECK_ARG(p.mode >= 0 && d.M > 0 && d.N > 0 && d.K > 0 && act_ok(d.act));
   VCA_CHECK_ARG(d.M <= (1 << 30) && d.N <= (1 << 30) && d.K <= (1 << 30));   // (tile edges stay in an int)
   VCA_CHECK_ARG(!(d.a_col && !d.b_col));                   // no product here reads only its rows by columns
@@ -1169,10 +1174,11 @@ long long ws_floats_of(const vca_matmul_desc* d) {
   long long n = 0;
   const int nc = (p.g.K * (d->type == VCA_T_F32 ? 4ll : 2ll) + 127) / 128;
   const bool low = d->M <= LOW_ROWS && !d->a_col && !d->b_col;
-  for (int form = 0; form < 3; ++form) {                   // not by DMA, by DMA, and with the 256-wide tiles
-    p.low = form && low;
-    p.tall = form && !d->a_col;
+  for (int form = 0; form < 4; ++form) {                   // not by DMA, by DMA, with the 256-wide tiles, in a pair
+    p.low = (form == 1 || form == 2) && low;
+    p.tall = (form == 1 || form == 2) && !d->a_col;
     p.wide = form == 2 && p.mode == MODE_16;
+    p.pair = form == 3;
     if (pick(p, nc) && ws_of(p) > n) n = ws_of(p);
   }
   return n;
@@ -1186,10 +1192,7 @@ bool aligned(int type, std::initializer_list<const void*> ps) {
   return (bits & (type == VCA_T_F32 ? 3 : 1)) == 0;
 }
 
-// The product itself: into C, or into its partial products in ws where the plan splits it.
-int launch_product(Plan& p, const vca_matmul_desc& d, const void* a, const void* b, const void* bias, const void* res,
-                   void* c, void* z, float* ws, hipStream_t s) {
-  MatArgs& g = p.g;
+void bind(MatArgs& g, const void* a, const void* b, const void* bias, const void* res, void* c, void* z, float* ws) {
   g.a = a;
   g.b = b;
   g.bias = bias;
@@ -1197,6 +1200,13 @@ int launch_product(Plan& p, const vca_matmul_desc& d, const void* a, const void*
   g.c = c;
   g.z = z;
   g.part = g.ksplit > 1 ? ws : nullptr;
+}
+
+// The product itself: into C, or into its partial products in ws where the plan splits it.
+int launch_product(Plan& p, const vca_matmul_desc& d, const void* a, const void* b, const void* bias, const void* res,
+                   void* c, void* z, float* ws, hipStream_t s) {
+  MatArgs& g = p.g;
+  bind(g, a, b, bias, res, c, z, ws);
   const bool ac = d.a_col != 0, bc = d.b_col != 0;
   if (p.bm == 0) {
     const dim3 grid((g.N + 15) / 16, g.ksplit);
@@ -1209,6 +1219,52 @@ int launch_product(Plan& p, const vca_matmul_desc& d, const void* a, const void*
     case MODE_F32: return launch_mode<MODE_F32>(p, ac, bc, s);
     case MODE_S3: return launch_mode<MODE_S3>(p, ac, bc, s);
     default: return launch_mode<MODE_S1>(p, ac, bc, s);
+  }
+}
+
+int grid_of(const Plan& p) { return p.g.ntm * p.g.ntn * p.g.ksplit; }
+
+// Whether both products of a backward pass go by one launch, side by side instead of one after the other (us, one launch and
+// two, with dz and db: bf16 300 x 512 x 512 11.6 / 16.2, 1801 x 1111 x 677 43 / 57; fp32 1000^3 52 / 63, 5000 x 1111 x 1333
+// 377 / 373).
+bool in_pair(const Plan& x, const Plan& w) {
+  return x.bm == 64 && x.bn == 64 && w.bm == 64 && w.bn == 64 && x.dma == w.dma && grid_of(x) <= (1 << 22) &&
+         grid_of(w) <= (1 << 22);
+}
+
+// Plans of both.  Other tiles are given up for one launch if the whole of it fits the CUs at once (600^3 fp32 27.3 -> 23.6;
+// 4800 x 512 x 1280, 1080 workgroups, would go 137 -> 157).  Both products are always planned, wanted or not, so that dx
+// does not depend on whether dW is formed too.
+int plan_pair(const vca_linear_bwd& b, const vca_matmul_desc& x, const vca_matmul_desc& w, const void* dz, Plan& px, Plan& pw) {
+  const int ex = plan_of(&x, dz, b.w, px), ew = plan_of(&w, dz, b.x, pw);
+  if (ex && b.dx) return ex;
+  if (ew && b.dw) return ew;
+  if (ex || ew || in_pair(px, pw)) return 0;
+  Plan qx, qw;
+  if (plan_of(&x, dz, b.w, qx, true) || plan_of(&w, dz, b.x, qw, true)) return 0;
+  if (in_pair(qx, qw) && grid_of(qx) + grid_of(qw) <= 512) {
+    px = qx;
+    pw = qw;
+  }
+  return 0;
+}
+
+template <int MODE>
+int launch_pair_mode(const Plan& x, const Plan& w, hipStream_t s) {
+  const int first = grid_of(x);
+  const dim3 grid(first + grid_of(w));
+  constexpr int LDS = 2 * 128 * 128;
+  if (x.dma) hipLaunchKernelGGL((matmul_pair_kernel<MODE, true>), grid, dim3(256), LDS, s, x.g, w.g, first);
+  else hipLaunchKernelGGL((matmul_pair_kernel<MODE, false>), grid, dim3(256), LDS, s, x.g, w.g, first);
+  return vca_launch_status();
+}
+
+int launch_pair(const Plan& x, const Plan& w, hipStream_t s) {
+  switch (x.mode) {
+    case MODE_16: return launch_pair_mode<MODE_16>(x, w, s);
+    case MODE_F32: return launch_pair_mode<MODE_F32>(x, w, s);
+    case MODE_S3: return launch_pair_mode<MODE_S3>(x, w, s);
+    default: return launch_pair_mode<MODE_S1>(x, w, s);
   }
 }
 
@@ -1316,13 +1372,11 @@ extern "C" int vca_linear_act_bwd(const vca_linear_bwd* b, float* ws, long long 
   const void* dz = b->dz ? b->dz : b->gy;
   Plan px, pw;
   px.g.ksplit = pw.g.ksplit = 1;
-  if (b->dx) {
-    const int rc = plan_of(&x, dz, b->w, px);
+  if (b->dx || b->dw) {
+    const int rc = plan_pair(*b, x, w, dz, px, pw);
     if (rc) return rc;
-  }
-  if (b->dw) {
-    const int rc = plan_of(&w, dz, b->x, pw);
-    if (rc) return rc;
+    if (!b->dx) px.g.ksplit = 1;                           // (nothing of it to add up)
+    if (!b->dw) pw.g.ksplit = 1;
   }
   // one part of the workspace for each of db, dx and dw, so that what is split is added up by one launch at the end
   const long long at_x = b->db ? up4(act_bwd_ws(b->type, b->M, b->N)) : 0;
@@ -1333,7 +1387,14 @@ extern "C" int vca_linear_act_bwd(const vca_linear_bwd* b, float* ws, long long 
   clear(f);
   int e = 0;
   if (b->dz || b->db) e = act_bwd(b->type, b->M, b->N, b->act, b->slope, b->gy, b->z, b->dz, b->db, b->db_add, ws, f, s);
-  if (!e && b->dx) e = launch_product(px, x, dz, b->w, nullptr, nullptr, b->dx, nullptr, ws + at_x, s);
-  if (!e && b->dw) e = launch_product(pw, w, dz, b->x, nullptr, b->dw_add ? b->dw : nullptr, b->dw, nullptr, ws + at_w, s);
+  const void* old = b->dw_add ? b->dw : nullptr;
+  if (!e && b->dx && b->dw && in_pair(px, pw)) {
+    bind(px.g, dz, b->w, nullptr, nullptr, b->dx, nullptr, ws + at_x);
+    bind(pw.g, dz, b->x, nullptr, old, b->dw, nullptr, ws + at_w);
+    e = launch_pair(px, pw, s);
+  } else {
+    if (!e && b->dx) e = launch_product(px, x, dz, b->w, nullptr, nullptr, b->dx, nullptr, ws + at_x, s);
+    if (!e && b->dw) e = launch_product(pw, w, dz, b->x, nullptr, old, b->dw, nullptr, ws + at_w, s);
+  }
   return e ? e : launch_folds(f, px.g.ksplit > 1 ? &px.g : nullptr, pw.g.ksplit > 1 ? &pw.g : nullptr, b->type, s);
 }
