@@ -1167,14 +1167,14 @@ long long ws_of(const Plan& p) {
 }
 
 // Workspace floats of a product whatever its operands' alignment and strides, so that a caller may ask once a size.
-long long ws_floats_of(const vca_matmul_desc* d) {
+long long ws_floats_of(const vca_matmul_desc* d, bool pair) {
   Plan p;
   if (plan_of(d, nullptr, nullptr, p) != 0) return 0;
   if (!p.bm) return ws_of(p);
   long long n = 0;
   const int nc = (p.g.K * (d->type == VCA_T_F32 ? 4ll : 2ll) + 127) / 128;
   const bool low = d->M <= LOW_ROWS && !d->a_col && !d->b_col;
-  for (int form = 0; form < 4; ++form) {                   // not by DMA, by DMA, with the 256-wide tiles, in a pair
+  for (int form = 0; form < 3 + pair; ++form) {                   // not by DMA, by DMA, with the 256-wide tiles, in a pair
     p.low = (form == 1 || form == 2) && low;
     p.tall = (form == 1 || form == 2) && !d->a_col;
     p.wide = form == 2 && p.mode == MODE_16;
@@ -1301,7 +1301,7 @@ int act_rows(int M, int N, int esz) {                     // rows a workgroup of
 }  // namespace
 
 extern "C" long long vca_matmul_act_ws_floats(const vca_matmul_desc* d) {
-  return ws_floats_of(d);
+  return ws_floats_of(d, false);
 }
 
 extern "C" int vca_matmul_act(const vca_matmul_desc* d, const void* a, const void* b, const void* bias, const void* res,
@@ -1360,7 +1360,7 @@ static long long up4(long long n) { return (n + 3) / 4 * 4; }   // each part of 
 extern "C" long long vca_linear_act_bwd_ws_floats(const vca_linear_bwd* b) {
   if (!b || b->M <= 0 || b->N <= 0 || b->K <= 0) return 0;
   const vca_matmul_desc x = bwd_dx(*b), w = bwd_dw(*b);
-  return up4(act_bwd_ws(b->type, b->M, b->N)) + up4(ws_floats_of(&x)) + ws_floats_of(&w);
+  return up4(act_bwd_ws(b->type, b->M, b->N)) + up4(ws_floats_of(&x, true)) + ws_floats_of(&w, true);
 }
 
 extern "C" int vca_linear_act_bwd(const vca_linear_bwd* b, float* ws, long long ws_floats, void* stream) {
