@@ -850,8 +850,8 @@ def _at(t):
 
 
 def _linear_act_fwd(x, w, bias, res, code, z=None):
-    (M, K), N, dt, dev = x.shape, w.shape[0], x.dtype, x.device
-    y = torch.empty((M, N), device=dev, dtype=dt)
+    (M, K), N, dt = x.shape, w.shape[0], x.dtype
+    y = x.new_empty((M, N))
     L = _lib.lib(_ELEM_OF[dt])
     ns = _nsplit() if dt == torch.float32 else 1
     d = _lib.pack_matmul(M, N, K, _lib.TYPES[dt], ns, 0, 0, code[0], code[1], _row_step(x), _row_step(w), N,
@@ -860,7 +860,7 @@ def _linear_act_fwd(x, w, bias, res, code, z=None):
     n = _act_ws.get(key)
     if n is None:
         n = _act_ws[key] = int(L.vca_matmul_act_ws_floats(d))
-    ws = torch.empty(n, device=dev, dtype=torch.float32) if n else None
+    ws = x.new_empty(n, dtype=torch.float32) if n else None
     check(L.vca_matmul_act(d, x.data_ptr(), w.data_ptr(), _at(bias), _at(res), y.data_ptr(), _at(z), _at(ws), n, stream()),
           'matmul_act')
     return y
@@ -874,7 +874,7 @@ class LinearActFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         z = None
         if code[0] != ACT_NONE and (need[0] or need[1] or need[2]):
-            z = torch.empty((x.shape[0], w.shape[0]), device=x.device, dtype=_KEPT_IN[x.dtype])
+            z = x.new_empty((x.shape[0], w.shape[0]), dtype=_KEPT_IN[x.dtype])
         ctx.save_for_backward(x, w, z)
         ctx.code, ctx.bias_param = code, bias
         return _linear_act_fwd(x, w, bias, res, code, z)
@@ -896,26 +896,30 @@ def _linear_act_bwd(ctx, gy):
         need_w = need_b = False
     if not (need_x or need_w or need_b):
         return None, None, None, gy if need_r else None, None
-    (M, K), N, dt, dev = x.shape, w.shape[0], x.dtype, x.device
+    (M, K), N, dt = x.shape, w.shape[0], x.dtype
     g = gy.contiguous()
     wsink = _grad_sink(w) if need_w else None
     bsink = _grad_sink(ctx.bias_param) if need_b else None
     L = _lib.lib(_ELEM_OF[dt])
     ns = _nsplit(True) if dt == torch.float32 else 1
     code = ctx.code
-    dz = torch.empty((M, N), device=dev, dtype=dt) if z is not None and (need_x or need_w) else None
-    gx = torch.empty((M, K), device=dev, dtype=dt) if need_x else None
-    gw = (torch.empty((N, K), device=dev, dtype=dt) if wsink is None else wsink) if need_w else None
-    gb = (torch.empty(N, device=dev, dtype=dt) if bsink is None else bsink) if need_b else None
-    d = _lib.pack_linear_bwd(M, N, K, _lib.TYPES[dt], ns, code[0], wsink is not None, bsink is not None, code[1],
-                             _row_step(x), _row_step(w), g.data_ptr(), x.data_ptr(), w.data_ptr(), _at(z), _at(dz),
-                             _at(gx), _at(gw), _at(gb))
+    gx = g.new_empty((M, K)) if need_x else None
+    gw = (g.new_empty((N, K)) if wsink is None else wsink) if need_w else None
+    gb = (g.new_empty(N) if bsink is None else bsink) if need_b else None
     key = (M, N, K, dt, ns, 'bwd')
     n = _act_ws.get(key)
     if n is None:
+        d = _lib.pack_linear_bwd(M, N, K, _lib.TYPES[dt], ns, code[0], 0, 0, code[1], _row_step(x), _row_step(w),
+                                 *[0] * 8)
         n = _act_ws[key] = int(L.vca_linear_act_bwd_ws_floats(d))
-    ws = torch.empty(n, device=dev, dtype=torch.float32)
-    check(L.vca_linear_act_bwd(d, ws.data_ptr(), n, stream()), 'linear_act_bwd')
+    # dz and the workspace behind it, each from a 16-byte boundary
+    nz = (M * N * g.element_size() + 15) // 16 * 4 if z is not None and (need_x or need_w) else 0
+    ws = g.new_empty(nz + n, dtype=torch.float32)
+    at = ws.data_ptr()
+    d = _lib.pack_linear_bwd(M, N, K, _lib.TYPES[dt], ns, code[0], wsink is not None, bsink is not None, code[1],
+                             _row_step(x), _row_step(w), g.data_ptr(), x.data_ptr(), w.data_ptr(), _at(z),
+                             at if nz else 0, _at(gx), _at(gw), _at(gb))
+    check(L.vca_linear_act_bwd(d, at + 4 * nz if n else 0, n, stream()), 'linear_act_bwd')
     return gx, gw if wsink is None else None, gb if bsink is None else None, gy if need_r else None, None
 
 
