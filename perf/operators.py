@@ -24,29 +24,29 @@ NORM_EPS = 1e-6
 def listed():
     return [
         # one time step of a 512-wide layer, the width of the visual features: the smallest call, latency only
-        _linear('linear one row', 1, 512, 512, 'fp32', 'tanh', True, False, False),
+        _linear('linear, one row', 1, 512, 512, 'fp32', 'tanh', True, False, False),
         # a few tokens of a wide feed-forward layer when serving: bound by reading the weights once
-        _linear('linear 8 rows wide', 8, 4096, 16384, 'bf16', 'gelu', True, False, False),
+        _linear('linear, 8 rows wide', 8, 4096, 16384, 'bf16', 'gelu', True, False, False),
         # 32 clips x 75 frames through a 2560 -> 512 projection (the attention's query width), inference
-        _linear('linear 2400 frames', 2400, 2560, 512, 'fp32', 'leaky0.2', True, True, False),
+        _linear('linear, 2400 frames', 2400, 2560, 512, 'fp32', 'leaky0.2', True, True, False),
         # the 512 -> 1280 output projection on padded 150-frame clips, trained in exact fp32
-        _linear('linear fp32 training', 4800, 512, 1280, 'fp32', 'relu', True, True, True),
+        _linear('linear, fp32 training', 4800, 512, 1280, 'fp32', 'relu', True, True, True),
         # every size odd: valid frames of ragged clips gathered into rows, half precision
-        _linear('linear odd sizes', 1801, 1111, 677, 'fp16', 'silu', True, True, True),
+        _linear('linear, odd sizes', 1801, 1111, 677, 'fp16', 'silu', True, True, True),
         # the largest: a feed-forward layer over 8192 tokens, forward and all gradients
-        _linear('linear bf16 training', 8192, 4096, 4096, 'bf16', 'gelu', True, True, True),
+        _linear('linear, bf16 training', 8192, 4096, 4096, 'bf16', 'gelu', True, True, True),
         # gradients of a small head: few values, latency only
-        _tensors('norm', 'norm small head', 6, 5000, 'fp32', False),
+        _tensors('norm', 'norm, small head', 6, 5000, 'fp32', False),
         # gradients of a billion parameters in few large 16-bit buckets
-        _tensors('norm', 'norm bf16 buckets', 9, 1000000007, 'bf16', False),
+        _tensors('norm', 'norm, bf16 buckets', 9, 1000000007, 'bf16', False),
         # the generator side's 246 parameter tensors, 52 M values, each padded to four values in one flat buffer
-        _tensors('clip', 'clip generator side', 246, 51810275, 'fp32', True),
+        _tensors('clip', 'clip, generator side', 246, 51810275, 'fp32', True),
         # odd tensors packed without padding (starts off any vector's alignment), 16- and 32-bit types mixed
-        _tensors('clip', 'clip odd mixed types', 61, 3141593, 'mixed', False),
+        _tensors('clip', 'clip, odd mixed types', 61, 3141593, 'mixed', False),
         # a small network's update: latency only
-        _adam('adam small network', 1, 100000, False),
+        _adam('adam, small network', 1, 100000, False),
         # the generator side's update with its three flat buffers
-        _adam('adam generator side', 3, 51810276, True),
+        _adam('adam, generator side', 3, 51810276, True),
     ]
 
 
