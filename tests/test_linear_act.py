@@ -253,6 +253,59 @@ def test_values_that_are_not_finite_stay_in_their_rows(dtype):
     assert bool(y[149].isnan().all()) and bool((y[3].isinf() | (y[3] == r[3])).all())
 
 
+# rows through each form of the product: the few-row kernel, the small tiles, split reductions, the tall ones' rows and the
+# 256-wide tiles, with columns that end inside a tile
+KINKED = [(3, 64, 40), (70, 48, 90), (129, 4100, 67), (1801, 128, 680), (3500, 136, 4001)]
+
+
+@gpu
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16'])
+@pytest.mark.parametrize('act', ['relu', 'leaky0.2'])
+@pytest.mark.parametrize('M,K,N', KINKED)
+def test_kinked_slopes_of_small_values(M, K, N, act, dtype):
+    """Pre-activations of either sign around 2^-60, far below half's range but well inside that of fp32 and bf16.  Each row
+    of w has one entry, +-1, and each x is a power of two, so z is exact and the slopes are known: dx and db (sums of at
+    most M slopes that are multiples of an ulp of 0.2f: M u of them) and dw (powers of two of one sign a column times
+    slopes) come out within their summation and one rounding."""
+    from vcagan_amd import ops
+    t = TYPES[dtype]
+    g = torch.Generator().manual_seed(M)
+    x = torch.ldexp(torch.ones(M, K), torch.randint(-62, -58, (M, K), generator=g))
+    x = (x * torch.where(torch.rand(M, K, generator=g) < 0.5, -1.0, 1.0)).to(t).cuda()
+    w = torch.zeros(N, K)
+    w[torch.arange(N), torch.randint(0, K, (N,), generator=g)] = torch.where(torch.rand(N, generator=g) < 0.5, -1.0, 1.0)
+    w = w.to(t).cuda()
+    gy = torch.randint(1, 4, (M, N), generator=g).to(t).cuda()
+    leaves = [v.requires_grad_(True) for v in (x, w, torch.zeros(N, dtype=t).cuda())]
+    y = ops.linear_act(*leaves, act=act)
+    got = torch.autograd.grad(y, leaves, gy)
+    X, W, G = x.detach().double(), w.detach().double(), gy.double()
+    z = _mm(X, W.t())
+    low = 0.0 if act == 'relu' else 0.2
+    e = torch.finfo(t).eps / 2
+    assert bool((z != 0).all()) and bool(((y.detach().double() - torch.where(z > 0, z, low * z)).abs() <= e * z.abs()).all())
+    dz = G * torch.where(z > 0, 1.0, low)
+    D = dz * (1 + 2 * e)                                   # the slope 0.2f and dz, each rounded once
+    for v, want, size, terms in ((got[0], _mm(dz, W), _mm(D, W.abs()), N), (got[1], _mm(dz.t(), X), _mm(D.t(), X.abs()), M),
+                                 (got[2], dz.sum(0), D.sum(0), M)):
+        assert bool(((v.double() - want).abs() <= (2 * e + (terms + 8) * U) * size + e * want.abs()).all()), act
+
+
+@gpu
+@pytest.mark.parametrize('act,low', [('relu', 0.0), ('leaky0.2', 0.2)])
+def test_slopes_at_every_magnitude(act, low):
+    """One power of two a row, of both signs, from the smallest normal bf16 value to past the end of half's range."""
+    from vcagan_amd import ops
+    for name, bottom in (('bf16', -126), ('fp16', -24), ('fp32', -126)):
+        t = TYPES[name]
+        mag = 2.0 ** torch.arange(bottom, 16, dtype=torch.float64)
+        z = torch.cat([mag, -mag, mag * 0])
+        x = z.to(t).cuda()[:, None].requires_grad_(True)
+        y = ops.linear_act(x, torch.ones(1, 1, dtype=t).cuda(), act=act)
+        gx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert torch.equal(gx[:, 0].cpu(), torch.where(z > 0, 1.0, low).to(t)), name
+
+
 @gpu
 def test_slopes_far_out():
     """The smooth activations' slopes reach 0 and 1 far from the origin instead of 0 x infinity."""

@@ -25,8 +25,9 @@ template <int MODE> struct ElemOf { typedef float T; };
 template <> struct ElemOf<MODE_16> { typedef vca_e16 T; };
 
 // What the value under the activation is kept in for the backward pass.  Its rounding enters dz next to dz's own, so it
-// has to be the smaller of the two: three more bits than bf16 in the same room (the slopes are 0, 1 or flat long before
-// half's range ends, an infinity included), fp32 beside half.
+// has to be the smaller of the two: three more bits than bf16 in the same room, fp32 beside half.  Half's range is
+// narrower than bf16's at both ends.  At the upper one the slopes are 0, 1 or flat, an infinity included.  At the lower
+// one the smooth slopes are flat too, but the kinked ones turn on the sign, so a positive value stays positive (keep_z).
 #ifdef VCA_E16_FP16
 typedef float vca_z16;
 #else
@@ -187,6 +188,21 @@ __device__ __forceinline__ AnyVec<T, V> res_of(const MatArgs& g, int m, int n) {
   return q;
 }
 
+// The V values under the activation as they are kept: where relu or leaky will read no more than their sign out of half
+// (see ZOf), a positive one is at least half's smallest, which rounding to nearest would take to zero up to 2^-25.
+template <typename Z, int V>
+__device__ __forceinline__ void keep_z(const MatArgs& g, int m, int n, const float (&v)[V]) {
+  Z* p = reinterpret_cast<Z*>(g.z) + (size_t)m * g.N + n;
+  if (sizeof(Z) == 2 && (g.act == VCA_ACT_RELU || g.act == VCA_ACT_LEAKY)) {
+    float k[V];
+#pragma unroll
+    for (int r = 0; r < V; ++r) k[r] = v[r] > 0.f ? fmaxf(v[r], 0x1p-24f) : v[r];
+    store_any<Z, V>(p, g.N - n, k);
+  } else {
+    store_any<Z, V>(p, g.N - n, v);
+  }
+}
+
 // Bias, activation and residual of V neighbouring columns n .. n + V - 1 of row m; stores y and, if kept, z.
 template <typename T, int V>
 __device__ __forceinline__ void finish(const MatArgs& g, int m, int n, float (&v)[V], const AnyVec<T, V>& bias,
@@ -196,8 +212,7 @@ __device__ __forceinline__ void finish(const MatArgs& g, int m, int n, float (&v
 #pragma unroll
     for (int r = 0; r < V; ++r) v[r] += (float)bias.e[r];
   }
-  typedef typename ZOf<T>::type Z;
-  if (g.z) store_any<Z, V>(reinterpret_cast<Z*>(g.z) + (size_t)m * g.N + n, left, v);
+  if (g.z) keep_z<typename ZOf<T>::type, V>(g, m, n, v);
   act_all(v, g.act, g.slope);
   if (g.res) {
 #pragma unroll

@@ -836,7 +836,8 @@ def _rows_2d(t, broadcast=False):
 
 
 _ELEM_OF = {torch.float32: None, torch.bfloat16: 'bf16', torch.float16: 'fp16'}   # 16-bit products are compiled per type
-# what the value under the activation is kept in: rounded less than dz, next to whose rounding its own comes
+# what the value under the activation is kept in: rounded less than dz, next to whose rounding its own comes (half keeps the
+# sign of every bf16 value that relu or leaky's slope turns on: the kernels lift a positive one to half's smallest)
 _KEPT_IN = {torch.float32: torch.float32, torch.bfloat16: torch.float16, torch.float16: torch.float32}
 _act_ws = {}     # sizes and types of a forward or backward pass -> workspace floats
 
