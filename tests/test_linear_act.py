@@ -307,6 +307,23 @@ def test_slopes_at_every_magnitude(act, low):
 
 
 @gpu
+@pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
+def test_slopes_at_a_nan(dtype):
+    """torch's: relu hands the incoming gradient on, leaky scales it, the smooth ones' gradients are NaN."""
+    from vcagan_amd import ops
+    t = TYPES[dtype]
+    z = torch.tensor([math.nan, 1.0, -1.0], dtype=t)
+    for act, fn in ACTS.items():
+        x, ref = (z.clone().cuda()[:, None].requires_grad_(True) for _ in range(2))
+        gy = torch.tensor([3.0, 5.0, 7.0], dtype=t).cuda()[:, None]
+        got, = torch.autograd.grad(ops.linear_act(x, torch.ones(1, 1, dtype=t).cuda(), act=act), x, gy)
+        want, = torch.autograd.grad(fn(ref), ref, gy)
+        assert torch.equal(got.isnan(), want.isnan()), act
+        if act in (None, 'relu', 'leaky0.2'):
+            assert torch.equal(got, want), act
+
+
+@gpu
 def test_slopes_far_out():
     """The smooth activations' slopes reach 0 and 1 far from the origin instead of 0 x infinity."""
     from vcagan_amd import ops

@@ -113,12 +113,12 @@ __device__ __forceinline__ void act_all(float (&v)[V], int act, float slope) {
 }
 
 __device__ __forceinline__ float act_slope(float z, int act, float slope) {
-  // beyond +-60 the smooth activations' slopes are 0 or 1 to fp32; the clamp keeps 0 x infinity out of them (a NaN
-  // comes through the unclamped term)
+  // beyond +-60 the smooth activations' slopes are 0 or 1 to fp32; the clamp keeps 0 x infinity out of them.  At a NaN
+  // they are one (it comes through the unclamped term), relu's is 1 and leaky's its slope, as torch's are.
   const float c = fminf(fmaxf(z, -60.f), 60.f);
   switch (act) {
     case VCA_ACT_LEAKY: return z > 0.f ? 1.f : slope;
-    case VCA_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+    case VCA_ACT_RELU: return z <= 0.f ? 0.f : 1.f;
     case VCA_ACT_TANH: {
       const float h = tanhf(z);
       return 1.f - h * h;
