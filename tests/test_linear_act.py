@@ -418,6 +418,27 @@ def test_each_gradient_is_the_same_whichever_are_wanted(M, K, N, dtype):
 
 
 @gpu
+def test_forward_mode_is_refused_and_traces_keep_the_call():
+    """A tangent is never dropped without a word, whichever input carries it and with or without gradients enabled, and
+    a trace replays the operator on new inputs instead of the traced call's result."""
+    from torch.autograd import forward_ad
+    from vcagan_amd import ops
+    args = _inputs(4, 8, 5, torch.float32, 1)[:4]
+    for i in range(4):
+        for grad in (True, False):
+            with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                dual = [forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(args)]
+                with pytest.raises(NotImplementedError):
+                    ops.linear_act(*dual[:3], act='silu', residual=dual[3])
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: ops.linear_act(x, args[1]), (args[0],), (args[0],))
+    f = torch.jit.trace(lambda x: ops.linear_act(x, *args[1:3], act='silu'), args[0], check_trace=False)
+    for s in (2, 3):
+        x = _inputs(4, 8, 5, torch.float32, s)[0]
+        assert torch.equal(f(x), ops.linear_act(x, *args[1:3], act='silu'))
+
+
+@gpu
 def test_streams_and_graph_replay():
     """Forward and backward captured together and replayed on new inputs beside eager work of the same shapes."""
     from vcagan_amd import ops
