@@ -323,6 +323,34 @@ def test_slopes_at_a_nan(dtype):
             assert torch.equal(got, want), act
 
 
+def _act64(act, z):
+    """(value, slope) of the smooth activations in 64 bits, from the side that does not cancel; on the CPU."""
+    if act == 'gelu':
+        phi = 0.5 * torch.special.erfc(-z / math.sqrt(2.0))
+        return z * phi, phi + z * torch.exp(-0.5 * z * z) / math.sqrt(2.0 * math.pi)
+    c, a = math.sqrt(2.0 / math.pi), 0.044715
+    k, dk = (z, torch.ones_like(z)) if act == 'silu' else (2 * c * (z + a * z ** 3), 2 * c * (1 + 3 * a * z * z))
+    s = 1.0 / (1.0 + torch.exp(-k))
+    return z * s, s + z * dk * s / (1.0 + torch.exp(k))
+
+
+@gpu
+@pytest.mark.parametrize('dtype', ['bf16', 'fp16'])
+@pytest.mark.parametrize('act', ['gelu', 'gelu_tanh', 'silu'])
+def test_small_values_of_the_activations_keep_their_digits(act, dtype):
+    """Far out on the negative side the value is a small product, not a difference: y is off by one rounding to its type (and
+    half's subnormals), and by the fp32 evaluation's share: at most 16 u, and 6 u of the exponential's argument k (its terms,
+    and the factor log2 e), |k| <= 88."""
+    from vcagan_amd import ops
+    t = TYPES[dtype]
+    z = torch.linspace({'gelu': -13.0, 'gelu_tanh': -9.0, 'silu': -80.0}[act], 9.0, 100001).to(t).unique()
+    y = ops.linear_act(z.cuda()[:, None], torch.ones(1, 1, dtype=t).cuda(), act=act).double().cpu()[:, 0]
+    want = _act64(act, z.double())[0]
+    f = torch.finfo(t)
+    tol = want.abs() * (f.eps / 2 + (16 + 6 * 88) * U) + f.smallest_normal * f.eps / 2
+    assert bool(((y - want).abs() <= tol).all()), z[(y - want).abs() > tol]
+
+
 @gpu
 def test_slopes_far_out():
     """The smooth activations' slopes reach 0 and 1 far from the origin instead of 0 x infinity."""

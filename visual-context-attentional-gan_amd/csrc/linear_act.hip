@@ -67,14 +67,24 @@ __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp
 // 1 / (1 + e^-x): the hardware's exponential and reciprocal, each within an ulp or two; 0 and 1 at the ends
 __device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.f + fast_exp(-x)); }
 
-// e = exp(-z^2 / 2) and erfc(|z| / sqrt 2) by Abramowitz & Stegun 7.1.26 (five-term polynomial in 1 / (1 + p x) times
-// e, off by at most 1.5e-7): a dozen instructions where erff takes four times as many, and at 33 M values that is
-// 30 us of the 8192 x 4096 forward pass
-__device__ __forceinline__ float erfc_half(float z, float& e) {
-  const float x = fabsf(z) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
-  e = fast_exp(-x * x);
-  return t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * e;
+// e = exp(-z^2 / 2) and Phi(-|z|), the normal distribution's tail, as t P(t) e with t = 1 / (1 + 0.26 |z|).  P was fitted for
+// this file: least squares on 6000 Chebyshev nodes of t, reweighted until the relative error is level, 3.2e-8 over
+// |z| <= 15, behind which the tail is below fp32.  Evaluated in fp32, t P(t) is within 12 half ulps wherever the tail lies,
+// so gelu keeps its digits far out on the negative side, for about half of erff's instructions.
+__device__ __forceinline__ float normal_tail(float z, float& e) {
+  const float a = fabsf(z) > 15.f ? 15.f : fabsf(z);       // (a NaN stays one)
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.26f * a);
+  e = fast_exp(-0.5f * a * a);
+  float p = 0.029960118f;
+  p = p * t - 0.15018713f;
+  p = p * t + 0.2460446f;
+  p = p * t - 0.1447271f;
+  p = p * t + 0.15665133f;
+  p = p * t + 0.052859996f;
+  p = p * t + 0.10256f;
+  p = p * t + 0.10308303f;
+  p = p * t + 0.10375513f;
+  return t * p * e;
 }
 
 __device__ __forceinline__ float act_f(float z, int act, float slope) {
@@ -84,7 +94,7 @@ __device__ __forceinline__ float act_f(float z, int act, float slope) {
     case VCA_ACT_TANH: return tanhf(z);
     case VCA_ACT_GELU: {                                     // z Phi(z); the small tail is multiplied, never subtracted
       float e;
-      const float q = 0.5f * erfc_half(z, e);
+      const float q = normal_tail(z, e);
       return z * (z > 0.f ? 1.f - q : q);
     }
     case VCA_ACT_GELU_TANH: return z * sigmoid_f(2.f * GELU_C * (z + GELU_A * z * z * z));   // (1 + tanh u) / 2
@@ -125,7 +135,7 @@ __device__ __forceinline__ float act_slope(float z, int act, float slope) {
     }
     case VCA_ACT_GELU: {
       float e;
-      const float q = 0.5f * erfc_half(z, e);
+      const float q = normal_tail(z, e);
       return (z > 0.f ? 1.f - q : q) + c * e * 0.3989422804014327f;
     }
     case VCA_ACT_GELU_TANH: {
