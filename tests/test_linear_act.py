@@ -352,6 +352,35 @@ def test_small_values_of_the_activations_keep_their_digits(act, dtype):
 
 
 @gpu
+@pytest.mark.parametrize('act', ['gelu', 'gelu_tanh', 'silu'])
+def test_fp32_activations_are_as_good_as_fp32(act):
+    """Value and slope of fp32 tensors against 64 bits, relative to their terms.  The exponential is good to 2 u and its
+    argument k to 6 u |k| (silu's and gelu's exactly); the rest: sigmoid 8 u, its slope d = s (1 - s) 14 u; the normal tail
+    7 u for its polynomial, 3.1 x 2 u for the reciprocal it is taken at, 2 u for e; 1 - q and the product with z 1 u each."""
+    from vcagan_amd import ops
+    z = torch.linspace({'gelu': -12.5, 'gelu_tanh': -9.5, 'silu': -85.0}[act], 9.0, 300001).unique()
+    x = z.cuda()[:, None].requires_grad_(True)
+    y = ops.linear_act(x, torch.ones(1, 1).cuda(), act=act)
+    gx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    y, gx, z = y.detach()[:, 0].cpu().double(), gx[:, 0].cpu().double(), z.double()
+    want, slope = _act64(act, z)
+    own = torch.where(slope.abs() < 0.25, 2 * slope.abs(), 1.0)      # the last sum's rounding, of a value at most 1.13
+    if act == 'gelu':
+        phi = want.abs() / z.abs()
+        phi[z == 0] = 0.5
+        of_value, of_slope = 20.0, 20 * phi + 10 * (slope - phi).abs() + own
+    else:
+        k = torch.zeros_like(z) if act == 'silu' else 1.6 * (z + 0.044715 * z ** 3).abs()
+        s = want.abs() / z.abs()
+        s[z == 0] = 0.5
+        of_value, of_slope = 10 + 6 * k, (9 + 6 * k) * s + (20 + 6 * k) * (slope - s).abs() + own
+    off, tol = (y - want).abs(), of_value * U * want.abs()
+    assert bool((off <= tol).all()), float((off - tol).max())
+    off = (gx - slope).abs() - of_slope * U
+    assert bool((off <= 0).all()), (z[off > 0], off[off > 0])
+
+
+@gpu
 def test_slopes_far_out():
     """The smooth activations' slopes reach 0 and 1 far from the origin instead of 0 x infinity."""
     from vcagan_amd import ops
