@@ -75,6 +75,36 @@ def test_norm_and_clip(sizes, offset, dtypes):
 
 
 @gpu
+@pytest.mark.parametrize('count', [2040, 2048, 2049, 5000])
+def test_lists_of_thousands(count):
+    """Below, at and above the number of partial sums that a launch of its own adds up, eagerly and replayed on other
+    values beside eager calls: the norm has the bits of the norm alone, and every tensor is scaled once."""
+    from vcagan_amd import ops
+    sizes = [1 + (37 * i) % 900 for i in range(count)]
+    ts = _list(sizes, (torch.float32, torch.bfloat16, torch.float16), 8, 1)
+    plan = ops.GradNorm(ts)
+    plan.norm()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        replayed = plan.clip_(0.5)
+    values = torch.randn(sum(sizes), generator=torch.Generator().manual_seed(1)).cuda()
+    for rep in range(4):
+        for t, v in zip(ts, (values * (rep + 1)).split(sizes)):       # (the types differ: one by one)
+            t.copy_(v)
+        before = [t.clone() for t in ts]
+        want, alone = _norm64(ts), plan.norm()
+        if rep == 0:
+            norm = float(plan.clip_(0.5))
+        else:
+            graph.replay()
+            torch.cuda.synchronize()
+            norm = float(replayed)
+        assert norm == float(alone) and abs(norm - want) <= want * (F32 + 2.0 ** -30), rep
+        _check_clipped(ts, before, 0.5 / (want + 1e-6))
+
+
+@gpu
 @pytest.mark.parametrize('scale', [1e-30, 1e-22, 1e18, 1e30])
 def test_norm_of_values_whose_squares_leave_the_fp32_range(scale):
     from vcagan_amd import ops

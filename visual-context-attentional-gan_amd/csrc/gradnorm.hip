@@ -24,6 +24,11 @@ constexpr long long MIN_CHUNK = 16384;   // bytes: four 16-byte loads a thread
 constexpr int FUSED_PARTS = 256;         // partial sums up to which the Adam update adds them up itself: one a thread.
                                          // 1 M values 10.8 us, with a launch of its own for that 11.5; 25 M (1500 sums, read
                                          // by 6000 workgroups): 140 and 136
+// Partial sums up to which every workgroup of the clipping launch adds them up itself: as many as a list has whose tensors are
+// few.  Every tensor brings at least one more, so for long lists the sums would be quadratic work.  us, each workgroup and by
+// a launch of its own (norm included): 246 tensors, 1968 sums, 207 MB 49.3 / 49.7; tensors of 500 values: 1000 41.2 / 40.4,
+// 3000 116 / 95, 10000 553 / 300, 20000 1732 / 728.
+constexpr int CLIP_PARTS = MAX_CHUNKS;
 constexpr int SMALL_WAVES = 16;
 constexpr long long SMALL_CHUNK = 4096;  // bytes a wave takes at a time in the single-workgroup form
 // Chunks up to which one workgroup does everything; us, one workgroup and two launches, norm: 64 KB 3.2 / 4.6, 128 KB
@@ -250,8 +255,15 @@ __global__ __launch_bounds__(THR) void norm_fold_kernel(const double* __restrict
   if (threadIdx.x == 0) out[0] = (float)true_norm(total, scale);
 }
 
-// Every workgroup adds up the slots itself (at most some 2200 values out of L2, under the time of one more launch)
-// and scales its chunk; with a factor of one there is nothing to do.  Chunks are taken from the last to the first: the
+// The sum of a long list's slots into the first of them: all have been read behind the sum's barrier.
+__global__ __launch_bounds__(THR) void norm_total_kernel(double* __restrict__ ws, int n) {
+  __shared__ double part[THR / 64];
+  const double total = fold(ws, n, part);
+  if (threadIdx.x == 0) ws[0] = total;
+}
+
+// Every workgroup adds up the slots itself (out of L2, under the time of one more launch; n is 1 for a list whose tensors
+// are so many that norm_total_kernel has done it, CLIP_PARTS) and scales its chunk; with a factor of one there is nothing to do.  Chunks are taken from the last to the first: the
 // norm's pass left the end of the list in the caches (400 MB 192 us, from the first 200).  Bound by memory: norm and
 // clipping of 207 MB together 119 us, 5.2 TB/s of the 621 MB read and written.
 __global__ __launch_bounds__(THR) void clip_chunks_kernel(const Table t, const double* __restrict__ ws, int n,
@@ -527,6 +539,10 @@ extern "C" int vca_grad_clip(int ntensor, const void* const* h_ptrs, const long 
   int parts = 0;
   const int rc = norm_partials(false, ntensor, h_ptrs, h_numel, h_types, bytes, ws, ws_doubles, s, parts);
   if (rc) return rc;
+  if (parts > CLIP_PARTS) {
+    hipLaunchKernelGGL(norm_total_kernel, dim3(1), dim3(THR), 0, s, ws, parts);
+    parts = 1;
+  }
   const long long chunk = chunk_bytes(bytes);
   bool first = true;
   for (int end = ntensor; end > 0;) {                    // tables from the end of the list backwards
