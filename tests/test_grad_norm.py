@@ -166,6 +166,22 @@ def test_the_memory_of_a_list_stays_when_a_tensor_gets_other_data():
 
 
 @gpu
+def test_shared_memory_is_that_of_the_list_not_of_its_tensors_later():
+    from vcagan_amd import ops
+    a = torch.randn(1000).cuda()
+    n = ops.GradNorm([a, a[100:200]])
+    n.tensors[1].data = torch.zeros(100, device='cuda')
+    with pytest.raises(ValueError):
+        n.clip_(1.0)
+    a, b = (torch.randn(1000).cuda() for _ in range(2))
+    before = [a.clone(), b.clone()]
+    n, old = ops.GradNorm([a, b]), b.detach()
+    b.data = a
+    n.clip_(1.0)
+    _check_clipped([a, old], before, 1.0 / (_norm64(before) + 1e-6))
+
+
+@gpu
 def test_elements_beyond_32_bits():
     from vcagan_amd import ops
     n = 2 ** 31 + 12345

@@ -2363,8 +2363,8 @@ class GradNorm:
     def clip_(self, max_norm, scaler=None):
         """Scale every tensor in place by min(1, max_norm / (norm + 1e-6)) and return the norm."""
         max_norm = _max_norm(max_norm)
-        if self._disjoint is None:
-            at = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in self.tensors if t.numel())
+        if self._disjoint is None:                     # of the memory recorded, whatever the tensors have by now
+            at = sorted((p, n * (2 if k else 4)) for p, n, k in zip(self._ptrs, self._numel, self._types) if n)
             self._disjoint = all(a + n <= b for (a, n), (b, _) in zip(at, at[1:]))
         if not self._disjoint:
             raise ValueError('GradNorm.clip_: two of the tensors share memory (the same gradient twice?)')
