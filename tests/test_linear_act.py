@@ -496,6 +496,26 @@ def test_forward_mode_is_refused_and_traces_keep_the_call():
 
 
 @gpu
+def test_ragged_batches_keep_a_bounded_number_of_sizes(monkeypatch):
+    """A row count of its own in every call: what is remembered of them stays bounded, and forgetting changes nothing."""
+    from vcagan_amd import ops
+    monkeypatch.setattr(ops, '_act_ws', {})
+    x, w, b, _, _ = _inputs(300, 1200, 70, torch.float32, 3)
+    x.requires_grad_(True)
+
+    def one(m):
+        y = ops.linear_act(x[:m], w, b, act='silu')
+        return y.detach(), torch.autograd.grad(y, x, torch.ones_like(y))[0]
+    want = [one(m) for m in range(1, 300, 7)]
+    assert len(ops._act_ws) == 2 * len(want)
+    monkeypatch.setattr(ops, '_act_ws', {})
+    monkeypatch.setattr(ops, '_ACT_WS_KEPT', 16)
+    for m, (y, gx) in zip(range(1, 300, 7), want):
+        got = one(m)
+        assert torch.equal(got[0], y) and torch.equal(got[1], gx) and len(ops._act_ws) <= 16
+
+
+@gpu
 def test_streams_and_graph_replay():
     """Forward and backward captured together and replayed on new inputs beside eager work of the same shapes."""
     from vcagan_amd import ops
@@ -640,6 +660,13 @@ def test_packed_structures_are_the_declared_ones():
     assert bytes(_lib.MatmulDesc(*v)) == _lib.pack_matmul(*v)
     v = [3, 5, 7, 1, 1, 6, 1, 0, 0.25, 11, 13, 64, 128, 192, 0, 320, 384, 448, 512]
     assert bytes(_lib.LinearBwd(*[None if x == 0 and i > 10 else x for i, x in enumerate(v)])) == _lib.pack_linear_bwd(*v)
+
+
+def test_remembered_workspace_sizes_are_bounded(monkeypatch):
+    from vcagan_amd import ops
+    monkeypatch.setattr(ops, '_act_ws', {})
+    for m in range(3 * ops._ACT_WS_KEPT):
+        assert ops._keep_ws((m, 5), m) == m and ops._act_ws[(m, 5)] == m and len(ops._act_ws) <= ops._ACT_WS_KEPT
 
 
 def test_refusals_without_a_gpu():

@@ -841,6 +841,14 @@ _ELEM_OF = {torch.float32: None, torch.bfloat16: 'bf16', torch.float16: 'fp16'} 
 # sign of every bf16 value that relu or leaky's slope turns on: the kernels lift a positive one to half's smallest)
 _KEPT_IN = {torch.float32: torch.float32, torch.bfloat16: torch.float16, torch.float16: torch.float32}
 _act_ws = {}     # sizes and types of a forward or backward pass -> workspace floats
+_ACT_WS_KEPT = 4096     # of them: batches with a row count of their own every step would never stop adding
+
+
+def _keep_ws(key, floats):
+    if len(_act_ws) >= _ACT_WS_KEPT:
+        _act_ws.clear()                                                 # (asking again costs a few microseconds)
+    _act_ws[key] = floats
+    return floats
 
 
 def _row_step(t):
@@ -861,7 +869,7 @@ def _linear_act_fwd(x, w, bias, res, code, z=None):
     key = (M, N, K, dt, ns)
     n = _act_ws.get(key)
     if n is None:
-        n = _act_ws[key] = int(L.vca_matmul_act_ws_floats(d))
+        n = _keep_ws(key, int(L.vca_matmul_act_ws_floats(d)))
     ws = x.new_empty(n, dtype=torch.float32) if n else None
     check(L.vca_matmul_act(d, x.data_ptr(), w.data_ptr(), _at(bias), _at(res), y.data_ptr(), _at(z), _at(ws), n, stream()),
           'matmul_act')
@@ -913,7 +921,7 @@ def _linear_act_bwd(ctx, gy):
     if n is None:
         d = _lib.pack_linear_bwd(M, N, K, _lib.TYPES[dt], ns, code[0], 0, 0, code[1], _row_step(x), _row_step(w),
                                  *[0] * 8)
-        n = _act_ws[key] = int(L.vca_linear_act_bwd_ws_floats(d))
+        n = _keep_ws(key, int(L.vca_linear_act_bwd_ws_floats(d)))
     # dz and the workspace behind it, each from a 16-byte boundary
     nz = (M * N * g.element_size() + 15) // 16 * 4 if z is not None and (need_x or need_w) else 0
     ws = g.new_empty(nz + n, dtype=torch.float32)
