@@ -340,6 +340,43 @@ def test_adam_with_clipping_and_scaler_skips_an_overflow():
 
 
 @gpu
+@pytest.mark.parametrize('amsgrad', [False, True])
+@pytest.mark.parametrize('sizes', [[4096, 400], [3000000, 1200004]])
+@pytest.mark.parametrize('bad', [math.inf, math.nan, 'flag'])
+def test_adam_with_clipping_and_scaler_skips_in_both_forms(bad, sizes, amsgrad):
+    """Few partial sums (every workgroup adds them up) and many (a launch of its own): a gradient that is not finite, in the
+    first or the last group, or a flag that is already up beside finite gradients, changes nothing but the flag; the
+    other side's flag, the scale and the step count stay, and the step after it counts from there."""
+    from vcagan_amd import ops
+    opt, groups, ref = _adam_pair(sizes, amsgrad, 4)
+    sc = ops.LossScaler(groups[0][0].device, init_scale=8.0)
+
+    def good(t):
+        want = _norm64([g for _, g in groups]) / 8.0
+        norm = opt.step(sc, 0, max_norm=want / 2)
+        assert abs(float(norm) - want) <= want * (F32 + 2.0 ** -30) and int(opt.t_dev) == t
+        for r, (_, g) in zip(ref, groups):
+            r.step(g, t, 1e-3, 1e-2, (want / 2) / (want + 1e-6) / 8.0)
+        _check_adam(opt, groups, ref)
+    good(1)
+    state = lambda: [f for f, _ in groups] + [st[k] for st in opt.state for k in ('m', 'v', 'vmax') if st[k] is not None]
+    kept = [t.clone() for t in state()]
+    for k, at in ((0, 0), (1, sizes[1] - 1)):
+        was = groups[k][1][at].clone()
+        if bad == 'flag':
+            sc.state[1] = 1
+        else:
+            groups[k][1][at] = bad
+        norm = float(opt.step(sc, 0, max_norm=1.0))
+        assert math.isfinite(norm) if bad == 'flag' else math.isnan(norm) if bad != bad else norm == math.inf
+        assert [int(v) for v in sc.state[1:3]] == [1, 0] and int(opt.t_dev) == 1 and sc.value == 8.0
+        assert all(torch.equal(a, b) for a, b in zip(kept, state()))
+        groups[k][1][at] = was
+        sc.state[1] = 0
+    good(2)
+
+
+@gpu
 def test_adam_with_clipping_under_graph_replay():
     opt, groups, ref = _adam_pair([70000, 400], True, 3)
     opt.step(max_norm=5.0)

@@ -158,6 +158,17 @@ def test_fp32_sizes_between_the_tiles(M, K, N, mode):
 
 
 @gpu
+@pytest.mark.parametrize('act', ['relu', 'leaky0.2'])
+@pytest.mark.parametrize('M,K,N,dtype,mode', [
+    (2400, 2560, 512, 'fp32', 'fp32'), (4800, 512, 1280, 'fp32', 'fp32'), (4800, 1280, 512, 'fp32', 'fp32'),
+    (900, 700, 1300, 'fp32', 'fp32'), (2400, 2560, 512, 'fp32', 'bf16x3'), (4800, 512, 1280, 'fp32', 'bf16x3'),
+    (4800, 516, 1280, 'fp32', 'fp16x3'), (4800, 512, 1280, 'fp32', 'mixed'), (4096, 128, 4096, 'bf16', 'fp32'),
+    (3500, 136, 4001, 'bf16', 'fp32'), (4104, 200, 4000, 'fp16', 'fp32')])
+def test_kinked_activations_through_the_tall_and_the_large_tiles(M, K, N, dtype, mode, act):
+    _run(M, K, N, TYPES[dtype], act, 13, mode)
+
+
+@gpu
 @pytest.mark.parametrize('dtype', ['fp32', 'bf16', 'fp16'])
 @pytest.mark.parametrize('act', list(ACTS))
 def test_activations(act, dtype):
