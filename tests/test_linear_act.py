@@ -639,6 +639,66 @@ def test_a_training_step_of_the_operators_together():
 
 
 @gpu
+def test_each_step_of_the_operators_together():
+    """The same network, every step against 64 bits from the parameters and moments the step before it left, so that no
+    deviation feeds back.  A gradient is off by at most 4e-5 of its tensor's largest value (three products in a row of at
+    most 96 terms, each 104 u of the sum of its terms' magnitudes, itself at most twice the largest), the norm by 4e-5 of
+    itself, and the moments and the update follow to first order: with eg the error of c g,
+      m  0.1 eg + 3 u (|0.9 m| + |0.1 c g|)        v  0.002 |c g| eg + 0.001 eg^2 + 4 u v
+      p  lr' (em / den + |m| ev / (2 sqrt(v) root) / den^2) x 1.5 + 6 u |update| + 2 u |p|
+    where v is at least four times its error; that has to be nearly everywhere."""
+    from vcagan_amd import ops
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            g = torch.Generator().manual_seed(5)
+            self.w1 = torch.nn.Parameter(torch.randn(96, 64, generator=g) / 8)
+            self.b1 = torch.nn.Parameter(torch.randn(96, generator=g) / 8)
+            self.w2 = torch.nn.Parameter(torch.randn(64, 96, generator=g) / 10)
+            self.b2 = torch.nn.Parameter(torch.randn(64, generator=g) / 8)
+    net = Net().cuda()
+    (flat, grad), = groups = [ops.flatten_module(net)]
+    opt = ops.FusedAdam(groups, lr=1e-3)
+    near = 0
+    for t in (1, 2, 3):
+        g = torch.Generator().manual_seed(10 + t)
+        x, gy = (torch.randn(80, 64, generator=g).cuda() for _ in range(2))
+        p, m, v = (a.double().clone() for a in (flat, opt.state[0]['m'], opt.state[0]['v']))
+        rp = [q.detach().double().requires_grad_(True) for q in net.parameters()]
+        F.linear(F.gelu(F.linear(x.double(), rp[0], rp[1])), rp[2], rp[3]).backward(gy.double())
+        opt.zero_grad()
+        with ops.direct_param_grad():
+            ops.linear_act(ops.linear_act(x, net.w1, net.b1, act='gelu'), net.w2, net.b2, residual=x).backward(gy)
+        g64, eg = torch.zeros_like(p), torch.zeros_like(p)
+        for q, r in zip(net.parameters(), rp):
+            at = (q.data_ptr() - flat.data_ptr()) // 4
+            g64[at:at + q.numel()] = r.grad.reshape(-1)
+            eg[at:at + q.numel()] = 4e-5 * float(r.grad.abs().max())
+        assert bool(((grad.double() - g64).abs() <= eg).all())
+        total = float(g64.pow(2).sum().sqrt())
+        norm = opt.step(max_norm=total * 0.3 * t)              # in force every step, by a factor of its own
+        assert abs(float(norm) - total) <= 4e-5 * total
+        c = min(1.0, total * 0.3 * t / (total + 1e-6))
+        g64, eg = c * g64, c * (eg + 4e-5 * g64.abs())
+        em = 0.1 * eg + 3 * U * (0.9 * m.abs() + 0.1 * g64.abs())
+        m = 0.9 * m + 0.1 * g64
+        v = 0.999 * v + 0.001 * g64 * g64
+        ev = 0.002 * g64.abs() * eg + 0.001 * eg * eg + 4 * U * v
+        st = opt.state[0]
+        assert bool(((st['m'].double() - m).abs() <= em).all()) and bool(((st['v'].double() - v).abs() <= ev).all())
+        rate, root = 1e-3 / (1 - 0.9 ** t), math.sqrt(1 - 0.999 ** t)
+        den = v.sqrt() / root + 1e-8
+        upd = rate * m / den
+        tol = (1.5 * rate * (em / den + m.abs() * ev / (2 * v.sqrt() * root).clamp_min(1e-30) / den ** 2) +
+               6 * U * upd.abs() + 2 * U * p.abs())
+        sure = (4 * ev <= v) | (v == 0)                        # (v == 0: the padding)
+        near += int((~sure).sum())
+        assert bool(((flat.double() - (p - upd)).abs() <= tol)[sure].all())
+    assert near <= 0.01 * flat.numel()
+
+
+@gpu
 def test_refusals_on_device_tensors():
     from vcagan_amd import ops
     x, w, b, r, _ = _inputs(6, 12, 8, torch.float32, 0)
