@@ -464,6 +464,32 @@ def test_refusals_on_device_tensors():
         opt.step(max_norm=1.0)
 
 
+class _PlainOptimizer:
+    """An optimizer with the training step's interface from before there was any clipping."""
+
+    def __init__(self):
+        self.all_grads = torch.zeros(8)
+        self.flats, self.calls = {}, []
+
+    def step(self, scaler=None, side=0):
+        self.calls.append((scaler, side))
+        return 'ignored'
+
+
+def _gan_step(**kw):
+    from vcagan_amd import train_step
+    g, d = _PlainOptimizer(), _PlainOptimizer()
+    return train_step.GanStep({}, (g, d), 'grid', **kw), g, d
+
+
+def test_gan_step_without_clipping_calls_its_optimizers_as_before():
+    step, g, d = _gan_step()
+    step._st = dict(g3=torch.zeros(1))
+    out = step.finish()
+    assert g.calls == [(None, 1)] and set(out) == {'g3'}
+    assert step._update(d, 0, step.d_max_norm) is None and d.calls == [(None, 0)]
+
+
 def test_refusals_of_lists():
     from vcagan_amd import ops
     with pytest.raises(ValueError):

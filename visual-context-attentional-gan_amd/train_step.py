@@ -185,6 +185,13 @@ class GanStep:
                 main.wait_stream(st)
         ops.join_side_streams()
 
+    def _update(self, opt, side, max_norm):
+        """One side's optimizer step; its gradients' norm where they are clipped.  Without clipping the optimizer is called as
+        ever, step(scaler, side), so one that knows nothing of max_norm goes on working."""
+        if max_norm is not None:
+            return opt.step(self.scaler, side, max_norm)
+        opt.step(self.scaler, side)
+
     def _zero(self, names):
         """Clear the flat gradients of the named networks; whole sides (contiguous buffers) with one fill."""
         names = tuple(names)
@@ -340,7 +347,7 @@ class GanStep:
         """d_optimizer.step(), the generator losses and their backward pass; with overlap the pass ends at the phoneme
         features and g_trunk() takes it through the visual front-end."""
         m, st = self.m, self._st
-        d_norm = self.d_opt.step(self.scaler, 0, self.d_max_norm)
+        d_norm = self._update(self.d_opt, 0, self.d_max_norm)
         g1, g2, g3 = st['g']
         phon, sd, T = st['phon'], st['sd'], st['T']
         dis = (m['dis1'], m['dis2'], m['dis3'])
@@ -414,7 +421,7 @@ class GanStep:
 
     def finish(self):
         """g_optimizer.step() (train.py:236); returns the step's losses and outputs."""
-        g_norm = self.g_opt.step(self.scaler, 1, self.g_max_norm)
+        g_norm = self._update(self.g_opt, 1, self.g_max_norm)
         if g_norm is not None:
             self._st['g_norm'] = g_norm
         if self.scaler is not None:
