@@ -490,6 +490,15 @@ def test_gan_step_without_clipping_calls_its_optimizers_as_before():
     assert step._update(d, 0, step.d_max_norm) is None and d.calls == [(None, 0)]
 
 
+def test_gan_step_refuses_a_bound_when_it_is_built():
+    for bad in (-1.0, math.nan, (1.0, -2.0), [math.nan, None], (1.0,), (1.0, 2.0, 3.0)):
+        with pytest.raises(ValueError):
+            _gan_step(max_norm=bad)
+    step, _, _ = _gan_step(max_norm=(2, None))
+    assert (step.g_max_norm, step.d_max_norm) == (2.0, None)
+    assert _gan_step(max_norm=0.5)[0].d_max_norm == 0.5
+
+
 def test_refusals_of_lists():
     from vcagan_amd import ops
     with pytest.raises(ValueError):

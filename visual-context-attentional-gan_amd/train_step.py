@@ -147,7 +147,10 @@ class GanStep:
         if scaler is None and ops.half_gradients():
             scaler = ops.LossScaler(next(models['gen'].parameters()).device)
         self.scaler = scaler
-        self.g_max_norm, self.d_max_norm = max_norm if isinstance(max_norm, (tuple, list)) else (max_norm, max_norm)
+        pair = max_norm if isinstance(max_norm, (tuple, list)) else (max_norm, max_norm)
+        if len(pair) != 2:
+            raise ValueError('GanStep: max_norm is a number or a pair (generator side, discriminator side), got %r' % (max_norm,))
+        self.g_max_norm, self.d_max_norm = (None if v is None else ops._max_norm(v) for v in pair)
         if dist.is_available() and dist.is_initialized():
             ops.set_seed(torch.initial_seed(), dist.get_rank(group))   # each replica draws its own dropout masks
 
