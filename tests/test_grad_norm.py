@@ -377,6 +377,22 @@ def test_adam_with_clipping_and_scaler_skips_in_both_forms(bad, sizes, amsgrad):
 
 
 @gpu
+def test_clipped_adam_refuses_groups_that_share_parameters():
+    """The groups are updated by one launch: a buffer that is in two of them would be written by both at once."""
+    from vcagan_amd import ops
+    f, g = torch.ones(64).cuda(), torch.ones(64).cuda()
+    for groups in ([(f, g), (f, g)], [(f[:32], g[:32]), (f[16:48], g[16:48])], [(f[32:], g[32:]), (f, g)]):
+        opt = ops.FusedAdam(groups)
+        with pytest.raises(ValueError):
+            opt.step(max_norm=1.0)
+        assert int(opt.t_dev) == 0 and opt.t == 0 and bool((f == 1).all())
+    opt = ops.FusedAdam([(f[32:], g[32:]), (f[:32], g[:32])])                   # neighbours; gradients may be shared
+    assert abs(float(opt.step(max_norm=1.0)) - 8.0) <= 1e-6 and bool((f != 1).all())
+    opt = ops.FusedAdam([(f[32:], g[:32]), (f[:32], g[:32])])
+    assert abs(float(opt.step(max_norm=1.0)) - 8.0) <= 1e-6
+
+
+@gpu
 def test_adam_with_clipping_under_graph_replay():
     opt, groups, ref = _adam_pair([70000, 400], True, 3)
     opt.step(max_norm=5.0)

@@ -2514,6 +2514,10 @@ class FusedAdam:
     def _clipped(self, scaler, side, max_norm):
         L = _lib.lib()
         n = len(self.groups)
+        if n > 1:
+            at = sorted((f.data_ptr(), 4 * f.numel()) for f, _ in self.groups)
+            if any(a + size > b for (a, size), (b, _) in zip(at, at[1:])):        # (one launch updates all groups at once)
+                raise ValueError('FusedAdam.step: max_norm with groups that share parameters')
         tab = (_lib.AdamGroup * n)(*[(ptr(f), ptr(g), ptr(st['m']), ptr(st['v']), ptr(st['vmax']), f.numel())
                                      for (f, g), st in zip(self.groups, self.state)])
         nws = int(L.vca_grad_norm_ws_doubles(n, None, None, None))
