@@ -4,12 +4,12 @@
 //   c    = min(1, max_norm / (norm + 1e-6))           (a NaN norm gives a NaN factor, an infinite one the factor 0)
 //   clip:  g <- c g          Adam:  g' = c g / loss scale + wd p, then the usual moments and update
 //
-// All of it streams memory: the norm reads every byte once, clipping reads again and writes, the update reads p, g, m,
-// v (, vmax) and writes all but g.  Squares and sums are held in fp64: one conversion and one fp64 FMA per value are far
-// below what the vector units can do while the value arrives from HBM, no square over- or underflows for any fp32
-// gradient (so the sum is finite exactly when every gradient is, which the loss scaler's overflow test uses), and the
-// result is the exact sum to fp64 rounding.  No atomics: a list is cut into chunks, every chunk's sum goes to its own
-// workspace slot and the slots are added in a fixed order, so equal inputs give equal bits.
+// All of it streams memory: the norm reads every byte once, clipping reads again and writes, the update reads p, g,
+// m, v (, vmax) and writes all but g.  Squares and sums are held in fp64: one conversion and one fp64 FMA per value
+// are far below what the vector units can do while the value arrives from HBM, no square over- or underflows for any
+// fp32 gradient (so the sum is finite exactly when every gradient is, which the loss scaler's overflow test uses),
+// and the result is the exact sum to fp64 rounding.  No atomics: a list is cut into chunks, every chunk's sum goes to
+// its own workspace slot and the slots are added in a fixed order, so equal inputs give equal bits.
 //
 // The tensor table travels in the kernel arguments (TABLE tensors a launch), so nothing has to be uploaded, kept alive
 // or invalidated, and a captured launch carries its own copy.
@@ -22,12 +22,13 @@ constexpr int THR = 256;
 constexpr int MAX_CHUNKS = 2048;      // chunks a list is cut into, not counting each tensor's last one: 8 workgroups a CU
 constexpr long long MIN_CHUNK = 16384;   // bytes: four 16-byte loads a thread
 constexpr int FUSED_PARTS = 256;         // partial sums up to which the Adam update adds them up itself: one a thread.
-                                         // 1 M values 10.8 us, with a launch of its own for that 11.5; 25 M (1500 sums, read
-                                         // by 6000 workgroups): 140 and 136
-// Partial sums up to which every workgroup of the clipping launch adds them up itself: as many as a list has whose tensors are
-// few.  Every tensor brings at least one more, so for long lists the sums would be quadratic work.  us, each workgroup and by
-// a launch of its own (norm included): 246 tensors, 1968 sums, 207 MB 49.3 / 49.7; tensors of 500 values: 1000 41.2 / 40.4,
-// 3000 116 / 95, 10000 553 / 300, 20000 1732 / 728.
+                                         // 1 M values 10.8 us, with a launch of its own for that 11.5; 25 M (1500
+                                         // sums, read by 6000 workgroups): 140 and 136
+// Partial sums up to which every workgroup of the clipping launch adds them up itself: as many as a list has whose
+// tensors are few.  Every tensor brings at least one more, so for long lists the sums would be quadratic work.  us, each
+// workgroup / a launch of its own, norm included:
+//   246 tensors, 1968 sums, 207 MB   49.3 / 49.7
+//   tensors of 500 values            1000: 41.2 / 40.4   3000: 116 / 95   10000: 553 / 300   20000: 1732 / 728
 constexpr int CLIP_PARTS = MAX_CHUNKS;
 constexpr int SMALL_WAVES = 16;
 constexpr long long SMALL_CHUNK = 4096;  // bytes a wave takes at a time in the single-workgroup form
@@ -98,9 +99,9 @@ __device__ __forceinline__ Span span_of(const void* p, long long n, int esz, lon
   return s;
 }
 
-// Streaming accesses: what is read or written for the last time leaves no copy in the caches.  In front of a second pass
-// they keep the first one's bytes in the 256 MB memory-side cache: clipping 52 M fp32 values 142 -> 119 us (read and
-// written; read alone it stays at 144), the Adam update 404 -> 339 us; a norm alone, 2 GB of bf16, 335 -> 314 us.
+// Streaming accesses: what is read or written for the last time leaves no copy in the caches.  In front of a second
+// pass they keep the first one's bytes in the 256 MB memory-side cache: clipping 52 M fp32 values 142 -> 119 us (read
+// and written; read alone it stays at 144), the Adam update 404 -> 339 us; a norm alone, 2 GB of bf16, 335 -> 314 us.
 __device__ __forceinline__ u32x4 load_once(const void* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
 }
@@ -229,10 +230,10 @@ __device__ __forceinline__ float clip_factor(double norm, float max_norm) {
   return c >= 1. ? 1.f : (float)c;    // a NaN stays one
 }
 
-// Partial sums, a chunk a workgroup.  Bound by memory: 2 GB of bf16 in 310 us, 6.4 TB/s; 207 MB of fp32 whose first part
-// is still cached 39 us, 5.3 TB/s.
-// ONCE: nothing reads the tensors again behind it
-// step / next: where given, *next = *step + 1 on the way (see adam_clip_kernel)
+// Partial sums, a chunk a workgroup.  Bound by memory: 2 GB of bf16 in 310 us, 6.4 TB/s; 207 MB of fp32 whose first
+// part is still cached 39 us, 5.3 TB/s.
+//   ONCE         nothing reads the tensors again behind it
+//   step / next  where given, *next = *step + 1 on the way (see adam_clip_kernel)
 template <bool ONCE>
 __global__ __launch_bounds__(THR) void norm_chunks_kernel(const Table t, double* __restrict__ ws,
                                                           const int* __restrict__ step, int* __restrict__ next) {
@@ -262,10 +263,11 @@ __global__ __launch_bounds__(THR) void norm_total_kernel(double* __restrict__ ws
   if (threadIdx.x == 0) ws[0] = total;
 }
 
-// Every workgroup adds up the slots itself (out of L2, under the time of one more launch; n is 1 for a list whose tensors
-// are so many that norm_total_kernel has done it, CLIP_PARTS) and scales its chunk; with a factor of one there is nothing to do.  Chunks are taken from the last to the first: the
-// norm's pass left the end of the list in the caches (400 MB 192 us, from the first 200).  Bound by memory: norm and
-// clipping of 207 MB together 119 us, 5.2 TB/s of the 621 MB read and written.
+// Every workgroup adds up the slots itself (out of L2, under the time of one more launch; n is 1 for a list whose
+// tensors are so many that norm_total_kernel has done it, CLIP_PARTS) and scales its chunk; with a factor of one
+// there is nothing to do.  Chunks are taken from the last to the first: the norm's pass left the end of the list in
+// the caches (400 MB 192 us, from the first 200).  Bound by memory: norm and clipping of 207 MB together 119 us, 5.2
+// TB/s of the 621 MB read and written.
 __global__ __launch_bounds__(THR) void clip_chunks_kernel(const Table t, const double* __restrict__ ws, int n,
                                                           float max_norm, const float* __restrict__ scale,
                                                           float* __restrict__ out) {
@@ -309,8 +311,8 @@ struct AdamCfg {
   double b1d, b2d;
 };
 
-// The step's words from the sum of squares, by one thread: {norm, c / loss scale, learning rate / (1 - b1^t),
-// sqrt(1 - b2^t)}.  Returns whether there is a step: with a scaler a gradient that is not finite raises the flag, and the
+// The step's words from the sum of squares, by one thread:
+// {norm, c / loss scale, learning rate / (1 - b1^t), sqrt(1 - b2^t)}.  Returns whether there is a step: with a scaler a gradient that is not finite raises the flag, and the
 // count stays.  `step` is this step's number.
 struct AdamWords { float norm, factor, rate, root; };
 

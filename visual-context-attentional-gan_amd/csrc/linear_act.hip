@@ -24,10 +24,11 @@ enum { MODE_16 = 0, MODE_F32 = 1, MODE_S3 = 2, MODE_S1 = 3 };   // 16-bit tensor
 template <int MODE> struct ElemOf { typedef float T; };
 template <> struct ElemOf<MODE_16> { typedef vca_e16 T; };
 
-// What the value under the activation is kept in for the backward pass.  Its rounding enters dz next to dz's own, so it
-// has to be the smaller of the two: three more bits than bf16 in the same room, fp32 beside half.  Half's range is
-// narrower than bf16's at both ends.  At the upper one the slopes are 0, 1 or flat, an infinity included.  At the lower
-// one the smooth slopes are flat too, but the kinked ones turn on the sign, so a positive value stays positive (keep_z).
+// What the value under the activation is kept in for the backward pass.  Its rounding enters dz next to dz's own, so
+// it has to be the smaller of the two: three more bits than bf16 in the same room, fp32 beside half.  Half's range is
+// narrower than bf16's at both ends.  At the upper one the slopes are 0, 1 or flat, an infinity included.  At the
+// lower one the smooth slopes are flat too, but the kinked ones turn on the sign, so a positive value stays positive
+// (keep_z).
 #ifdef VCA_E16_FP16
 typedef float vca_z16;
 #else
@@ -61,10 +62,10 @@ template <typename T> union Vec16 {
 // ------------------------------------------------------------------------------------------------
 // activations, in fp32
 //
-// FULL, for fp32 tensors: the exponential is the library's and its argument's rounding is carried along, so that value and
-// slope are good to some 20 half ulps of their terms.  16-bit tensors, whose own rounding is 2^13 of those and more, take the
-// hardware's exponential: an argument k costs it some |k| half ulps.  (fp32 4800 x 512 -> 1280 with gelu, forward and all
-// gradients: 209 us, 205 with the hardware's.)
+// FULL, for fp32 tensors: the exponential is the library's, and gelu carries along what its argument's square loses, so
+// that value and slope are good to some 20 half ulps of their terms (the tanh form of gelu: and 6 of its exponent).
+// 16-bit tensors, whose own rounding is 2^13 of those and more, take the hardware's exponential: an argument k costs it
+// some |k| half ulps.  (fp32 4800 x 512 -> 1280 with gelu, forward and all gradients: 209 us, 205 with the hardware's.)
 // ------------------------------------------------------------------------------------------------
 constexpr float GELU_C = 0.7978845608028654f, GELU_A = 0.044715f;   // sqrt(2 / pi)
 
@@ -158,8 +159,9 @@ __device__ __forceinline__ void act_all(float (&v)[V], int act, float slope) {
 
 template <bool FULL>
 __device__ __forceinline__ float act_slope(float z, int act, float slope) {
-  // beyond +-200 the smooth activations' slopes are 0 or 1 to fp32's last subnormal; the clamp keeps 0 x infinity out of them.
-  // At a NaN they are one (it comes through the unclamped term), relu's is 1 and leaky's its slope, as torch's are.
+  // beyond +-200 the smooth activations' slopes are 0 or 1 to fp32's last subnormal; the clamp keeps 0 x infinity out
+  // of them.  At a NaN they are one (it comes through the unclamped term), relu's is 1 and leaky's its slope, as
+  // torch's are.
   const float c = fminf(fmaxf(z, -200.f), 200.f);
   float e;
   switch (act) {
@@ -269,13 +271,13 @@ __device__ __forceinline__ void finish(const MatArgs& g, int m, int n, float (&v
 // ------------------------------------------------------------------------------------------------
 // The tiled product.  A workgroup owns a BM x BN tile of C and walks the reduction in chunks of 128 bytes of a row
 // (64 16-bit or 32 fp32 elements) through two LDS stages (four where memory has to be waited for, see launch_layout):
-// chunk c + 1 travels while chunk c feeds the matrix cores, one barrier a chunk.  DMA: whole chunks go straight from memory
-// to LDS (16-byte pieces, operands 16-byte aligned); the reduction's last, partial chunk, and every chunk of operands of
-// another alignment, go through registers with masks.
+// chunk c + 1 travels while chunk c feeds the matrix cores, one barrier a chunk.  DMA: whole chunks go straight from
+// memory to LDS (16-byte pieces, operands 16-byte aligned); the reduction's last, partial chunk, and every chunk of
+// operands of another alignment, go through registers with masks.
 //
-// fp32 is bound by the matrix cores: 8192^3 at 139 TFLOP/s of the library's 154 (128-wide tiles); smaller ones lose to
-// tiles that do not divide over the CUs and to the ends of short reductions, 2400 x 2560 -> 512 64 us = 98 TFLOP/s.  16 bits with these tiles are bound by LDS and by the
-// wait for a chunk: 2048^3 29 us = 590 TFLOP/s.
+// fp32 is bound by the matrix cores: 8192^3 at 139 TFLOP/s of the library's 154 (128-wide tiles); smaller ones lose
+// to tiles that do not divide over the CUs and to the ends of short reductions, 2400 x 2560 -> 512 64 us = 98
+// TFLOP/s.  16 bits with these tiles are bound by LDS and by the wait for a chunk: 2048^3 29 us = 590 TFLOP/s.
 //
 // LDS images of an operand with R rows in the tile:
 //   k contiguous      [R][128 B], 16-byte pieces of a row XOR-ed with row & 7: the 16 rows a fragment load touches
@@ -376,7 +378,8 @@ struct Operand {
   }
 };
 
-// (The restrict gives the read alias information; without any the compiler waits for every LDS-DMA in flight before it.)
+// (The restrict gives the read alias information; without any the compiler waits for every LDS-DMA in flight before
+// it.)
 __device__ __forceinline__ s16x4 read_transposed(const char* __restrict__ p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
 }
@@ -444,9 +447,9 @@ __device__ __forceinline__ void tile_of(const MatArgs& g, int id, int total, int
   tn = t / rows;
 }
 
-// The end of a tile.  A split reduction stores its partial tile as it is.  Otherwise the accumulators pass through LDS
-// (fp32, 16-byte pieces of a row XOR-ed with the row) so that a thread finishes 16 bytes of a row of C and a wave writes
-// whole lines, in as many parts as the tile is larger than the LDS of the two stages.
+// The end of a tile.  A split reduction stores its partial tile as it is.  Otherwise the accumulators pass through
+// LDS (fp32, 16-byte pieces of a row XOR-ed with the row) so that a thread finishes 16 bytes of a row of C and a wave
+// writes whole lines, in as many parts as the tile is larger than the LDS of the two stages.
 template <typename T, int BM, int BN, int NWM, int NWN>
 __device__ __forceinline__ void store_tile(const MatArgs& g, const f32x4 (&acc)[BM / NWM / 16][BN / NWN / 16], char* smem,
                                            int m0, int n0, int kz, int wm, int wn, int lc, int lg, int tid) {
@@ -591,9 +594,9 @@ __device__ __forceinline__ void product_block(const MatArgs& g, int id, int tota
   };
 
   if (c0 < whole) {
-    // TURN: each tile starts at a chunk of its own.  Where every CU walks through its rows of W at the same column and the
-    // rows lie a power of two apart, few of the memory's channels are asked at a time (4096 -> 16384 in bf16, 8 rows 29.8 ->
-    // 25.8 us, 64 rows 31.6 -> 27.5; with less than half the CUs at work it changes nothing).
+    // TURN: each tile starts at a chunk of its own.  Where every CU walks through its rows of W at the same column
+    // and the rows lie a power of two apart, few of the memory's channels are asked at a time (4096 -> 16384 in bf16,
+    // 8 rows 29.8 -> 25.8 us, 64 rows 31.6 -> 27.5; with less than half the CUs at work it changes nothing).
     const int turn = TURN ? tn % (whole - c0) : 0;
     A.start();
     B.start();
@@ -606,8 +609,8 @@ __device__ __forceinline__ void product_block(const MatArgs& g, int id, int tota
     };
     for (int c = c0; c < min(whole, c0 + STAGES - 1); ++c) send(c);
     for (int c = c0; c < whole; ++c) {
-      // Chunk c has landed, in every wave behind the barrier: at most the STAGES - 2 chunks behind it are under way.  Every
-      // wave has left the stage that is sent to next, chunk c - 1's, with its reads done.
+      // Chunk c has landed, in every wave behind the barrier: at most the STAGES - 2 chunks behind it are under way.
+      // Every wave has left the stage that is sent to next, chunk c - 1's, with its reads done.
       if (STAGES > 2 && c + STAGES - 2 < whole) {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * (A.PIECES + B.PIECES)) : "memory");
       } else {
@@ -652,18 +655,19 @@ __global__ __launch_bounds__(256) void matmul_pair_kernel(const MatArgs x, const
 }
 
 // ------------------------------------------------------------------------------------------------
-// The tiled product for large 16-bit ones: 256 x 256 tiles, eight waves of 128 x 64 each, two to a SIMD, one workgroup to
-// a CU.  LDS carries 2 x 64 KB stages and feeds the waves 192 KB of fragments a chunk, under the time the matrix cores need
-// for it.  The waves overlap by themselves: while the 32 MFMAs of one half chunk run, the 12 fragments of the next half are
-// read (the second half of chunk c, then the first of chunk c + 1) and, in the second half, a piece of chunk c + 2 is sent
-// behind each row of MFMAs.  The chunk's only barrier sits in its middle: there every wave has its last fragments of chunk
-// c in registers, chunk c + 1 has landed (it was sent a whole chunk earlier), and chunk c's stage is free to be refilled.
+// The tiled product for large 16-bit ones: 256 x 256 tiles, eight waves of 128 x 64 each, two to a SIMD, one
+// workgroup to a CU.  LDS carries 2 x 64 KB stages and feeds the waves 192 KB of fragments a chunk, under the time
+// the matrix cores need for it.  The waves overlap by themselves: while the 32 MFMAs of one half chunk run, the 12
+// fragments of the next half are read (the second half of chunk c, then the first of chunk c + 1) and, in the second
+// half, a piece of chunk c + 2 is sent behind each row of MFMAs.  The chunk's only barrier sits in its middle: there
+// every wave has its last fragments of chunk c in registers, chunk c + 1 has landed (it was sent a whole chunk
+// earlier), and chunk c's stage is free to be refilled.
 //
 // Bound by the matrix cores: 8192^3 in bf16 at 1390 (x W^T), 1447 (dx) and 1465 TFLOP/s (dW), where the library's
-// product reaches 1485; with few chunks a tile the pipeline's ends show, 8192 x 4096 x 4096: 1270, 1300, 1408.  Tried and
-// slower: four waves of 128 x 128 (fewer fragment reads, but accumulators that do not fit the registers next to the
-// fragments: 459 us against 339), touching the next chunk's lines in L2, the barrier shifted by a quarter chunk, chunks
-// visited in an order that differs between tiles.
+// product reaches 1485; with few chunks a tile the pipeline's ends show, 8192 x 4096 x 4096: 1270, 1300, 1408.  Tried
+// and slower: four waves of 128 x 128 (fewer fragment reads, but accumulators that do not fit the registers next to
+// the fragments: 459 us against 339), touching the next chunk's lines in L2, the barrier shifted by a quarter chunk,
+// chunks visited in an order that differs between tiles.
 // ------------------------------------------------------------------------------------------------
 template <bool KC>
 struct WideOperand {
@@ -865,8 +869,8 @@ __device__ __forceinline__ void fold_bias(const BiasArgs& b, int block, float (*
   db[n] = (T)(b.add ? t + (float)db[n] : t);
 }
 
-// What is left to add up behind a forward pass (one product) or a backward pass (two products and the bias gradient), in
-// one launch: workgroups [0, first[1]) take product 0, [first[1], first[2]) product 1, the rest the bias gradient.
+// What is left to add up behind a forward pass (one product) or a backward pass (two products and the bias gradient),
+// in one launch: workgroups [0, first[1]) take product 0, [first[1], first[2]) product 1, the rest the bias gradient.
 struct FoldArgs {
   MatArgs g[2];
   BiasArgs b;
@@ -884,14 +888,14 @@ __global__ __launch_bounds__(256) void fold_kernel(const FoldArgs f) {
 
 // ------------------------------------------------------------------------------------------------
 // Few rows (M <= 16, both operands with k contiguous): the product reads W once and does next to nothing with it, so
-// there is no tile to share through LDS.  A workgroup owns 16 columns of C (and a range of the reduction where there are
-// few columns); each lane streams 16 bytes of a W row, and of an x row out of the caches, straight into an MFMA operand.
-// A wave takes two neighbouring chunks of 64 bytes at a time, so the line of each of its 16 rows is asked for by one wave
-// in a row (31 us against 35 with single chunks dealt out to the waves, 4096 -> 16384 in bf16, 8 rows), and the next two
-// fly under this pair's products.  More in flight (four chunks: 32 us), 32 columns a workgroup (34) or four waves (33)
-// were longer.  Bound by memory: 5.3 TB/s with one row, 4.9 with four (4096 -> 16384), whose x fragments pass through L2 as
-// well: with more rows the tiles above take over (FEW_BYTES).  The waves' partial tiles meet in LDS.  Rows of x beyond M
-// repeat the last one.
+// there is no tile to share through LDS.  A workgroup owns 16 columns of C (and a range of the reduction where there
+// are few columns); each lane streams 16 bytes of a W row, and of an x row out of the caches, straight into an MFMA
+// operand. A wave takes two neighbouring chunks of 64 bytes at a time, so the line of each of its 16 rows is asked
+// for by one wave in a row (31 us against 35 with single chunks dealt out to the waves, 4096 -> 16384 in bf16, 8
+// rows), and the next two fly under this pair's products.  More in flight (four chunks: 32 us), 32 columns a
+// workgroup (34) or four waves (33) were longer.  Bound by memory: 5.3 TB/s with one row, 4.9 with four (4096 ->
+// 16384), whose x fragments pass through L2 as well: with more rows the tiles above take over (FEW_BYTES).  The
+// waves' partial tiles meet in LDS.  Rows of x beyond M repeat the last one.
 // ------------------------------------------------------------------------------------------------
 constexpr int FEW_WAVES = 8, FEW_PAIR = 2, FEW_GROUP = FEW_WAVES * FEW_PAIR;
 
@@ -975,9 +979,11 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_rows_kernel(const MatArgs 
 }
 
 // ------------------------------------------------------------------------------------------------
-// dz = gy act'(z) and the columns' sums of it.  A workgroup takes a strip of 32 x 16 bytes of columns and a range of
-// rows (8 at a time); its column sums (of the unrounded dz, fp32) go to a slab, slabs are added in order.  Bound by memory:
-// 8192 x 4096 bf16, gelu: 39 us, 5.1 TB/s.
+// dz = gy act'(z) and the columns' sums of it.  dz is rounded to the tensors' type because it is an operand of the two
+// products behind it: the gradients of 16-bit layers carry its rounding beside their own (8192 x 4096 bf16: 0.0024 of
+// their size instead of 0.0017), and two operands for its high and low part would double those products.
+// A workgroup takes a strip of 32 x 16 bytes of columns and a range of rows (8 at a time); its column sums (of the unrounded dz, fp32) go to a slab, slabs are added in order.  Bound by
+// memory: 8192 x 4096 bf16, gelu: 39 us, 5.1 TB/s.
 // ------------------------------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void act_bwd_kernel(int M, int N, int act, float slope, const T* __restrict__ gy,
@@ -1054,24 +1060,31 @@ struct Plan {
   bool pair;                          // only the 64 x 64 tiles may
 };
 
-// Rows of x times bytes of W up to which few_rows_kernel takes a product of at most 16 rows: every workgroup of 16 columns
-// reads x again, a tile of 64 columns a quarter of that.  us, few_rows_kernel and tiles: bf16 4096 -> 16384, 1 row
-// 25.1 / 26.2, 4 rows 27.6 / 26, 8 rows 31 / 25.8, 16 rows 39 / 26; 4096 -> 4096, 8 rows 10.2 / 11.9; fp32 4096 -> 4096,
-// 16 rows 25 / 21; 512 -> 512, 16 rows 4.2 / 6.6.
+// Rows of x times bytes of W up to which few_rows_kernel takes a product of at most 16 rows: every workgroup of 16
+// columns reads x again, a tile of 64 columns a quarter of that.  us, few_rows_kernel and tiles: bf16 4096 -> 16384,
+// 1 row 25.1 / 26.2, 4 rows 27.6 / 26, 8 rows 31 / 25.8, 16 rows 39 / 26; 4096 -> 4096, 8 rows 10.2 / 11.9; fp32 4096
+// -> 4096, 16 rows 25 / 21; 512 -> 512, 16 rows 4.2 / 6.6.
 constexpr double FEW_BYTES = 500e6;
 constexpr int LOW_ROWS = 128;         // see launch_layout
 
-// Tile and split of a product, by the time the candidates would take.  A tile's chunk costs a CU `work` us of its matrix
-// cores; a workgroup that has a CU to itself cannot go below `wait` us a chunk (LDS and memory latency, one barrier a
-// chunk), a CU with r workgroups takes max(wait, r work), and all of them together no less than the operands' trip from
-// memory.  `ends`: filling the pipeline and storing the tile.  A split adds one launch and a pass over the partial products.
-// Fitted to launches of 2 to 2000 us on this part; the choice is within some 10 % of the best one measured at each.  Where
-// sides change (us): fp32 8192 x 4096, K 4096: 64-wide tiles 2349, 128 2043.  16 bits 2048^3: 64 29, 128 30, 256 39 (split);
-// 4800 x 2560, K 5120: 197, 137, 112; 64 x 4096, K 4096: 64-wide unsplit 23, split four ways 13.  Up to 32 rows tiles of
-// 32 x 64, against 64 x 64: 32 x 4096 -> 4096 12.2 / 13.5, fp32 21.3 / 25.8.  Tall tiles of fp32 products, whose counts fall
-// between those of the square ones: 4800 x 512 -> 1280 128 x 64 63 / 64 x 64 69; 4800 x 1280 -> 512 80 x 64 62 / 73;
-// 900 x 700 -> 1300 23 / 29; 2400 x 2560 -> 512 160 x 64 split four ways 65 / 128 x 128 split three ways 68; but
-// 1500 x 2048 -> 2048 80 x 64 147 / 114.  (In 16 bits they gain 2 us at the most: 4800 x 512 -> 1280 11.9 / 13.6.)
+// Tile and split of a product, by the time the candidates would take.  A tile's chunk costs a CU `work` us of its
+// matrix cores; a workgroup that has a CU to itself cannot go below `wait` us a chunk (LDS and memory latency, one
+// barrier a chunk), a CU with r workgroups takes max(wait, r work), and all of them together no less than the
+// operands' trip from memory.  `ends`: filling the pipeline and storing the tile.  A split adds one launch and a pass
+// over the partial products.
+// The four numbers of each tile were fitted to launches of 2 to 2000 us on this part; the choice is within some 10 % of
+// the best one measured at each.  Where sides change (us):
+//   fp32 8192 x 4096 <- 4096       64 wide 2349, 128 wide 2043
+//   fp32 tall tiles                4800 x 1280 <- 512    128 x 64  63, 64 x 64  69
+//                                  4800 x 512 <- 1280     80 x 64  62, 64 x 64  73
+//                                  900 x 1300 <- 700      tall     23, 64 x 64  29
+//                                  2400 x 512 <- 2560    160 x 64 split four ways 65, 128 x 128 split three ways 68
+//                                  but 1500 x 2048 <- 2048  80 x 64 147, 64 x 64 114
+//   16 bits 2048^3                 64 wide 29, 128 wide 30, 256 wide 39 (split)
+//   16 bits 4800 x 2560 <- 5120    64 wide 197, 128 wide 137, 256 wide 112
+//   16 bits 64 x 4096 <- 4096      64 wide 23, the same split four ways 13
+//   16 bits 4800 x 1280 <- 512     tall tiles 11.9, 64 wide 13.6: too little for forms of their own
+//   32 x 4096 <- 4096              32 x 64 tiles 12.2, 64 x 64 13.5; fp32 21.3 and 25.8
 struct TileCost { int bm, bn; double work, wait, ends; };
 constexpr TileCost COST[4][6] = {
     {{256, 256, 1.55, 1.55, 8.}, {128, 128, 0.53, 0.85, 2.}, {64, 64, 0.20, 0.45, 0.8}, {32, 64, 0.12, 0.24, 2.}},   // 16 bits
@@ -1087,7 +1100,9 @@ bool pick(Plan& p, int nc) {
   double best = 0.;
   p.bm = 0;
   for (const TileCost& t : COST[p.mode]) {
-    if (!t.bm || (p.pair && t.bm != 64) || (t.bm == 256 && !p.wide) || (t.bm == 32 && !(p.low && g.M <= 32)) || (t.bm > t.bn && !p.tall)) continue;
+    if (!t.bm || (p.pair && t.bm != 64) || (t.bm == 256 && !p.wide) || (t.bm == 32 && !(p.low && g.M <= 32)) ||
+        (t.bm > t.bn && !p.tall))
+      continue;
     const long long tiles = ((g.M + (long long)t.bm - 1) / t.bm) * ((g.N + (long long)t.bn - 1) / t.bn);
     if (tiles >= (1 << 24)) continue;
     const double wait = t.wait * (p.low && g.M <= 64 && t.bm == 64 && p.mode == MODE_16 ? 0.75 : 1.);   // (four stages)
@@ -1145,9 +1160,10 @@ int plan_of(const vca_matmul_desc* dp, const void* a, const void* b, Plan& p, bo
   const double wbytes = (double)d.N * d.K * esz;
   if (d.M <= 16 && d.N <= (1 << 26) && !d.a_col && !d.b_col && (p.mode == MODE_16 || p.mode == MODE_F32) &&
       d.M * wbytes <= FEW_BYTES) {
-    // A workgroup streams its 16 rows of W at some 30 GB/s, all of them at most at 5 TB/s; where columns alone give too few
-    // of them to load the memory, the reduction is split too, if that saves more than the launch that adds the parts (one
-    // row, split and unsplit: bf16 16384 -> 1024 12.9 / 21.7 us, fp32 2560 -> 512 7.2 / 9.6, fp32 4096^2 21.2 / 20.3).
+    // A workgroup streams its 16 rows of W at some 30 GB/s, all of them at most at 5 TB/s; where columns alone give
+    // too few of them to load the memory, the reduction is split too, if that saves more than the launch that adds
+    // the parts (one row, split and unsplit: bf16 16384 -> 1024 12.9 / 21.7 us, fp32 2560 -> 512 7.2 / 9.6, fp32
+    // 4096^2 21.2 / 20.3).
     p.bm = 0;
     const int nc = (d.K * esz + 63) / 64, blocks = (d.N + 15) / 16;
     double best = 0.;
@@ -1203,10 +1219,10 @@ int launch_layout(const Plan& p, hipStream_t s) {
     return p.dma ? launch_kernel<MODE, AKC, BKC, 128, 128, 2, true, 2>(p, s)
                  : launch_kernel<MODE, AKC, BKC, 128, 128, 2, false, 2>(p, s);
   if (!p.dma) return launch_kernel<MODE, AKC, BKC, 64, 64, 2, false, 2>(p, s);
-  // Up to 128 rows the weights come from memory, not from another workgroup's lines in L2: three chunks under way instead
-  // of one (16 bits 4096 -> 16384, 64 rows: 38 us against 40, 128: 48 against 56; fp32 4096^2, 64: 28 against 32).  Larger
-  // products only lose workgroups a CU by it (2000 x 2048 -> 512: 15.5 against 14.9), column-major operands too
-  // (64 x 4096 x 4096, dx: 15.5 against 13.6).
+  // Up to 128 rows the weights come from memory, not from another workgroup's lines in L2: three chunks under way
+  // instead of one (16 bits 4096 -> 16384, 64 rows: 38 us against 40, 128: 48 against 56; fp32 4096^2, 64: 28 against
+  // 32).  Larger products only lose workgroups a CU by it (2000 x 2048 -> 512: 15.5 against 14.9), column-major
+  // operands too (64 x 4096 x 4096, dx: 15.5 against 13.6).
   if constexpr (AKC && BKC) {
     if (p.low)
       return turn ? launch_kernel<MODE, true, true, 64, 64, 2, true, 4, true>(p, s)
@@ -1284,17 +1300,17 @@ int launch_product(Plan& p, const vca_matmul_desc& d, const void* a, const void*
 
 int grid_of(const Plan& p) { return p.g.ntm * p.g.ntn * p.g.ksplit; }
 
-// Whether both products of a backward pass go by one launch, side by side instead of one after the other (us, one launch and
-// two, with dz and db: bf16 300 x 512 x 512 11.6 / 16.2, 1801 x 1111 x 677 43 / 57; fp32 1000^3 52 / 63, 5000 x 1111 x 1333
-// 377 / 373).
+// Whether both products of a backward pass go by one launch, side by side instead of one after the other (us, one
+// launch and two, with dz and db: bf16 300 x 512 x 512 11.6 / 16.2, 1801 x 1111 x 677 43 / 57; fp32 1000^3 52 / 63,
+// 5000 x 1111 x 1333 377 / 373).
 bool in_pair(const Plan& x, const Plan& w) {
   return x.bm == 64 && x.bn == 64 && w.bm == 64 && w.bn == 64 && x.dma == w.dma && grid_of(x) <= (1 << 22) &&
          grid_of(w) <= (1 << 22);
 }
 
-// Plans of both.  Other tiles are given up for one launch if the whole of it fits the CUs at once (600^3 fp32 27.3 -> 23.6;
-// 4800 x 512 x 1280, 1080 workgroups, would go 137 -> 157).  Both products are always planned, wanted or not, so that dx
-// does not depend on whether dW is formed too.
+// Plans of both.  Other tiles are given up for one launch if the whole of it fits the CUs at once (600^3 fp32 27.3 ->
+// 23.6; 4800 x 512 x 1280, 1080 workgroups, would go 137 -> 157).  Both products are always planned, wanted or not,
+// so that dx does not depend on whether dW is formed too.
 int plan_pair(const vca_linear_bwd& b, const vca_matmul_desc& x, const vca_matmul_desc& w, const void* dz, Plan& px, Plan& pw) {
   const int ex = plan_of(&x, dz, b.w, px), ew = plan_of(&w, dz, b.x, pw);
   if (ex && b.dx) return ex;
