@@ -526,7 +526,8 @@ int vca_loss_scale_update(float* scale, int* state, float growth, float backoff,
  * A(m, k) = a[m lda + k] or, with a_col, a[k lda + m]; B(n, k) = b[n ldb + k] or, with b_col, b[k ldb + n]; res and c have
  * row strides ldr and ldc (all in elements; ldr may be 0).  y = x W^T: neither; dx = dz W: b_col; dW = dz^T x: both.
  * Any sizes and strides, pointers aligned to their element.  bias, res, z may be NULL; z [M][N] receives the value
- * under the activation (for the backward pass): fp32, for bf16 tensors half.  res may be c: the product is added to it.
+ * under the activation (for the backward pass): fp32, for bf16 tensors half (where relu or leaky read its sign, a positive
+ * one at least half's smallest).  res may be c: the product is added to it.
  * type: VCA_T_F32, or the 16-bit type of this build (vca_elem_type).  nsplit: products per element pair, 1 for 16-bit
  * tensors; fp32 tensors 0 (exact fp32 MFMA), 3 or 1 (split into / rounded to 16 bits in registers).
  * act: 0 none, 1 leaky (slope), 3 relu, 4 tanh, 5 gelu (erf), 6 gelu (tanh form), 7 silu.
