@@ -837,8 +837,8 @@ def _rows_2d(t, broadcast=False):
 
 
 _ELEM_OF = {torch.float32: None, torch.bfloat16: 'bf16', torch.float16: 'fp16'}   # 16-bit products are compiled per type
-# what the value under the activation is kept in: rounded less than dz, next to whose rounding its own comes (half keeps the
-# sign of every bf16 value that relu or leaky's slope turns on: the kernels lift a positive one to half's smallest)
+# what the value under the activation is kept in: rounded less than dz, next to whose rounding its own comes (half keeps
+# the sign of every bf16 value that relu or leaky's slope turns on: the kernels lift a positive one to half's smallest)
 _KEPT_IN = {torch.float32: torch.float32, torch.bfloat16: torch.float16, torch.float16: torch.float32}
 _act_ws = {}     # sizes and types of a forward or backward pass -> workspace floats
 _ACT_WS_KEPT = 4096     # of them: batches with a row count of their own every step would never stop adding
@@ -979,8 +979,8 @@ def linear_act(x, w, bias=None, act=None, residual=None):
     x2, w2 = _rows_2d(x), _rows_2d(w)
     b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     r = None if residual is None else _rows_2d(residual, True)
-    # Forward-mode derivatives (refused by the autograd function: no tangent may get lost) and torch.jit.trace see a call only
-    # where it goes through the function; without either, inference saves its 3 us of 12 (one row).
+    # Forward-mode derivatives (refused by the autograd function: no tangent may get lost) and torch.jit.trace see a call
+    # only where it goes through the function; without either, inference saves its 3 us of 12 (one row).
     if (torch.is_grad_enabled() and any([t.requires_grad for t in tensors]) or forward_ad._current_level >= 0 or
             torch._C._get_tracing_state() is not None):
         y = LinearActFn.apply(x2, w2, b, r, code)

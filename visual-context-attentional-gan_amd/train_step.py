@@ -149,7 +149,8 @@ class GanStep:
         self.scaler = scaler
         pair = max_norm if isinstance(max_norm, (tuple, list)) else (max_norm, max_norm)
         if len(pair) != 2:
-            raise ValueError('GanStep: max_norm is a number or a pair (generator side, discriminator side), got %r' % (max_norm,))
+            raise ValueError('GanStep: max_norm is a number or a pair (generator side, discriminator side), got %r'
+                             % (max_norm,))
         self.g_max_norm, self.d_max_norm = (None if v is None else ops._max_norm(v) for v in pair)
         if dist.is_available() and dist.is_initialized():
             ops.set_seed(torch.initial_seed(), dist.get_rank(group))   # each replica draws its own dropout masks
@@ -189,8 +190,8 @@ class GanStep:
         ops.join_side_streams()
 
     def _update(self, opt, side, max_norm):
-        """One side's optimizer step; its gradients' norm where they are clipped.  Without clipping the optimizer is called as
-        ever, step(scaler, side), so one that knows nothing of max_norm goes on working."""
+        """One side's optimizer step; its gradients' norm where they are clipped.  Without clipping the optimizer is called
+        as ever, step(scaler, side), so one that knows nothing of max_norm goes on working."""
         if max_norm is not None:
             return opt.step(self.scaler, side, max_norm)
         opt.step(self.scaler, side)
